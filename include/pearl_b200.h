@@ -469,6 +469,167 @@ typedef struct pb2_grouped_gemm_params {
 } pb2_grouped_gemm_params;
 PB2_API int pb2_noisy_gemm_grouped(const pb2_grouped_gemm_params* p, void* stream);
 
+/* -------------------------------------------- the un-mined layer operators --
+ * No reference counterpart (its vLLM plugin takes these from vLLM): what
+ * stands around the products in a quantized linear or MoE layer.  Each is
+ * asynchronous on `stream`, allocates nothing and reads every argument's
+ * device memory only on the device, so all can be captured in a CUDA graph. */
+#define PB2_TYPE_F32 0
+#define PB2_TYPE_BF16 1
+#define PB2_TYPE_F16 2
+#define PB2_ACT_NONE 0
+#define PB2_ACT_RELU 1
+#define PB2_ACT_SILU 2      /* x / (1 + e^-x) */
+#define PB2_ACT_GELU 3      /* x Phi(x) */
+#define PB2_ACT_GELU_TANH 4 /* x (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))) / 2 */
+
+/* route_tokens: the experts of every token.
+ *   s = softmax of the row's logits, or 1 / (1 + e^-x) of each (f32);
+ *   the choice goes by s + bias[e], or without a bias by the logits (both
+ *   scores grow with them);
+ *   num_groups > 1: only experts of the topk_groups best groups (of
+ *   num_experts / num_groups experts each) take part; a group's value is its
+ *   highest expert's, with a bias the sum of its two highest;
+ *   topk_ids[t] = the top_k experts in descending order, ties to the lowest
+ *   index (also between groups);
+ *   topk_weights[t] = s of those experts (without the bias), divided by
+ *   their sum when `renormalize`, times `scaling`.
+ * A logit of -inf or NaN masks its expert: s = 0, chosen after every other
+ * expert that takes part.  A row that masks every expert gets weights 0, and
+ * +inf logits of a softmax share the row alike.  num_experts <= 256,
+ * top_k <= 32, top_k <= topk_groups * num_experts / num_groups. */
+#define PB2_SCORE_SOFTMAX 0
+#define PB2_SCORE_SIGMOID 1
+typedef struct pb2_route_params {
+  int device;
+  const void* logits; /* (num_tokens, num_experts) of logits_type */
+  int logits_type;    /* PB2_TYPE_* */
+  int64_t num_tokens, num_experts, top_k;
+  int scoring;        /* PB2_SCORE_* */
+  const float* bias;  /* (num_experts), optional */
+  int64_t num_groups, topk_groups;
+  int renormalize;
+  float scaling;
+  float* topk_weights; /* (num_tokens, top_k) */
+  int32_t* topk_ids;   /* (num_tokens, top_k) */
+} pb2_route_params;
+PB2_API int pb2_route_tokens(const pb2_route_params* p, void* stream);
+
+/* gemm_epilogue: C = act(A_scales * B_scales * (A . B^T) + bias) + residual,
+ * the sum of products exact in int32, the rest in f32, rounded to C's type
+ * once.  A (m,k), B (n,k) int8, 16-byte aligned, k % 16 == 0; any m and n
+ * (rows of C move 16 bytes at a time when n % 8 == 0 and C and residual are
+ * 16-byte aligned).  residual may be C.  host_signal_sync (optional, as for
+ * pb2_gemm) receives PB2_ERR_DEVICE_TIMEOUT in its error word. */
+typedef struct pb2_gemm_epilogue_params {
+  int device;
+  int64_t m, n, k;
+  const int8_t* A;
+  const int8_t* B;
+  const float* A_scales; /* (m) */
+  const float* B_scales; /* (n) */
+  void* C;               /* (m,n) of c_type */
+  int c_type;            /* PB2_TYPE_BF16 or PB2_TYPE_F16 */
+  const void* bias;      /* (n), optional */
+  int bias_type;         /* PB2_TYPE_F32 or c_type */
+  int activation;        /* PB2_ACT_* */
+  const void* residual;  /* (m,n) of c_type, optional */
+  void* host_signal_sync;
+} pb2_gemm_epilogue_params;
+PB2_API int pb2_gemm_epilogue(const pb2_gemm_epilogue_params* p, void* stream);
+
+/* quantize_gated: row i of xq = the quantized act(g) * u of row
+ * row_index[i] (row i without an index) of x, whose rows hold n gate values
+ * and then n up values:
+ *   v = act(g) * u, Hadamard transform of width block_size (as pb2_quantize,
+ *   0 = none), times smooth (n), in f32;
+ *   scales[i] = max|v| * fl(1 / max_val), xq = rint(v * (max_val / max|v|))
+ *   clamped to +-max_val (0 for a row of zeros).
+ * x_rows is the number of rows of x; an index outside it gives a row of
+ * zeros.  n % 8 == 0, x and smooth 16-byte and xq 8-byte aligned. */
+typedef struct pb2_gated_quant_params {
+  int device;
+  const void* x; /* (x_rows, 2 n) of x_type */
+  int x_type;    /* PB2_TYPE_BF16 or PB2_TYPE_F16 */
+  int64_t m, n, x_rows;
+  int activation;           /* PB2_ACT_* */
+  const int32_t* row_index; /* (m), optional */
+  const float* smooth;      /* (n), optional */
+  int8_t* xq;               /* (m,n) */
+  float* scales;            /* (m) */
+  int max_val;
+  int block_size;
+} pb2_gated_quant_params;
+PB2_API int pb2_quantize_gated(const pb2_gated_quant_params* p, void* stream);
+
+/* gemm_grouped: the un-mined product of every expert of a layer.  Rows of A
+ * (m,k) in expert order (as for pb2_noisy_gemm_grouped), expert e's ending at
+ * routing_offsets[e] (pb2_build_routing_data's, read on the device; clamped
+ * to [0, m]); B (num_experts, n, k), B_scales (num_experts, n);
+ *   C[row] = A_scales[row] * B_scales[e] * (A[row] . B[e]^T),
+ * written to row c_row_index[row] of C's c_rows rows when the index is given
+ * (rows outside are skipped).  Rows past the last expert's end are not
+ * written.  num_experts <= 256; types, alignment and host_signal_sync as for
+ * pb2_gemm_epilogue. */
+typedef struct pb2_gemm_grouped_params {
+  int device;
+  int64_t m, n, k;
+  const int8_t* A;
+  const int8_t* B;
+  const float* A_scales;
+  const float* B_scales;
+  void* C;
+  int c_type;
+  int64_t num_experts;
+  const int32_t* routing_offsets; /* (num_experts) */
+  const int32_t* c_row_index;     /* (m), optional */
+  int64_t c_rows;
+  void* host_signal_sync;
+} pb2_gemm_grouped_params;
+PB2_API int pb2_gemm_grouped(const pb2_gemm_grouped_params* p, void* stream);
+
+/* combine_slots: out[t] = residual[t] + sum over j of topk_weights[t, j] *
+ * slots[t * top_k + j], f32 sums in the order of j, rounded once.  A slot
+ * whose weight is 0 is not read.  residual may be out. */
+typedef struct pb2_combine_params {
+  int device;
+  const void* slots;         /* (num_tokens * top_k, n) of type */
+  const float* topk_weights; /* (num_tokens, top_k) */
+  const void* residual;      /* (num_tokens, n), optional */
+  void* out;                 /* (num_tokens, n) */
+  int type;                  /* PB2_TYPE_BF16 or PB2_TYPE_F16 */
+  int64_t num_tokens, top_k, n;
+} pb2_combine_params;
+PB2_API int pb2_combine_slots(const pb2_combine_params* p, void* stream);
+
+/* gated_experts: the second half of the experts' MLP in one call:
+ * quantize_gated of x (slots = num_tokens * top_k rows in slot order) into
+ * expert order (slot_indices), gemm_grouped with w back to slot order,
+ * combine_slots.  workspace: pb2_gated_experts_workspace_bytes(slots, inner,
+ * hidden) bytes, 16-byte aligned.  The slots' products are rounded to `type`
+ * between the last two steps. */
+typedef struct pb2_gated_experts_params {
+  int device;
+  const void* x; /* (slots, 2 inner) of type */
+  int type;      /* PB2_TYPE_BF16 or PB2_TYPE_F16 */
+  int64_t num_tokens, top_k, num_experts, inner, hidden;
+  int activation;
+  const float* smooth; /* (inner), optional */
+  int max_val, block_size;
+  const int8_t* w;       /* (num_experts, hidden, inner) */
+  const float* w_scales; /* (num_experts, hidden) */
+  const int32_t* slot_indices;    /* (slots) */
+  const int32_t* routing_offsets; /* (num_experts) */
+  const float* topk_weights;      /* (num_tokens, top_k) */
+  const void* residual;           /* (num_tokens, hidden), optional */
+  void* out;                      /* (num_tokens, hidden) */
+  void* workspace;
+  int64_t workspace_bytes;
+  void* host_signal_sync;
+} pb2_gated_experts_params;
+PB2_API int pb2_gated_experts(const pb2_gated_experts_params* p, void* stream);
+PB2_API int64_t pb2_gated_experts_workspace_bytes(int64_t slots, int64_t inner, int64_t hidden);
+
 /* ------------------------------------------- noisy_gemm, static scratch ---
  * No counterpart in the reference.  The same mined GEMM as pb2_noisy_gemm,
  * for callers that cannot allocate device memory: a host that only reaches

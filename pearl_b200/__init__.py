@@ -38,6 +38,8 @@ from .pearl_gemm_interface import (
     noisy_gemm,
     tensor_hash,
 )
+from .linear import gemm_epilogue
+from . import linear
 from . import moe
 from . import quantization
 from . import device_waits
@@ -57,11 +59,13 @@ __all__ = [
     "denoise_converter",
     "extract_indices",
     "gemm",
+    "gemm_epilogue",
     "get_host_signal_header",
     "get_host_signal_header_size",
     "get_host_signal_sync_fields",
     "get_host_signal_sync_size",
     "inner_hash",
+    "linear",
     "moe",
     "quantization",
     "device_waits",

@@ -36,6 +36,8 @@ EXPORTED = [
     "pb2_build_routing_data_scratchpad_bytes", "pb2_quantize", "pb2_scatter_rows",
     "pb2_merkle_layers", "pb2_merkle_nodes", "pb2_set_wait_budget_cycles", "pb2_wait_selftest",
     "pb2_rcp_approx_f32", "pb2_noisy_gemm_grouped", "pb2_mined_gemm_fp8",
+    "pb2_route_tokens", "pb2_gemm_epilogue", "pb2_quantize_gated", "pb2_gemm_grouped", "pb2_combine_slots",
+    "pb2_gated_experts", "pb2_gated_experts_workspace_bytes",
 ]
 DEFAULT_WAIT_BUDGET_CYCLES = 2000000000
 
@@ -136,6 +138,46 @@ class ScatterParams(ctypes.Structure):
                 ("dst_rows", _i64), ("row_bytes", _i64)]
 
 
+class RouteParams(ctypes.Structure):
+    _fields_ = [("device", ctypes.c_int), ("logits", _vp), ("logits_type", ctypes.c_int), ("num_tokens", _i64),
+                ("num_experts", _i64), ("top_k", _i64), ("scoring", ctypes.c_int), ("bias", _vp),
+                ("num_groups", _i64), ("topk_groups", _i64), ("renormalize", ctypes.c_int),
+                ("scaling", ctypes.c_float), ("topk_weights", _vp), ("topk_ids", _vp)]
+
+
+class GemmEpilogueParams(ctypes.Structure):
+    _fields_ = [("device", ctypes.c_int), ("m", _i64), ("n", _i64), ("k", _i64), ("A", _vp), ("B", _vp),
+                ("A_scales", _vp), ("B_scales", _vp), ("C", _vp), ("c_type", ctypes.c_int), ("bias", _vp),
+                ("bias_type", ctypes.c_int), ("activation", ctypes.c_int), ("residual", _vp),
+                ("host_signal_sync", _vp)]
+
+
+class GatedQuantParams(ctypes.Structure):
+    _fields_ = [("device", ctypes.c_int), ("x", _vp), ("x_type", ctypes.c_int), ("m", _i64), ("n", _i64),
+                ("x_rows", _i64), ("activation", ctypes.c_int), ("row_index", _vp), ("smooth", _vp), ("xq", _vp),
+                ("scales", _vp), ("max_val", ctypes.c_int), ("block_size", ctypes.c_int)]
+
+
+class GemmGroupedParams(ctypes.Structure):
+    _fields_ = [("device", ctypes.c_int), ("m", _i64), ("n", _i64), ("k", _i64), ("A", _vp), ("B", _vp),
+                ("A_scales", _vp), ("B_scales", _vp), ("C", _vp), ("c_type", ctypes.c_int), ("num_experts", _i64),
+                ("routing_offsets", _vp), ("c_row_index", _vp), ("c_rows", _i64), ("host_signal_sync", _vp)]
+
+
+class CombineParams(ctypes.Structure):
+    _fields_ = [("device", ctypes.c_int), ("slots", _vp), ("topk_weights", _vp), ("residual", _vp), ("out", _vp),
+                ("type", ctypes.c_int), ("num_tokens", _i64), ("top_k", _i64), ("n", _i64)]
+
+
+class GatedExpertsParams(ctypes.Structure):
+    _fields_ = [("device", ctypes.c_int), ("x", _vp), ("type", ctypes.c_int), ("num_tokens", _i64), ("top_k", _i64),
+                ("num_experts", _i64), ("inner", _i64), ("hidden", _i64), ("activation", ctypes.c_int),
+                ("smooth", _vp), ("max_val", ctypes.c_int), ("block_size", ctypes.c_int), ("w", _vp),
+                ("w_scales", _vp), ("slot_indices", _vp), ("routing_offsets", _vp), ("topk_weights", _vp),
+                ("residual", _vp), ("out", _vp), ("workspace", _vp), ("workspace_bytes", _i64),
+                ("host_signal_sync", _vp)]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -157,7 +199,9 @@ def load() -> ctypes.CDLL:
                      "pb2_noisy_gemm", "pb2_gemm", "pb2_noisy_gemm_static_scratch", "pb2_noisy_gemm_grouped",
                      "pb2_mined_gemm_fp8",
                      "pb2_tensor_hash", "pb2_commitment_hash_from_merkle_roots",
-                     "pb2_build_routing_data", "pb2_quantize", "pb2_scatter_rows", "pb2_merkle_layers"):
+                     "pb2_build_routing_data", "pb2_quantize", "pb2_scatter_rows", "pb2_merkle_layers",
+                     "pb2_route_tokens", "pb2_gemm_epilogue", "pb2_quantize_gated", "pb2_gemm_grouped",
+                     "pb2_combine_slots", "pb2_gated_experts"):
             getattr(L, name).restype = ctypes.c_int
             getattr(L, name).argtypes = [ctypes.c_void_p, ctypes.c_void_p]
         L.pb2_noise_AB.restype = ctypes.c_int
@@ -172,6 +216,8 @@ def load() -> ctypes.CDLL:
         L.pb2_required_scratchpad_bytes.argtypes = [_i64, ctypes.c_int]
         L.pb2_gemm_workspace_bytes.restype = _i64
         L.pb2_gemm_workspace_bytes.argtypes = [ctypes.c_int, _i64, _i64, _i64]
+        L.pb2_gated_experts_workspace_bytes.restype = _i64
+        L.pb2_gated_experts_workspace_bytes.argtypes = [_i64, _i64, _i64]
         L.pb2_host_signal_header_size.restype = _i64
         L.pb2_host_signal_sync_size.restype = _i64
         L.pb2_status_string.restype = ctypes.c_char_p

@@ -1,0 +1,651 @@
+// product.cu -- int8 products with an epilogue: the linear layer
+//   C = act(sA[m] * sB[n] * (A . B^T) + bias[n]) + residual
+// and the experts' product of a MoE layer, whose rows are grouped by expert
+// and multiplied by their expert's weights, with the group boundaries read on
+// the device.
+//
+// One persistent CTA per SM walks 128 x 128 output tiles: a TMA warp fills a
+// ring of 128-byte K stages, a warp issues the tcgen05 int8 MMAs, and eight
+// epilogue warps turn one accumulator into C while the other one (both in
+// tensor memory) is being filled.  int32 sums are exact; the epilogue works
+// in f32 and rounds once.
+#include <algorithm>
+#include <cstring>
+
+#include "pb2_epilogue.cuh"
+
+namespace pb2 {
+namespace {
+
+constexpr int kTileRows = 128;  // rows of C per CTA
+constexpr int kTileK = 128;     // bytes of K per stage
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 32 * (2 + kEpiWarps);
+constexpr int kMaxStages = 10;
+constexpr int kBoxBytes = 32 * 128;  // an epilogue warp's 32 rows x 64 16-bit columns
+constexpr int kMaxGroups = 256;
+
+enum { kBiasNone = 0, kBiasF32 = 1, kBiasHalf = 2 };  // kBiasHalf: C's type
+
+struct ProductArgs {
+  CUtensorMap tmA;  // A (rows, K) int8
+  CUtensorMap tmB;  // B (groups * N, K) int8
+  const float* sA;
+  const float* sB;
+  void* C;
+  const void* bias;
+  const void* residual;
+  int c_f16, bias_kind, act;
+  int M, N, K;
+  int tiles_n, raster;
+  int groups;              // 0: one product of M rows
+  const int32_t* ends;     // groups: end row of each group
+  const int32_t* c_rows;   // optional: row r of the product goes to row c_rows[r] of C
+  long long c_dst_rows;
+  int a_bytes, stages;     // A bytes of a stage; stages in the ring
+  int vec;                 // rows of C and residual can be moved 16 bytes at a time
+  SignalSync* sync;
+  long long wait_budget;
+  uint32_t wait_hint_ns;
+};
+
+struct ProductSmem {
+  uint64_t full[kMaxStages];
+  uint64_t empty[kMaxStages];
+  uint64_t acc_full[2];
+  uint64_t acc_empty[2];
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort_flag;
+  int tile0[kMaxGroups + 1];  // first tile of each group
+  int row0[kMaxGroups + 1];   // first row of each group
+};
+
+struct Tile {
+  int group;  // of B and sB
+  int row0;   // first row of A
+  int rows;   // rows of the group from row0 on (may exceed the tile)
+  int tn;
+};
+
+// Tile t: groups follow one another; inside one, `raster` row tiles walk all
+// column tiles before the next row tiles, so B tiles are read by neighbours.
+template <bool kGrouped, int kRows>
+__device__ __forceinline__ Tile tile_at(const ProductArgs& a, const ProductSmem& S, int t) {
+  int g = 0, first = 0, rows = a.M, lt = t;
+  if constexpr (kGrouped) {
+    int lo = 0, hi = a.groups;  // the last group whose first tile is <= t
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (S.tile0[mid] <= t) lo = mid; else hi = mid;
+    }
+    g = lo;
+    first = S.row0[g];
+    rows = S.row0[g + 1] - first;
+    lt = t - S.tile0[g];
+  }
+  const int tiles_m = (rows + kRows - 1) / kRows;
+  const int span = min(a.raster, tiles_m);
+  const int block = lt / (span * a.tiles_n);
+  const int m0 = block * span;
+  const int mm = min(span, tiles_m - m0);
+  const int in = lt - block * span * a.tiles_n;
+  const int tm = m0 + in % mm;
+  return Tile{g, first + tm * kRows, rows - tm * kRows, in / mm};
+}
+
+// One stage of 1-SM int8 MMAs (128 bytes of K) and its commit, from one
+// elected lane.
+__device__ __forceinline__ void umma_i8_stage_warp(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc,
+                                                   uint32_t accumulate, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e, p;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t"
+      "setp.eq.u32 p, %4, %4;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::i8 [%0], %5, %6, %3, p;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::i8 [%0], %7, %8, %3, p;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::i8 [%0], %9, %10, %3, p;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%11];\n\t}" ::"r"(d),
+      "l"(ad), "l"(bd), "r"(idesc), "r"(accumulate), "l"(ad + 2), "l"(bd + 2), "l"(ad + 4), "l"(bd + 4), "l"(ad + 6),
+      "l"(bd + 6), "r"(smem_u32(bar))
+      : "memory");
+}
+
+template <int kAct>
+__device__ __forceinline__ void finish(uint32_t* v, float rs, const float2* cols) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 2) {
+    const float4 c = *reinterpret_cast<const float4*>(cols + i);  // {scale, bias} of two columns
+    v[i] = __float_as_uint(activate<kAct>(fmaf(float(int(v[i])) * rs, c.x, c.y)));
+    v[i + 1] = __float_as_uint(activate<kAct>(fmaf(float(int(v[i + 1])) * rs, c.z, c.w)));
+  }
+}
+
+// Group boundaries to shared memory: row0 and tile0 (exclusive prefix of the
+// groups' tiles).  Ends are clamped to [0, M] and made non-decreasing, so no
+// table of boundaries leads outside A.
+template <int kRows>
+__device__ __forceinline__ void build_groups(const ProductArgs& a, ProductSmem& S) {
+  for (int g = threadIdx.x; g < a.groups; g += kThreads) S.row0[g + 1] = min(max(a.ends[g], 0), a.M);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int row = 0, tile = 0;
+    S.row0[0] = 0;
+    for (int g = 0; g < a.groups; ++g) {
+      const int end = max(S.row0[g + 1], row);
+      S.tile0[g] = tile;
+      tile += (end - row + kRows - 1) / kRows * a.tiles_n;
+      S.row0[g + 1] = row = end;
+    }
+    S.tile0[a.groups] = tile;
+  }
+  __syncthreads();
+}
+
+template <int kTN, bool kGrouped>
+__global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ ProductArgs a) {
+  constexpr int kBBytes = kTN * kTileK;
+  constexpr int kHalf = kTN / 2;  // columns of an epilogue warp
+  constexpr uint32_t kIdesc = idesc_i8(kTileRows, kTN);
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int stage_bytes = a.a_bytes + kBBytes;
+  uint8_t* boxes = ring + a.stages * stage_bytes;
+  float2* col_mem = reinterpret_cast<float2*>(boxes + kEpiWarps * kBoxBytes);
+  ProductSmem& S = *reinterpret_cast<ProductSmem*>(col_mem + kEpiWarps * kHalf);
+  volatile int* abort_flag = &S.abort_flag;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < a.stages; ++i) {
+      mbar_init(&S.full[i], 1);
+      mbar_init(&S.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&S.acc_full[i], 1);
+      mbar_init(&S.acc_empty[i], kEpiWarps);
+    }
+    mbar_init(&S.drain, 1);
+    S.abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch(&a.tmA);
+    tma_prefetch(&a.tmB);
+  }
+  if (warp == 1) {
+    tmem_alloc(&S.tmem_base, 2 * kTN);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  griddep_wait();
+  griddep_launch_dependents();
+  if constexpr (kGrouped) build_groups<kTileRows>(a, S);
+  const uint32_t tmem = S.tmem_base;
+  const int tiles = kGrouped ? S.tile0[a.groups] : (a.M + kTileRows - 1) / kTileRows * a.tiles_n;
+  const int kblocks = (a.K + kTileK - 1) / kTileK;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    const bool leader = elect_one();
+    bool ok = true;
+    int st = 0, issued = 0;
+    uint32_t phase = 1;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      const Tile w = tile_at<kGrouped, kTileRows>(a, S, t);
+      const int brow = w.group * a.N + w.tn * kTN;
+      for (int kb = 0; kb < kblocks; ++kb) {
+        if (!(ok = mbar_wait_warp(&S.empty[st], phase, abort_flag, a.sync, a.wait_budget, a.wait_hint_ns))) break;
+        if (leader) {
+          uint8_t* sa = ring + st * stage_bytes;
+          mbar_arrive_expect_tx(&S.full[st], stage_bytes);
+          tma_load_2d(&a.tmA, &S.full[st], sa, kb * kTileK, w.row0);
+          tma_load_2d(&a.tmB, &S.full[st], sa + a.a_bytes, kb * kTileK, brow);
+        }
+        issued = min(issued + 1, a.stages);
+        if (++st == a.stages) { st = 0; phase ^= 1; }
+      }
+    }
+    // Every load in flight has landed and been consumed before the CTA ends
+    // (bounded).
+    for (int i = 0; i < issued; ++i) {
+      st = st == 0 ? a.stages - 1 : st - 1;
+      if (st == a.stages - 1) phase ^= 1;
+      const long long t0 = clock64();
+      while (!mbar_test(&S.empty[st], phase ^ 1) && clock64() - t0 < 100000000LL) {
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    bool ok = true;
+    int st = 0, n = 0;
+    uint32_t phase = 0;
+    const uint32_t sbase = smem_u32(ring);
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++n) {
+      const int slot = n & 1;
+      if (!(ok = mbar_wait_warp(&S.acc_empty[slot], ((n >> 1) & 1) ^ 1, abort_flag, a.sync, a.wait_budget, a.wait_hint_ns)))
+        break;
+      tc_fence_after();
+      for (int kb = 0; kb < kblocks; ++kb) {
+        if (!(ok = mbar_wait_warp(&S.full[st], phase, abort_flag, a.sync, a.wait_budget, a.wait_hint_ns))) break;
+        tc_fence_after();
+        const uint64_t ad = sdesc_sw128(sbase + st * stage_bytes);
+        const uint64_t bd = sdesc_sw128(sbase + st * stage_bytes + a.a_bytes);
+        umma_i8_stage_warp(tmem + slot * kTN, ad, bd, kIdesc, kb != 0, &S.empty[st]);
+        if (++st == a.stages) { st = 0; phase ^= 1; }
+      }
+      if (ok) umma_commit_warp(&S.acc_full[slot]);
+    }
+    umma_commit_warp(&S.drain);  // every MMA has retired before TMEM is released
+    const long long t0 = clock64();
+    while (!mbar_test(&S.drain, 0) && clock64() - t0 < 100000000LL) {
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue
+    // Warp: TMEM lane quadrant q (32 rows), half h of the tile's columns.
+    const int q = warp & 3, ew = warp - 2, h = ew >> 2;
+    uint8_t* box = boxes + ew * kBoxBytes;
+    float2* cols = col_mem + ew * kHalf;
+    const bool f16 = a.c_f16;
+    bool ok = true;
+    int n = 0;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++n) {
+      const Tile w = tile_at<kGrouped, kTileRows>(a, S, t);
+      const int slot = n & 1;
+      const int lrow = 32 * q + lane;
+      const int c0 = w.tn * kTN + h * kHalf;
+      const bool live = 32 * q < w.rows && c0 < a.N;  // this warp has something to store
+      float rs = 0.f;
+      long long dst = -1;
+      if (live) {
+        if (lrow < w.rows) {
+          const int r = w.row0 + lrow;
+          rs = a.sA[r];
+          dst = r;
+          if (kGrouped && a.c_rows) {
+            dst = a.c_rows[r];
+            if (dst >= a.c_dst_rows) dst = -1;
+          }
+        }
+        __syncwarp();
+        for (int j = lane; j < kHalf; j += 32) {
+          const int c = c0 + j;
+          float2 v = make_float2(0.f, 0.f);
+          if (c < a.N) {
+            v.x = a.sB[int64_t(w.group) * a.N + c];
+            if (!kGrouped && a.bias_kind)
+              v.y = a.bias_kind == kBiasF32 ? static_cast<const float*>(a.bias)[c] : half_at(a.bias, c, f16);
+          }
+          cols[j] = v;
+        }
+        __syncwarp();
+      }
+      if (!(ok = mbar_wait_warp(&S.acc_full[slot], (n >> 1) & 1, abort_flag, a.sync, a.wait_budget, a.wait_hint_ns)))
+        break;
+      tc_fence_after();
+      const uint32_t taddr = tmem + slot * kTN + (uint32_t(32 * q) << 16) + h * kHalf;
+      if (!live) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S.acc_empty[slot]);
+        continue;
+      }
+#pragma unroll 1
+      for (int ch = 0; ch < kHalf / 64; ++ch) {
+        uint32_t v[64];
+        __syncwarp();
+        tmem_ld32(taddr + 64 * ch, v);
+        tmem_ld32(taddr + 64 * ch + 32, v + 32);
+        tmem_wait_ld_into2(v, v + 32);
+        if (ch == kHalf / 64 - 1) {  // the accumulator is free for the tile after next
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&S.acc_empty[slot]);
+        }
+        const float2* cc = cols + 64 * ch;
+        const int col0 = c0 + 64 * ch;
+        switch (kGrouped ? PB2_ACT_NONE : a.act) {
+          case PB2_ACT_RELU: finish<PB2_ACT_RELU>(v, rs, cc); finish<PB2_ACT_RELU>(v + 32, rs, cc + 32); break;
+          case PB2_ACT_SILU: finish<PB2_ACT_SILU>(v, rs, cc); finish<PB2_ACT_SILU>(v + 32, rs, cc + 32); break;
+          case PB2_ACT_GELU: finish<PB2_ACT_GELU>(v, rs, cc); finish<PB2_ACT_GELU>(v + 32, rs, cc + 32); break;
+          case PB2_ACT_GELU_TANH:
+            finish<PB2_ACT_GELU_TANH>(v, rs, cc); finish<PB2_ACT_GELU_TANH>(v + 32, rs, cc + 32); break;
+          default: finish<PB2_ACT_NONE>(v, rs, cc); finish<PB2_ACT_NONE>(v + 32, rs, cc + 32);
+        }
+        // Rows leave through the warp's box (16-byte chunks, chunk j of row r
+        // at j ^ (r & 7)): eight lanes move one 128-byte row, so stores (and
+        // the residual's loads) are whole lines.
+        const int piece = lane & 7;
+        if (!kGrouped && a.residual) {
+#pragma unroll
+          for (int it = 0; it < 8; ++it) {
+            const int br = 4 * it + (lane >> 3);
+            const long long dr = __shfl_sync(0xffffffffu, dst, br);
+            const int col = col0 + 8 * piece;
+            uint4 r = make_uint4(0u, 0u, 0u, 0u);
+            if (dr >= 0 && col < a.N) {
+              const uint16_t* src = static_cast<const uint16_t*>(a.residual) + dr * a.N + col;
+              if (a.vec) {
+                r = *reinterpret_cast<const uint4*>(src);
+              } else {
+                uint16_t e[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                  if (col + j < a.N) e[j] = src[j];
+                r = make_uint4(e[0] | uint32_t(e[1]) << 16, e[2] | uint32_t(e[3]) << 16, e[4] | uint32_t(e[5]) << 16,
+                               e[6] | uint32_t(e[7]) << 16);
+              }
+            }
+            *reinterpret_cast<uint4*>(box + br * 128 + ((piece ^ (br & 7)) << 4)) = r;
+          }
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const uint4 r = *reinterpret_cast<const uint4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4));
+            const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+              const float2 f = unpack_half2(rw[p], f16);
+              v[8 * j + 2 * p] = __float_as_uint(__uint_as_float(v[8 * j + 2 * p]) + f.x);
+              v[8 * j + 2 * p + 1] = __float_as_uint(__uint_as_float(v[8 * j + 2 * p + 1]) + f.y);
+            }
+          }
+          __syncwarp();
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          uint32_t o[4];
+#pragma unroll
+          for (int p = 0; p < 4; ++p)
+            o[p] = pack_half2(__uint_as_float(v[8 * j + 2 * p]), __uint_as_float(v[8 * j + 2 * p + 1]), f16);
+          *reinterpret_cast<uint4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int it = 0; it < 8; ++it) {
+          const int br = 4 * it + (lane >> 3);
+          const long long dr = __shfl_sync(0xffffffffu, dst, br);
+          const int col = col0 + 8 * piece;
+          const uint4 val = *reinterpret_cast<const uint4*>(box + br * 128 + ((piece ^ (br & 7)) << 4));
+          if (dr >= 0 && col < a.N) {
+            uint16_t* out = static_cast<uint16_t*>(a.C) + dr * a.N + col;
+            if (a.vec) {
+              *reinterpret_cast<uint4*>(out) = val;
+            } else {
+              const uint32_t w4[4] = {val.x, val.y, val.z, val.w};
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (col + j < a.N) out[j] = uint16_t(w4[j / 2] >> (16 * (j & 1)));
+            }
+          }
+        }
+        __syncwarp();
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) {
+    __syncwarp();
+    tmem_dealloc(tmem, 2 * kTN);
+  }
+}
+
+// ------------------------------------------------------------------ host
+bool al16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+template <int kTN, bool kGrouped>
+int launch_product(ProductArgs& a, const int8_t* A, const int8_t* B, int64_t max_tiles_m, int device, cudaStream_t s) {
+  const int box_rows = std::min(kTileRows, (a.M + 7) / 8 * 8);
+  int st;
+  if ((st = make_tmap_2d(&a.tmA, A, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, a.M, kTileK, box_rows,
+                         CU_TENSOR_MAP_SWIZZLE_128B)) ||
+      (st = make_tmap_2d(&a.tmB, B, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, uint64_t(std::max(a.groups, 1)) * a.N, kTileK,
+                         kTN, CU_TENSOR_MAP_SWIZZLE_128B)))
+    return st;
+  a.a_bytes = box_rows * kTileK;
+  a.tiles_n = (a.N + kTN - 1) / kTN;
+  a.raster = 8;
+  const int fixed = 1024 + kEpiWarps * (kBoxBytes + kTN / 2 * 8) + int(sizeof(ProductSmem));
+  a.stages = std::min(kMaxStages, (232448 - fixed) / (a.a_bytes + kTN * kTileK));
+  a.wait_budget = wait_budget_cycles();
+  a.wait_hint_ns = suspend_hint_ns(a.wait_budget);
+  const int smem = fixed + a.stages * (a.a_bytes + kTN * kTileK);
+  auto kern = product_kernel<kTN, kGrouped>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return launch_status();
+  const int sms = sm_count(device) > 0 ? sm_count(device) : 148;
+  const int grid = int(std::max<int64_t>(1, std::min<int64_t>(max_tiles_m * a.tiles_n, sms)));
+  return launch_programmatic(kern, dim3(unsigned(grid)), kThreads, smem, s, 1, a);
+}
+
+// out[t] = residual[t] + sum_j w[t, j] * slots[t * top_k + j], f32 sums in
+// slot order; a thread per 8 columns.
+struct CombineArgs {
+  const void* slots;
+  const float* weights;
+  const void* residual;
+  void* out;
+  long long tokens;
+  int top_k, n, f16, vec;
+};
+
+__global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const int vecs = (a.n + 7) / 8;
+  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  const long long t = i / vecs;
+  if (t >= a.tokens) return;
+  const int col = int(i - t * vecs) * 8;
+  const bool f16 = a.f16;
+  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  auto add = [&](const void* base, long long row, float w) {
+    const uint16_t* p = static_cast<const uint16_t*>(base) + row * a.n + col;
+    if (a.vec) {
+      const uint4 r = *reinterpret_cast<const uint4*>(p);
+      const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = unpack_half2(rw[j], f16);
+        acc[2 * j] = fmaf(w, f.x, acc[2 * j]);
+        acc[2 * j + 1] = fmaf(w, f.y, acc[2 * j + 1]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (col + j < a.n) acc[j] = fmaf(w, half_at(p, j, f16), acc[j]);
+    }
+  };
+  for (int j = 0; j < a.top_k; ++j) {
+    const float w = a.weights[t * a.top_k + j];
+    if (w != 0.f) add(a.slots, t * a.top_k + j, w);
+  }
+  if (a.residual) add(a.residual, t, 1.0f);
+  uint16_t* o = static_cast<uint16_t*>(a.out) + t * a.n + col;
+  if (a.vec) {
+    *reinterpret_cast<uint4*>(o) = make_uint4(pack_half2(acc[0], acc[1], f16), pack_half2(acc[2], acc[3], f16),
+                                              pack_half2(acc[4], acc[5], f16), pack_half2(acc[6], acc[7], f16));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (col + j < a.n) o[j] = half_bits(acc[j], f16);
+  }
+}
+
+bool type16(int t) { return t == PB2_TYPE_BF16 || t == PB2_TYPE_F16; }
+
+}  // namespace
+}  // namespace pb2
+
+extern "C" int pb2_gemm_epilogue(const pb2_gemm_epilogue_params* pp, void* stream) {
+  pb2::NvtxRange nvtx_range("pb2_gemm_epilogue");
+  using namespace pb2;
+  if (!pp) return PB2_ERR_INVALID_ARGUMENT;
+  const pb2_gemm_epilogue_params& p = *pp;
+  if (p.m < 0 || p.n <= 0 || p.k <= 0 || p.m > INT32_MAX || p.n > INT32_MAX || p.k > INT32_MAX)
+    return PB2_ERR_INVALID_ARGUMENT;
+  if (!type16(p.c_type) || p.activation < PB2_ACT_NONE || p.activation > PB2_ACT_GELU_TANH)
+    return PB2_ERR_INVALID_ARGUMENT;
+  if (p.bias && p.bias_type != PB2_TYPE_F32 && p.bias_type != p.c_type) return PB2_ERR_INVALID_ARGUMENT;
+  if (p.k % 16 != 0) return PB2_ERR_UNSUPPORTED_CONFIG;  // 16-byte rows of A and B
+  if (p.m > 0 && (!p.A || !p.B || !p.A_scales || !p.B_scales || !p.C || !al16(p.A) || !al16(p.B)))
+    return PB2_ERR_INVALID_ARGUMENT;
+  int st = set_device(p.device);
+  if (st) return st;
+  if (p.m == 0) return PB2_OK;
+  ProductArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.sA = p.A_scales;
+  a.sB = p.B_scales;
+  a.C = p.C;
+  a.bias = p.bias;
+  a.bias_kind = !p.bias ? kBiasNone : p.bias_type == PB2_TYPE_F32 ? kBiasF32 : kBiasHalf;
+  a.residual = p.residual;
+  a.c_f16 = p.c_type == PB2_TYPE_F16;
+  a.act = p.activation;
+  a.M = int(p.m);
+  a.N = int(p.n);
+  a.K = int(p.k);
+  a.vec = p.n % 8 == 0 && al16(p.C) && al16(p.residual);
+  a.sync = static_cast<SignalSync*>(p.host_signal_sync);
+  return launch_product<128, false>(a, p.A, p.B, (p.m + kTileRows - 1) / kTileRows, p.device,
+                                    static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int pb2_gemm_grouped(const pb2_gemm_grouped_params* pp, void* stream) {
+  pb2::NvtxRange nvtx_range("pb2_gemm_grouped");
+  using namespace pb2;
+  if (!pp) return PB2_ERR_INVALID_ARGUMENT;
+  const pb2_gemm_grouped_params& p = *pp;
+  if (p.m < 0 || p.n <= 0 || p.k <= 0 || p.m > INT32_MAX || p.k > INT32_MAX) return PB2_ERR_INVALID_ARGUMENT;
+  if (p.num_experts <= 0 || p.num_experts > kMaxGroups || p.n > INT32_MAX / p.num_experts) return PB2_ERR_INVALID_ARGUMENT;
+  if (!type16(p.c_type)) return PB2_ERR_INVALID_ARGUMENT;
+  if (p.k % 16 != 0) return PB2_ERR_UNSUPPORTED_CONFIG;
+  if (p.c_row_index && p.c_rows < 0) return PB2_ERR_INVALID_ARGUMENT;
+  if (p.m > 0 && (!p.A || !p.B || !p.A_scales || !p.B_scales || !p.C || !p.routing_offsets || !al16(p.A) || !al16(p.B)))
+    return PB2_ERR_INVALID_ARGUMENT;
+  int st = set_device(p.device);
+  if (st) return st;
+  if (p.m == 0) return PB2_OK;
+  ProductArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.sA = p.A_scales;
+  a.sB = p.B_scales;
+  a.C = p.C;
+  a.c_f16 = p.c_type == PB2_TYPE_F16;
+  a.M = int(p.m);
+  a.N = int(p.n);
+  a.K = int(p.k);
+  a.groups = int(p.num_experts);
+  a.ends = p.routing_offsets;
+  a.c_rows = p.c_row_index;
+  a.c_dst_rows = p.c_row_index ? p.c_rows : p.m;
+  a.vec = p.n % 8 == 0 && al16(p.C);
+  a.sync = static_cast<SignalSync*>(p.host_signal_sync);
+  const int64_t tiles_m = p.m / kTileRows + std::min(p.num_experts, p.m);  // at most
+  return launch_product<128, true>(a, p.A, p.B, tiles_m, p.device, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int pb2_combine_slots(const pb2_combine_params* pp, void* stream) {
+  pb2::NvtxRange nvtx_range("pb2_combine_slots");
+  using namespace pb2;
+  if (!pp) return PB2_ERR_INVALID_ARGUMENT;
+  const pb2_combine_params& p = *pp;
+  if (p.num_tokens < 0 || p.top_k <= 0 || p.n <= 0 || p.num_tokens > INT32_MAX || p.top_k > INT32_MAX || p.n > INT32_MAX)
+    return PB2_ERR_INVALID_ARGUMENT;
+  if (!type16(p.type)) return PB2_ERR_INVALID_ARGUMENT;
+  if (p.num_tokens > 0 && (!p.slots || !p.topk_weights || !p.out)) return PB2_ERR_INVALID_ARGUMENT;
+  const int64_t blocks = (p.num_tokens * ((p.n + 7) / 8) + 255) / 256;
+  if (blocks > INT32_MAX) return PB2_ERR_INVALID_ARGUMENT;
+  int st = set_device(p.device);
+  if (st) return st;
+  if (p.num_tokens == 0) return PB2_OK;
+  CombineArgs a;
+  a.slots = p.slots;
+  a.weights = p.topk_weights;
+  a.residual = p.residual;
+  a.out = p.out;
+  a.tokens = p.num_tokens;
+  a.top_k = int(p.top_k);
+  a.n = int(p.n);
+  a.f16 = p.type == PB2_TYPE_F16;
+  a.vec = p.n % 8 == 0 && al16(p.slots) && al16(p.out) && al16(p.residual);
+  return launch_programmatic(combine_kernel, dim3(unsigned(blocks)), 256, 0, static_cast<cudaStream_t>(stream), 1, a);
+}
+
+extern "C" int64_t pb2_gated_experts_workspace_bytes(int64_t slots, int64_t inner, int64_t hidden) {
+  if (slots <= 0 || inner <= 0 || hidden <= 0) return 0;
+  auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
+  return up(slots * inner) + up(slots * 4) + up(slots * hidden * 2);
+}
+
+extern "C" int pb2_gated_experts(const pb2_gated_experts_params* pp, void* stream) {
+  pb2::NvtxRange nvtx_range("pb2_gated_experts");
+  using namespace pb2;
+  if (!pp) return PB2_ERR_INVALID_ARGUMENT;
+  const pb2_gated_experts_params& p = *pp;
+  if (p.num_tokens < 0 || p.top_k <= 0 || p.inner <= 0 || p.hidden <= 0 || p.top_k > INT32_MAX ||
+      p.num_tokens > INT32_MAX / p.top_k)
+    return PB2_ERR_INVALID_ARGUMENT;
+  const int64_t slots = p.num_tokens * p.top_k;
+  auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
+  if (slots > 0 && (!p.workspace || !al16(p.workspace) ||
+                    p.workspace_bytes < pb2_gated_experts_workspace_bytes(slots, p.inner, p.hidden) || !p.slot_indices))
+    return PB2_ERR_INVALID_ARGUMENT;
+  uint8_t* ws = static_cast<uint8_t*>(p.workspace);
+  pb2_gated_quant_params q;
+  std::memset(&q, 0, sizeof(q));
+  q.device = p.device;
+  q.x = p.x;
+  q.x_type = p.type;
+  q.m = q.x_rows = slots;
+  q.n = p.inner;
+  q.activation = p.activation;
+  q.row_index = p.slot_indices;
+  q.smooth = p.smooth;
+  q.xq = reinterpret_cast<int8_t*>(ws);
+  q.scales = reinterpret_cast<float*>(ws + up(slots * p.inner));
+  q.max_val = p.max_val;
+  q.block_size = p.block_size;
+  pb2_gemm_grouped_params g;
+  std::memset(&g, 0, sizeof(g));
+  g.device = p.device;
+  g.m = slots;
+  g.n = p.hidden;
+  g.k = p.inner;
+  g.A = q.xq;
+  g.B = p.w;
+  g.A_scales = q.scales;
+  g.B_scales = p.w_scales;
+  g.C = ws + up(slots * p.inner) + up(slots * 4);
+  g.c_type = p.type;
+  g.num_experts = p.num_experts;
+  g.routing_offsets = p.routing_offsets;
+  g.c_row_index = p.slot_indices;
+  g.c_rows = slots;
+  g.host_signal_sync = p.host_signal_sync;
+  pb2_combine_params c;
+  std::memset(&c, 0, sizeof(c));
+  c.device = p.device;
+  c.slots = g.C;
+  c.topk_weights = p.topk_weights;
+  c.residual = p.residual;
+  c.out = p.out;
+  c.type = p.type;
+  c.num_tokens = p.num_tokens;
+  c.top_k = p.top_k;
+  c.n = p.hidden;
+  // The later steps' arguments before any step is queued.
+  if (!type16(p.type) || p.num_experts <= 0 || p.num_experts > kMaxGroups || p.hidden > INT32_MAX / p.num_experts ||
+      p.inner > INT32_MAX || (slots > 0 && (!p.w || !al16(p.w) || !p.w_scales || !p.routing_offsets || !p.topk_weights || !p.out)))
+    return PB2_ERR_INVALID_ARGUMENT;
+  if (p.inner % 16 != 0) return PB2_ERR_UNSUPPORTED_CONFIG;
+  int st = pb2_quantize_gated(&q, stream);
+  if (!st) st = pb2_gemm_grouped(&g, stream);
+  if (!st) st = pb2_combine_slots(&c, stream);
+  return st;
+}

@@ -21,7 +21,7 @@
 #include <algorithm>
 #include <cmath>
 
-#include "pb2_common.cuh"
+#include "pb2_epilogue.cuh"
 
 namespace pb2 {
 namespace {
@@ -68,15 +68,10 @@ __device__ __forceinline__ uint4 load_raw(const QuantArgs& a, int row, int vec, 
   return *reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + int64_t(row) * a.n + 8 * vec);
 }
 
-// Vector `vec` of `row` from its raw bytes: the Hadamard transform of width
-// a.block and the smooth scale.  Every lane of the warp must call it with the
-// same `iter` (the butterflies shuffle across lanes).
-template <typename T>
-__device__ __forceinline__ void vec_from_raw(const QuantArgs& a, int row, int vec, bool valid, uint4 raw,
-                                             float* v) {
-  const T* e = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = valid ? to_f32<T>(e[i]) : 0.f;
+// The block Hadamard transform (width a.block) of the row's vector `vec`, in
+// place.  Every lane of the warp must call it (the butterflies shuffle across
+// lanes).
+__device__ __forceinline__ void transform_vec(const QuantArgs& a, int vec, float* v) {
   if (a.block > 0) {
 #pragma unroll
     for (int s = 1; s < 8; s <<= 1) {  // butterflies inside the 8-element vector
@@ -99,6 +94,18 @@ __device__ __forceinline__ void vec_from_raw(const QuantArgs& a, int row, int ve
     for (int i = 0; i < 8; ++i) v[i] *= a.norm;
     if (vec % (a.block / 8) == 0) v[0] = -v[0];  // first element of the block
   }
+}
+
+// Vector `vec` of `row` from its raw bytes: the Hadamard transform of width
+// a.block and the smooth scale.  Every lane of the warp must call it with the
+// same `iter` (the butterflies shuffle across lanes).
+template <typename T>
+__device__ __forceinline__ void vec_from_raw(const QuantArgs& a, int row, int vec, bool valid, uint4 raw,
+                                             float* v) {
+  const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = valid ? to_f32<T>(e[i]) : 0.f;
+  transform_vec(a, vec, v);
   if (a.smooth && valid) {
     const float* sp = a.smooth + (a.smooth_per_row ? int64_t(row) * a.n : 0) + 8 * vec;
     const float4 s0 = *reinterpret_cast<const float4*>(sp);
@@ -207,6 +214,109 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) quant_rows_reg_kern
   }
 }
 
+// act(gate) * up quantized: row i of xq from row index[i] of x, whose rows
+// hold a.n gate values and then a.n up values.  The products of the row stay in registers (kIters vectors of eight a
+// thread) between the max pass and the rounding pass: x is read once and the
+// activation computed once.
+struct GatedArgs {
+  QuantArgs q;
+  const int32_t* index;
+  int x_rows;
+};
+
+template <typename T, int kAct>
+__device__ __forceinline__ void gated_vec(const GatedArgs& a, const T* row, int vec, bool valid, float* v) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = 0.f;
+  if (valid) {
+    const uint4 g = *reinterpret_cast<const uint4*>(row + 8 * vec);
+    const uint4 u = *reinterpret_cast<const uint4*>(row + a.q.n + 8 * vec);
+    const T* ge = reinterpret_cast<const T*>(&g);
+    const T* ue = reinterpret_cast<const T*>(&u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = activate<kAct>(to_f32<T>(ge[i])) * to_f32<T>(ue[i]);
+  }
+  transform_vec(a.q, vec, v);
+  if (a.q.smooth && valid) {
+    const float4 s0 = *reinterpret_cast<const float4*>(a.q.smooth + 8 * vec);
+    const float4 s1 = *reinterpret_cast<const float4*>(a.q.smooth + 8 * vec + 4);
+    v[0] *= s0.x; v[1] *= s0.y; v[2] *= s0.z; v[3] *= s0.w;
+    v[4] *= s1.x; v[5] *= s1.y; v[6] *= s1.z; v[7] *= s1.w;
+  }
+}
+
+__device__ __forceinline__ void store_quantized(const QuantArgs& a, int64_t row, int vec, const float* v, float inv) {
+  uint32_t packed[2] = {0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float q = fminf(fmaxf(rintf(v[i] * inv), -a.max_val), a.max_val);
+    packed[i / 4] |= (uint32_t(int32_t(q)) & 0xFFu) << (8 * (i % 4));
+  }
+  *reinterpret_cast<uint2*>(a.xq + row * a.n + 8 * vec) = make_uint2(packed[0], packed[1]);
+}
+
+// kIters = 0: any row length, the products computed in both passes.
+template <typename T, int kAct, int kIters, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) quant_gated_kernel(const GatedArgs a) {
+  __shared__ float warp_max[kThreads / 32];
+  griddep_wait();
+  griddep_launch_dependents();
+  const int64_t row = blockIdx.x;
+  const int nvec = a.q.n / 8;
+  const int src = a.index ? a.index[row] : int(row);
+  const bool in = src >= 0 && src < a.x_rows;
+  const T* x = static_cast<const T*>(a.q.x) + (in ? int64_t(src) * 2 * a.q.n : 0);
+  float amax = 0.f;
+  constexpr int kKept = kIters > 0 ? kIters : 1;
+  float v[kKept][8];
+  const int iters = kIters > 0 ? kIters : (nvec + kThreads - 1) / kThreads;
+#pragma unroll
+  for (int it = 0; it < iters; ++it) {
+    float(&w)[8] = v[kIters > 0 ? it : 0];
+    const int vec = it * kThreads + threadIdx.x;
+    gated_vec<T, kAct>(a, x, vec, in && vec < nvec, w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(w[i]));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x / 32] = amax;
+  __syncthreads();
+  amax = 0.f;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) amax = fmaxf(amax, warp_max[w]);
+  const float inv = amax > 0.f ? a.q.max_val / amax : 0.f;
+  if (threadIdx.x == 0) a.q.scales[row] = amax * a.q.inv_max_val;
+#pragma unroll
+  for (int it = 0; it < iters; ++it) {
+    float(&w)[8] = v[kIters > 0 ? it : 0];
+    const int vec = it * kThreads + threadIdx.x;
+    if constexpr (kIters == 0) gated_vec<T, kAct>(a, x, vec, in && vec < nvec, w);
+    if (vec < nvec) store_quantized(a.q, row, vec, w, inv);
+  }
+}
+
+template <typename T, int kAct>
+int launch_gated(const GatedArgs& a, cudaStream_t s) {
+  const int nvec = a.q.n / 8;
+  const dim3 grid(unsigned(a.q.m));
+  if (nvec <= 256) return launch_programmatic(quant_gated_kernel<T, kAct, 4, 64>, grid, 64, 0, s, 1, a);
+  if (nvec <= 1024) return launch_programmatic(quant_gated_kernel<T, kAct, 4, 256>, grid, 256, 0, s, 1, a);
+  if (nvec <= 2048) return launch_programmatic(quant_gated_kernel<T, kAct, 4, 512>, grid, 512, 0, s, 1, a);
+  return launch_programmatic(quant_gated_kernel<T, kAct, 0, 512>, grid, 512, 0, s, 1, a);
+}
+
+template <typename T>
+int launch_gated_act(const GatedArgs& a, int act, cudaStream_t s) {
+  switch (act) {
+    case PB2_ACT_RELU: return launch_gated<T, PB2_ACT_RELU>(a, s);
+    case PB2_ACT_SILU: return launch_gated<T, PB2_ACT_SILU>(a, s);
+    case PB2_ACT_GELU: return launch_gated<T, PB2_ACT_GELU>(a, s);
+    case PB2_ACT_GELU_TANH: return launch_gated<T, PB2_ACT_GELU_TANH>(a, s);
+    default: return launch_gated<T, PB2_ACT_NONE>(a, s);
+  }
+}
+
 // Launched with programmatic stream serialization: the grid is scheduled
 // while the previous kernel drains and waits for it in griddep_wait, and it
 // lets the next kernel (the GEMM reading its output) start its own set-up.
@@ -282,6 +392,48 @@ extern "C" int pb2_quantize(const pb2_quant_params* pp, void* stream) {
   else
     launch_quant<__nv_bfloat16>(a, s);
   return launch_status();
+}
+
+extern "C" int pb2_quantize_gated(const pb2_gated_quant_params* pp, void* stream) {
+  pb2::NvtxRange nvtx_range("pb2_quantize_gated");
+  using namespace pb2;
+  if (!pp) return PB2_ERR_INVALID_ARGUMENT;
+  const pb2_gated_quant_params& p = *pp;
+  if (p.m < 0 || p.n <= 0 || p.m > INT32_MAX || p.n > INT32_MAX || p.x_rows < 0 || p.x_rows > INT32_MAX)
+    return PB2_ERR_INVALID_ARGUMENT;
+  if (p.m > 0 && (!p.x || !p.xq || !p.scales)) return PB2_ERR_INVALID_ARGUMENT;
+  if (!p.row_index && p.x_rows != p.m) return PB2_ERR_INVALID_ARGUMENT;
+  if (p.max_val <= 0 || p.max_val > 127) return PB2_ERR_INVALID_ARGUMENT;
+  if (p.x_type != PB2_TYPE_BF16 && p.x_type != PB2_TYPE_F16) return PB2_ERR_INVALID_ARGUMENT;
+  if (p.activation < PB2_ACT_NONE || p.activation > PB2_ACT_GELU_TANH) return PB2_ERR_INVALID_ARGUMENT;
+  if (p.n % 8 != 0) return PB2_ERR_UNSUPPORTED_CONFIG;
+  if (p.block_size != 0) {
+    const int k = p.block_size;
+    if (k < 8 || (k & (k - 1)) != 0 || k > 256 || p.n % k != 0) return PB2_ERR_UNSUPPORTED_CONFIG;
+  }
+  if (reinterpret_cast<uintptr_t>(p.x) % 16 || reinterpret_cast<uintptr_t>(p.xq) % 8 ||
+      reinterpret_cast<uintptr_t>(p.smooth) % 16)
+    return PB2_ERR_INVALID_ARGUMENT;
+  int st = set_device(p.device);
+  if (st) return st;
+  if (p.m == 0) return PB2_OK;
+  GatedArgs a;
+  a.q.x = p.x;
+  a.q.smooth = p.smooth;
+  a.q.smooth_per_row = 0;
+  a.q.xq = p.xq;
+  a.q.scales = p.scales;
+  a.q.m = int(p.m);
+  a.q.n = int(p.n);
+  a.q.block = p.block_size;
+  a.q.norm = p.block_size ? float(1.0 / sqrt(double(p.block_size))) : 1.0f;
+  a.q.max_val = float(p.max_val);
+  a.q.inv_max_val = float(1.0 / double(p.max_val));
+  a.index = p.row_index;
+  a.x_rows = int(p.x_rows);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return p.x_type == PB2_TYPE_F16 ? launch_gated_act<__half>(a, p.activation, s)
+                                  : launch_gated_act<__nv_bfloat16>(a, p.activation, s);
 }
 
 namespace pb2 {

@@ -7,7 +7,14 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .pearl_gemm_interface import _device_index, _fail, _stream
+from .linear import _activation, _half_type, _operand, _sync_word
+from .pearl_gemm_interface import _call_on, _device_index, _fail, _stream
+from .quantization import _check_block
+
+_SCORING = {"softmax": 0, "sigmoid": 1}
+_LOGIT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+MAX_EXPERTS = 256  # the routing order sorts 8-bit expert ids
+MAX_TOP_K = 32
 
 
 def get_build_routing_data_scratchpad_bytes(numel: int) -> int:
@@ -189,3 +196,162 @@ def noisy_gemm_grouped(
         g.c_row_index, g.c_rows = _ptr(c_row_index), C.shape[0]
     with torch.cuda.device(A.device):
         _lib.call("pb2_noisy_gemm_grouped", g, _stream(A.device), "noisy_gemm_grouped")
+
+
+# ------------------------------------------------------- un-mined operators --
+# No reference counterpart: the reference takes these steps of the layer from
+# vLLM (pearl_moe_experts.py:377-434 runs them around its GEMM2).
+def route_tokens(logits, topk_weights, topk_ids, *, scoring: str = "softmax", bias=None, num_groups: int = 1,
+                 topk_groups: int = 1, renormalize: bool = True, scaling: float = 1.0) -> None:
+    """The experts of every token: ``topk_ids`` (m, top_k) int32 in
+    descending order, ties to the lowest index, and ``topk_weights`` (m,
+    top_k) float32, from ``logits`` (m, num_experts) float32 / bf16 / fp16.
+
+    Scores s are the row's softmax or sigmoids.  ``bias`` (num_experts,)
+    float32 is added for the choice only.  With ``num_groups`` > 1 only the
+    ``topk_groups`` best groups of experts take part; a group is worth its
+    best expert, or with a bias the sum of its two best.  The weights are s
+    of the chosen experts, divided by their sum when ``renormalize``, times
+    ``scaling``.  A logit of -inf or NaN masks its expert (score 0, chosen
+    last); a row that masks every expert gets weights 0.  ``topk_ids`` is
+    what build_routing_data takes."""
+    if logits.dim() != 2 or topk_ids.dim() != 2:
+        _fail("logits and topk_ids must be 2D (m, num_experts) and (m, top_k)")
+    m, experts = logits.shape
+    top_k = topk_ids.shape[1]
+    dev = logits.device
+    if scoring not in _SCORING:
+        _fail(f"scoring must be 'softmax' or 'sigmoid', got {scoring!r}")
+    if not 1 <= experts <= MAX_EXPERTS:
+        _fail(f"num_experts must be in 1..{MAX_EXPERTS}, got {experts}")
+    if num_groups < 1 or experts % num_groups or not 1 <= topk_groups <= num_groups:
+        _fail(f"num_groups must divide {experts} experts and topk_groups be in 1..num_groups, got "
+              f"{num_groups} and {topk_groups}")
+    if not 1 <= top_k <= min(MAX_TOP_K, topk_groups * (experts // num_groups)):
+        _fail(f"top_k must be in 1..{min(MAX_TOP_K, topk_groups * (experts // num_groups))}, got {top_k}")
+    p = _lib.RouteParams()
+    p.logits = _operand(logits, "logits", (m, experts), tuple(_LOGIT_TYPES), dev)
+    p.topk_weights = _operand(topk_weights, "topk_weights", (m, top_k), (torch.float32,), dev)
+    p.topk_ids = _operand(topk_ids, "topk_ids", (m, top_k), (torch.int32,), dev)
+    if bias is not None:
+        p.bias = _operand(bias, "bias", (experts,), (torch.float32,), dev)
+    p.logits_type, p.num_tokens, p.num_experts, p.top_k = _LOGIT_TYPES[logits.dtype], m, experts, top_k
+    p.scoring, p.num_groups, p.topk_groups = _SCORING[scoring], num_groups, topk_groups
+    p.renormalize, p.scaling = bool(renormalize), scaling
+    _call_on(dev, "pb2_route_tokens", p, "route_tokens")
+
+
+def gemm_grouped(A, B, A_scales, B_scales, C, routing_offsets, *, c_row_index=None, host_signal_sync=None) -> None:
+    """The un-mined product of every expert in one launch: rows of ``A``
+    (m, k) int8 in expert order, expert e's ending at ``routing_offsets[e]``
+    (build_routing_data's, read on the device: no host copy of the counts),
+    against ``B`` (E, n, k) int8; A_scales (m,), B_scales (E, n) float32;
+
+        C[i] = A_scales[i] * B_scales[e] * (A[i] . B[e]^T)   (bf16 or fp16)
+
+    With ``c_row_index`` ((m,) int32, e.g. slot_indices) row i goes to row
+    c_row_index[i] of C instead; rows outside C are skipped.  Rows past the
+    last expert's end are not written.  k a multiple of 16, E <= 256."""
+    if A.dim() != 2 or B.dim() != 3 or C.dim() != 2:
+        _fail("A and C must be 2-D and B 3-D (num_experts, n, k)")
+    m, k = A.shape
+    experts, n, _ = B.shape
+    dev = A.device
+    if k % 16:
+        _fail(f"k must be a multiple of 16, got {k}")
+    if not 1 <= experts <= MAX_EXPERTS:
+        _fail(f"num_experts must be in 1..{MAX_EXPERTS}, got {experts}")
+    half = _half_type(C, "C")
+    p = _lib.GemmGroupedParams()
+    p.A = _operand(A, "A", (m, k), (torch.int8,), dev)
+    p.B = _operand(B, "B", (experts, n, k), (torch.int8,), dev)
+    p.A_scales = _operand(A_scales, "A_scales", (m,), (torch.float32,), dev)
+    p.B_scales = _operand(B_scales, "B_scales", (experts, n), (torch.float32,), dev)
+    p.C = _operand(C, "C", (m if c_row_index is None else C.shape[0], n), (C.dtype,), dev)
+    p.routing_offsets = _operand(routing_offsets, "routing_offsets", (experts,), (torch.int32,), dev)
+    if c_row_index is not None:
+        p.c_row_index = _operand(c_row_index, "c_row_index", (m,), (torch.int32,), dev)
+        p.c_rows = C.shape[0]
+    p.m, p.n, p.k, p.num_experts, p.c_type = m, n, k, experts, half
+    p.host_signal_sync = _sync_word(host_signal_sync)
+    _call_on(dev, "pb2_gemm_grouped", p, "gemm_grouped")
+
+
+def combine_slots(slots, topk_weights, out, *, residual=None) -> None:
+    """out[t] = residual[t] + sum_j topk_weights[t, j] * slots[t * top_k + j]:
+    the token's experts added up in float32 in the order of j, rounded once.
+    slots (m * top_k, n), out and ``residual`` (m, n), all bf16 or all fp16;
+    topk_weights (m, top_k) float32.  A slot whose weight is 0 is not read;
+    ``residual`` may be out itself."""
+    if topk_weights.dim() != 2 or out.dim() != 2:
+        _fail("topk_weights and out must be 2D (m, top_k) and (m, n)")
+    m, top_k = topk_weights.shape
+    n = out.shape[1]
+    dev = out.device
+    half = _half_type(out, "out")
+    p = _lib.CombineParams()
+    p.slots = _operand(slots, "slots", (m * top_k, n), (out.dtype,), dev)
+    p.topk_weights = _operand(topk_weights, "topk_weights", (m, top_k), (torch.float32,), dev)
+    p.out = _operand(out, "out", (m, n), (out.dtype,), dev)
+    if residual is not None:
+        p.residual = _operand(residual, "residual", (m, n), (out.dtype,), dev)
+    p.type, p.num_tokens, p.top_k, p.n = half, m, top_k, n
+    _call_on(dev, "pb2_combine_slots", p, "combine_slots")
+
+
+def get_gated_experts_workspace_bytes(slots: int, inner: int, hidden: int) -> int:
+    """Workspace bytes of gated_experts for ``slots`` routed slots."""
+    return int(_lib.load().pb2_gated_experts_workspace_bytes(int(slots), int(inner), int(hidden)))
+
+
+def gated_experts(x, w, w_scales, out, slot_indices, routing_offsets, topk_weights, *, residual=None,
+                  smooth_scale=None, activation: str = "silu", max_val: int = 127, block_size: int = 0,
+                  workspace=None, host_signal_sync=None) -> None:
+    """The second half of the experts' MLP: ``x`` (m * top_k, 2 inner), the
+    first product's rows in slot order (gate values, then up values), through
+    quantize_gated into expert order, gemm_grouped with ``w`` (E, hidden,
+    inner) int8 / ``w_scales`` (E, hidden) float32 and combine_slots into
+    ``out`` (m, hidden).  ``slot_indices`` (m * top_k,) and
+    ``routing_offsets`` (E,) are build_routing_data's, ``topk_weights`` (m,
+    top_k) route_tokens'.  x, out and ``residual`` are all bf16 or all fp16;
+    ``smooth_scale`` (1, inner) or (inner,) float32.  ``workspace`` (uint8,
+    get_gated_experts_workspace_bytes) is taken from torch's allocator when
+    not given.  The slots' products are rounded to out's type before they are
+    added up."""
+    if w.dim() != 3 or topk_weights.dim() != 2:
+        _fail("w must be 3-D (num_experts, hidden, inner) and topk_weights 2D (m, top_k)")
+    experts, hidden, inner = w.shape
+    m, top_k = topk_weights.shape
+    slots = m * top_k
+    dev = x.device
+    if inner % 16:
+        _fail(f"inner must be a multiple of 16, got {inner}")
+    if not 1 <= experts <= MAX_EXPERTS:
+        _fail(f"num_experts must be in 1..{MAX_EXPERTS}, got {experts}")
+    if not 0 < max_val <= 127:
+        _fail(f"max_val must be in 1..127, got {max_val}")
+    _check_block(block_size, inner)
+    half = _half_type(x, "x")
+    p = _lib.GatedExpertsParams()
+    p.x = _operand(x, "x", (slots, 2 * inner), (x.dtype,), dev)
+    p.w = _operand(w, "w", (experts, hidden, inner), (torch.int8,), dev)
+    p.w_scales = _operand(w_scales, "w_scales", (experts, hidden), (torch.float32,), dev)
+    p.out = _operand(out, "out", (m, hidden), (x.dtype,), dev)
+    p.slot_indices = _operand(slot_indices, "slot_indices", (slots,), (torch.int32,), dev)
+    p.routing_offsets = _operand(routing_offsets, "routing_offsets", (experts,), (torch.int32,), dev)
+    p.topk_weights = _operand(topk_weights, "topk_weights", (m, top_k), (torch.float32,), dev)
+    if residual is not None:
+        p.residual = _operand(residual, "residual", (m, hidden), (x.dtype,), dev)
+    if smooth_scale is not None:
+        p.smooth = _operand(smooth_scale, "smooth_scale", (1, inner) if smooth_scale.dim() == 2 else (inner,),
+                            (torch.float32,), dev)
+    need = get_gated_experts_workspace_bytes(slots, inner, hidden)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    elif not workspace.is_cuda or workspace.device != dev or workspace.dtype != torch.uint8 or workspace.numel() < need:
+        _fail(f"workspace must be a uint8 tensor on {dev} of at least {need} bytes")
+    p.workspace, p.workspace_bytes = workspace.data_ptr(), workspace.numel()
+    p.type, p.num_tokens, p.top_k, p.num_experts, p.inner, p.hidden = half, m, top_k, experts, inner, hidden
+    p.activation, p.max_val, p.block_size = _activation(activation), max_val, block_size
+    p.host_signal_sync = _sync_word(host_signal_sync)
+    _call_on(dev, "pb2_gated_experts", p, "gated_experts")

@@ -61,6 +61,19 @@ def _device_index(t: torch.Tensor) -> int:
     return t.device.index if t.device.index is not None else torch.cuda.current_device()
 
 
+def _call_on(device: torch.device, name: str, params, op: str) -> None:
+    """Queue a C-ABI call on ``device``'s current stream, with the caller's
+    current device left as it was."""
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    params.device = index
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if torch.cuda.current_device() == index:
+        _lib.call(name, params, stream, op)
+        return
+    with torch.cuda.device(device):
+        _lib.call(name, params, stream, op)
+
+
 def make_pow_target_tensor(value: int, device="cuda") -> torch.Tensor:
     """Create a pow_target tensor (8 x uint32, little-endian words) from a
     uint256 integer value (pearl_gemm_interface.py:8-16)."""

@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .pearl_gemm_interface import _device_index, _fail, _stream
+from .pearl_gemm_interface import _call_on, _device_index, _fail, _stream
 
 DEFAULT_HADAMARD_BLOCK_SIZE = 16  # hadamard.py:520
 
@@ -65,6 +65,53 @@ def quantize(
         _lib.call("pb2_quantize", p, _stream(x.device), "quantize")
 
 
+def quantize_gated(x, xq, xq_scales, *, activation: str = "silu", row_index=None, smooth_scale=None,
+                   max_val: int = 127, block_size: int = 0) -> None:
+    """The quantized gated activation of an MLP (no reference counterpart):
+    rows of ``x`` (rows, 2 N), bf16 or fp16, hold N gate and then N up values;
+    in float32
+
+        v = act(gate) * up, block-Hadamard transform of width block_size
+            (as ``quantize``; 0 = none), times smooth_scale (1, N) or (N,)
+        xq_scales = amax_row(v) * fl(1 / max_val)
+        xq = rint(v * (max_val / amax_row(v))), 0 for a row of zeros
+
+    xq (M, N) int8, xq_scales (M,) or (M, 1) float32.  With ``row_index``
+    ((M,) int32) row i of the result is row row_index[i] of x -- a MoE
+    layer's slots in expert order -- and an index outside x gives a row of
+    zeros; without it M = rows."""
+    from .linear import _activation, _half_type, _operand
+
+    if x.dim() != 2 or x.shape[1] % 2:
+        _fail("x must be 2D (M, 2 N): gate values, then up values")
+    rows, N = x.shape[0], x.shape[1] // 2
+    dev = x.device
+    half = _half_type(x, "x")
+    M = rows if row_index is None else row_index.numel()
+    p = _lib.GatedQuantParams()
+    p.x = _operand(x, "x", (rows, 2 * N), (x.dtype,), dev)
+    p.xq = _operand(xq, "xq", (M, N), (torch.int8,), dev)
+    p.scales = _operand(xq_scales, "xq_scales", (M, 1) if xq_scales.dim() == 2 else (M,), (torch.float32,), dev)
+    if row_index is not None:
+        p.row_index = _operand(row_index, "row_index", (M,), (torch.int32,), dev)
+    if smooth_scale is not None:
+        p.smooth = _operand(smooth_scale, "smooth_scale", (1, N) if smooth_scale.dim() == 2 else (N,),
+                            (torch.float32,), dev)
+    if N % 8:
+        _fail(f"the row length must be a multiple of 8, got {N}")
+    if not 0 < max_val <= 127:
+        _fail(f"max_val must be in 1..127, got {max_val}")
+    _check_block(block_size, N)
+    p.x_type, p.m, p.n, p.x_rows, p.activation = half, M, N, rows, _activation(activation)
+    p.max_val, p.block_size = max_val, block_size
+    _call_on(dev, "pb2_quantize_gated", p, "quantize_gated")
+
+
+def _check_block(block_size: int, n: int) -> None:
+    if block_size and (block_size not in (8, 16, 32, 64, 128, 256) or n % block_size):
+        raise ValueError(f"block_size must be 0 or a power of 2 in 8..256 that divides {n}, got {block_size}")
+
+
 def rcp_approx_f32(x: torch.Tensor) -> torch.Tensor:
     """rcp.approx.ftz.f32 of every element of a float32 CUDA tensor: the
     approximate reciprocal ``quantize`` takes for its inverse scale, as the
@@ -81,4 +128,4 @@ def rcp_approx_f32(x: torch.Tensor) -> torch.Tensor:
     return out
 
 
-__all__ = ["quantize", "rcp_approx_f32", "DEFAULT_HADAMARD_BLOCK_SIZE"]
+__all__ = ["quantize", "quantize_gated", "rcp_approx_f32", "DEFAULT_HADAMARD_BLOCK_SIZE"]

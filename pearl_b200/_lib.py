@@ -234,6 +234,17 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+_functions: dict = {}
+
+
+def function(name: str):
+    """The library's entry point of this name, looked up once."""
+    f = _functions.get(name)
+    if f is None:
+        f = _functions[name] = getattr(load(), name)
+    return f
+
+
 def check(status: int, op: str) -> None:
     if status == PB2_OK:
         return

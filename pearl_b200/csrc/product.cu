@@ -17,13 +17,14 @@
 namespace pb2 {
 namespace {
 
-constexpr int kTileRows = 128;  // rows of C per CTA
+constexpr int kCtaRows = 128;  // rows of C per CTA
 constexpr int kTileK = 128;     // bytes of K per stage
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 32 * (2 + kEpiWarps);
 constexpr int kMaxStages = 10;
 constexpr int kBoxBytes = 32 * 128;  // an epilogue warp's 32 rows x 64 16-bit columns
 constexpr int kMaxGroups = 256;
+constexpr uint16_t kPairMask = 0x3;
 
 enum { kBiasNone = 0, kBiasF32 = 1, kBiasHalf = 2 };  // kBiasHalf: C's type
 
@@ -144,11 +145,13 @@ __device__ __forceinline__ void build_groups(const ProductArgs& a, ProductSmem& 
   __syncthreads();
 }
 
-template <int kTN, bool kGrouped>
+template <bool kPair, int kTN, bool kGrouped>
 __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ ProductArgs a) {
-  constexpr int kBBytes = kTN * kTileK;
+  constexpr int kRows = kPair ? 2 * kCtaRows : kCtaRows;  // rows of a tile
+  constexpr int kBRows = kPair ? kTN / 2 : kTN;           // rows of B this CTA loads
+  constexpr int kBBytes = kBRows * kTileK;
   constexpr int kHalf = kTN / 2;  // columns of an epilogue warp
-  constexpr uint32_t kIdesc = idesc_i8(kTileRows, kTN);
+  constexpr uint32_t kIdesc = idesc_i8(kRows, kTN);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int stage_bytes = a.a_bytes + kBBytes;
@@ -157,6 +160,8 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
   ProductSmem& S = *reinterpret_cast<ProductSmem*>(col_mem + kEpiWarps * kHalf);
   volatile int* abort_flag = &S.abort_flag;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t rank = kPair ? cluster_ctarank() : 0;  // 0 issues the MMAs
+  const int first = kPair ? blockIdx.x >> 1 : blockIdx.x, stride = kPair ? gridDim.x >> 1 : gridDim.x;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < a.stages; ++i) {
@@ -165,7 +170,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&S.acc_full[i], 1);
-      mbar_init(&S.acc_empty[i], kEpiWarps);
+      mbar_init(&S.acc_empty[i], kPair ? 2 * kEpiWarps : kEpiWarps);
     }
     mbar_init(&S.drain, 1);
     S.abort_flag = 0;
@@ -174,17 +179,23 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
     tma_prefetch(&a.tmB);
   }
   if (warp == 1) {
-    tmem_alloc(&S.tmem_base, 2 * kTN);
-    tmem_relinquish();
+    if constexpr (kPair) {
+      tmem_alloc_2sm(&S.tmem_base, 2 * kTN);
+      tmem_relinquish_2sm();
+    } else {
+      tmem_alloc(&S.tmem_base, 2 * kTN);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (kPair) cluster_sync_all();  // both CTAs' barriers exist before a remote arrive or 2-SM load
   tc_fence_after();
   griddep_wait();
   griddep_launch_dependents();
-  if constexpr (kGrouped) build_groups<kTileRows>(a, S);
+  if constexpr (kGrouped) build_groups<kRows>(a, S);
   const uint32_t tmem = S.tmem_base;
-  const int tiles = kGrouped ? S.tile0[a.groups] : (a.M + kTileRows - 1) / kTileRows * a.tiles_n;
+  const int tiles = kGrouped ? S.tile0[a.groups] : (a.M + kRows - 1) / kRows * a.tiles_n;
   const int kblocks = (a.K + kTileK - 1) / kTileK;
 
   if (warp == 0) {
@@ -193,16 +204,23 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
     bool ok = true;
     int st = 0, issued = 0;
     uint32_t phase = 1;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      const Tile w = tile_at<kGrouped, kTileRows>(a, S, t);
-      const int brow = w.group * a.N + w.tn * kTN;
+    for (int t = first; t < tiles && ok; t += stride) {
+      const Tile w = tile_at<kGrouped, kRows>(a, S, t);
+      const int arow = w.row0 + int(rank) * kCtaRows;
+      const int brow = w.group * a.N + w.tn * kTN + int(rank) * kBRows;
       for (int kb = 0; kb < kblocks; ++kb) {
         if (!(ok = mbar_wait_warp(&S.empty[st], phase, abort_flag, a.sync, a.wait_budget, a.wait_hint_ns))) break;
         if (leader) {
           uint8_t* sa = ring + st * stage_bytes;
-          mbar_arrive_expect_tx(&S.full[st], stage_bytes);
-          tma_load_2d(&a.tmA, &S.full[st], sa, kb * kTileK, w.row0);
-          tma_load_2d(&a.tmB, &S.full[st], sa + a.a_bytes, kb * kTileK, brow);
+          if constexpr (kPair) {  // the leader's barrier counts both CTAs' bytes
+            if (rank == 0) mbar_arrive_expect_tx(&S.full[st], 2 * stage_bytes);
+            tma_load_2d_2sm(&a.tmA, &S.full[st], sa, kb * kTileK, arow);
+            tma_load_2d_2sm(&a.tmB, &S.full[st], sa + a.a_bytes, kb * kTileK, brow);
+          } else {
+            mbar_arrive_expect_tx(&S.full[st], stage_bytes);
+            tma_load_2d(&a.tmA, &S.full[st], sa, kb * kTileK, arow);
+            tma_load_2d(&a.tmB, &S.full[st], sa + a.a_bytes, kb * kTileK, brow);
+          }
         }
         issued = min(issued + 1, a.stages);
         if (++st == a.stages) { st = 0; phase ^= 1; }
@@ -218,29 +236,39 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       }
     }
   } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer
-    bool ok = true;
-    int st = 0, n = 0;
-    uint32_t phase = 0;
-    const uint32_t sbase = smem_u32(ring);
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++n) {
-      const int slot = n & 1;
-      if (!(ok = mbar_wait_warp(&S.acc_empty[slot], ((n >> 1) & 1) ^ 1, abort_flag, a.sync, a.wait_budget, a.wait_hint_ns)))
-        break;
-      tc_fence_after();
-      for (int kb = 0; kb < kblocks; ++kb) {
-        if (!(ok = mbar_wait_warp(&S.full[st], phase, abort_flag, a.sync, a.wait_budget, a.wait_hint_ns))) break;
+    // ------------------------------------------------------------ MMA issuer (the pair's leader)
+    if (rank == 0) {
+      bool ok = true;
+      int st = 0, n = 0;
+      uint32_t phase = 0;
+      const uint32_t sbase = smem_u32(ring);
+      for (int t = first; t < tiles && ok; t += stride, ++n) {
+        const int slot = n & 1;
+        if (!(ok = mbar_wait_warp(&S.acc_empty[slot], ((n >> 1) & 1) ^ 1, abort_flag, a.sync, a.wait_budget, a.wait_hint_ns)))
+          break;
         tc_fence_after();
-        const uint64_t ad = sdesc_sw128(sbase + st * stage_bytes);
-        const uint64_t bd = sdesc_sw128(sbase + st * stage_bytes + a.a_bytes);
-        umma_i8_stage_warp(tmem + slot * kTN, ad, bd, kIdesc, kb != 0, &S.empty[st]);
-        if (++st == a.stages) { st = 0; phase ^= 1; }
+        for (int kb = 0; kb < kblocks; ++kb) {
+          if (!(ok = mbar_wait_warp(&S.full[st], phase, abort_flag, a.sync, a.wait_budget, a.wait_hint_ns))) break;
+          tc_fence_after();
+          const uint64_t ad = sdesc_sw128(sbase + st * stage_bytes);
+          const uint64_t bd = sdesc_sw128(sbase + st * stage_bytes + a.a_bytes);
+          if constexpr (kPair)
+            umma_8bit_2sm_stage_warp<4, false>(tmem + slot * kTN, ad, bd, kIdesc, kb != 0, &S.empty[st], kPairMask);
+          else
+            umma_i8_stage_warp(tmem + slot * kTN, ad, bd, kIdesc, kb != 0, &S.empty[st]);
+          if (++st == a.stages) { st = 0; phase ^= 1; }
+        }
+        if (ok) {
+          if constexpr (kPair) umma_commit_2sm_warp(&S.acc_full[slot], kPairMask);
+          else umma_commit_warp(&S.acc_full[slot]);
+        }
       }
-      if (ok) umma_commit_warp(&S.acc_full[slot]);
-    }
-    umma_commit_warp(&S.drain);  // every MMA has retired before TMEM is released
-    const long long t0 = clock64();
-    while (!mbar_test(&S.drain, 0) && clock64() - t0 < 100000000LL) {
+      // Every MMA has retired before TMEM is released.
+      if constexpr (kPair) umma_commit_2sm_warp(&S.drain, 0x1);
+      else umma_commit_warp(&S.drain);
+      const long long t0 = clock64();
+      while (!mbar_test(&S.drain, 0) && clock64() - t0 < 100000000LL) {
+      }
     }
   } else {
     // ------------------------------------------------------------ epilogue
@@ -251,12 +279,22 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
     const bool f16 = a.c_f16;
     bool ok = true;
     int n = 0;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++n) {
-      const Tile w = tile_at<kGrouped, kTileRows>(a, S, t);
+    const uint32_t leader_empty = kPair ? mapa(&S.acc_empty[0], 0) : 0;
+    auto release = [&](int slot) {  // the warp's loads of the accumulator have completed (wait::ld)
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (kPair) mbar_arrive_relaxed_cluster(leader_empty + 8 * slot);
+        else mbar_arrive(&S.acc_empty[slot]);
+      }
+    };
+    for (int t = first; t < tiles && ok; t += stride, ++n) {
+      const Tile w = tile_at<kGrouped, kRows>(a, S, t);
       const int slot = n & 1;
-      const int lrow = 32 * q + lane;
+      const int q0 = int(rank) * kCtaRows + 32 * q;  // the warp's first row in the tile
+      const int lrow = q0 + lane;
       const int c0 = w.tn * kTN + h * kHalf;
-      const bool live = 32 * q < w.rows && c0 < a.N;  // this warp has something to store
+      const bool live = q0 < w.rows && c0 < a.N;  // this warp has something to store
       float rs = 0.f;
       long long dst = -1;
       if (live) {
@@ -287,9 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       tc_fence_after();
       const uint32_t taddr = tmem + slot * kTN + (uint32_t(32 * q) << 16) + h * kHalf;
       if (!live) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&S.acc_empty[slot]);
+        release(slot);
         continue;
       }
 #pragma unroll 1
@@ -300,9 +336,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         tmem_ld32(taddr + 64 * ch + 32, v + 32);
         tmem_wait_ld_into2(v, v + 32);
         if (ch == kHalf / 64 - 1) {  // the accumulator is free for the tile after next
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&S.acc_empty[slot]);
+          release(slot);
         }
         const float2* cc = cols + 64 * ch;
         const int col0 = c0 + 64 * ch;
@@ -385,41 +419,84 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       }
     }
   }
+  // Neither CTA of a pair leaves while its peer can still address its
+  // barriers or tensor memory.
   tc_fence_before();
   __syncthreads();
+  if constexpr (kPair) cluster_sync_all();
   tc_fence_after();
   if (warp == 1) {
     __syncwarp();
-    tmem_dealloc(tmem, 2 * kTN);
+    if constexpr (kPair) tmem_dealloc_2sm(tmem, 2 * kTN);
+    else tmem_dealloc(tmem, 2 * kTN);
   }
 }
 
 // ------------------------------------------------------------------ host
 bool al16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-template <int kTN, bool kGrouped>
-int launch_product(ProductArgs& a, const int8_t* A, const int8_t* B, int64_t max_tiles_m, int device, cudaStream_t s) {
-  const int box_rows = std::min(kTileRows, (a.M + 7) / 8 * 8);
+// CTA pairs that can be resident at once (SM pairs of one GPC).
+int resident_pairs(int device, const void* kern, int smem) {
+  static int cached[64] = {0};
+  int& n = cached[device & 63];
+  if (n == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2, 1, 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = size_t(smem);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    if (cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg) != cudaSuccess || clusters <= 0) {
+      cudaGetLastError();
+      clusters = std::max(1, sm_count(device) / 2);
+    }
+    n = clusters;
+  }
+  return n;
+}
+
+template <bool kPair, int kTN, bool kGrouped>
+int launch_product(ProductArgs& a, const int8_t* A, const int8_t* B, int device, cudaStream_t s) {
+  constexpr int kRows = kPair ? 2 * kCtaRows : kCtaRows;
+  constexpr int kBRows = kPair ? kTN / 2 : kTN;
+  const int box_rows = std::min(kCtaRows, (a.M + 7) / 8 * 8);
   int st;
   if ((st = make_tmap_2d(&a.tmA, A, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, a.M, kTileK, box_rows,
                          CU_TENSOR_MAP_SWIZZLE_128B)) ||
       (st = make_tmap_2d(&a.tmB, B, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, uint64_t(std::max(a.groups, 1)) * a.N, kTileK,
-                         kTN, CU_TENSOR_MAP_SWIZZLE_128B)))
+                         kBRows, CU_TENSOR_MAP_SWIZZLE_128B)))
     return st;
   a.a_bytes = box_rows * kTileK;
   a.tiles_n = (a.N + kTN - 1) / kTN;
   a.raster = 8;
   const int fixed = 1024 + kEpiWarps * (kBoxBytes + kTN / 2 * 8) + int(sizeof(ProductSmem));
-  a.stages = std::min(kMaxStages, (232448 - fixed) / (a.a_bytes + kTN * kTileK));
+  a.stages = std::min(kMaxStages, (232448 - fixed) / (a.a_bytes + kBRows * kTileK));
   a.wait_budget = wait_budget_cycles();
   a.wait_hint_ns = suspend_hint_ns(a.wait_budget);
-  const int smem = fixed + a.stages * (a.a_bytes + kTN * kTileK);
-  auto kern = product_kernel<kTN, kGrouped>;
+  const int smem = fixed + a.stages * (a.a_bytes + kBRows * kTileK);
+  auto kern = product_kernel<kPair, kTN, kGrouped>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return launch_status();
-  const int sms = sm_count(device) > 0 ? sm_count(device) : 148;
-  const int grid = int(std::max<int64_t>(1, std::min<int64_t>(max_tiles_m * a.tiles_n, sms)));
-  return launch_programmatic(kern, dim3(unsigned(grid)), kThreads, smem, s, 1, a);
+  // Row tiles: exact without groups; with them, whose sizes only the device
+  // knows, at most one ragged tile a group beyond the whole ones.
+  const int64_t tiles_m = kGrouped ? int64_t(a.M) / kRows + std::min(a.groups, a.M) : (int64_t(a.M) + kRows - 1) / kRows;
+  const int most = kPair ? resident_pairs(device, reinterpret_cast<const void*>(kern), smem)
+                         : std::max(1, sm_count(device));
+  const int64_t ctas = std::min<int64_t>(tiles_m * a.tiles_n, most) * (kPair ? 2 : 1);
+  return launch_programmatic(kern, dim3(unsigned(ctas)), kThreads, smem, s, kPair ? 2 : 1, a);
+}
+
+template <bool kGrouped>
+int run_product(ProductArgs& a, const int8_t* A, const int8_t* B, int device, cudaStream_t s) {
+  const int64_t rows = kGrouped ? a.M / a.groups : a.M;
+  if (rows > kCtaRows) return launch_product<true, 256, kGrouped>(a, A, B, device, s);
+  return launch_product<false, 128, kGrouped>(a, A, B, device, s);
 }
 
 // out[t] = residual[t] + sum_j w[t, j] * slots[t * top_k + j], f32 sums in
@@ -512,8 +589,7 @@ extern "C" int pb2_gemm_epilogue(const pb2_gemm_epilogue_params* pp, void* strea
   a.K = int(p.k);
   a.vec = p.n % 8 == 0 && al16(p.C) && al16(p.residual);
   a.sync = static_cast<SignalSync*>(p.host_signal_sync);
-  return launch_product<128, false>(a, p.A, p.B, (p.m + kTileRows - 1) / kTileRows, p.device,
-                                    static_cast<cudaStream_t>(stream));
+  return run_product<false>(a, p.A, p.B, p.device, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int pb2_gemm_grouped(const pb2_gemm_grouped_params* pp, void* stream) {
@@ -546,8 +622,7 @@ extern "C" int pb2_gemm_grouped(const pb2_gemm_grouped_params* pp, void* stream)
   a.c_dst_rows = p.c_row_index ? p.c_rows : p.m;
   a.vec = p.n % 8 == 0 && al16(p.C);
   a.sync = static_cast<SignalSync*>(p.host_signal_sync);
-  const int64_t tiles_m = p.m / kTileRows + std::min(p.num_experts, p.m);  // at most
-  return launch_product<128, true>(a, p.A, p.B, tiles_m, p.device, static_cast<cudaStream_t>(stream));
+  return run_product<true>(a, p.A, p.B, p.device, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int pb2_combine_slots(const pb2_combine_params* pp, void* stream) {

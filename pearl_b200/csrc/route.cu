@@ -99,15 +99,26 @@ __device__ __forceinline__ void load_lane(const RouteArgs& a, int64_t row, int l
 }
 
 __device__ __forceinline__ uint32_t order_key(float x) {
-  if (x != x) x = -INFINITY;
-  const uint32_t b = __float_as_uint(x + 0.0f);  // -0 and +0 tie
-  return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
+  const int b = __float_as_int(clean(x) + 0.0f);  // -0 and +0 tie
+  return uint32_t(b) ^ (uint32_t(b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k ^ (k >> 31 ? 0x80000000u : 0xffffffffu));
 }
 
 __device__ __forceinline__ float sigmoid_exact(float x) { return x == -INFINITY ? 0.f : 1.0f / (1.0f + expf(-x)); }
+
+// e^(v - top) with 0 for a masked logit and 1 for the top one (also where
+// both are infinite).
+__device__ __forceinline__ float softmax_term(float v, float top) {
+  return v == -INFINITY ? 0.f : v == top ? 1.f : __expf(v - top);
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+  return v;
+}
 
 // Keys of a lane in descending order: minimal networks of 0, 1, 5 and 19
 // comparators.
@@ -142,27 +153,41 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const RouteArgs
   const int64_t row = int64_t(t) * a.experts;
   float x[kPer];
   load_lane<kPer>(a, row, lane, x);
-  // Softmax statistics.
+  // The row's softmax statistics, where they are needed: renormalized
+  // weights are a softmax over the chosen experts alone.
   float top = -INFINITY, sum = 0.f;
-  if (!a.sigmoid) {
+  const bool full = !a.sigmoid && (!a.renorm || a.bias);
+  if (full) {
 #pragma unroll
     for (int j = 0; j < kPer; ++j) top = fmaxf(top, x[j]);
     top = key_value(__reduce_max_sync(kAll, order_key(top)));
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) sum += x[j] == -INFINITY ? 0.f : x[j] == top ? 1.f : __expf(x[j] - top);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
+    for (int j = 0; j < kPer; ++j) sum += softmax_term(x[j], top);
+    sum = warp_sum(sum);
   }
   auto score = [&](float v) {
     if (a.sigmoid) return sigmoid_exact(v);
-    return v == -INFINITY ? 0.f : (v == top ? 1.f : expf(v - top)) / sum;
+    return softmax_term(v, top) / sum;
   };
   uint32_t key[kPer];
+  if (a.bias) {
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    const int e = lane * kPer + j;
-    key[j] = e >= a.experts ? kOut : order_key(x[j] == -INFINITY || !a.bias ? x[j] : score(x[j]) + a.bias[e]);
-    s_key[warp][e] = key[j];
+    for (int j = 0; j < kPer; ++j) {
+      const int e = lane * kPer + j;
+      key[j] = e >= a.experts ? kOut : order_key(x[j] == -INFINITY ? x[j] : score(x[j]) + a.bias[e]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) key[j] = lane * kPer + j >= a.experts ? kOut : order_key(x[j]);
+  }
+  if constexpr (kPer == 1) {
+    s_key[warp][lane] = key[0];
+  } else if constexpr (kPer == 2) {
+    *reinterpret_cast<uint2*>(&s_key[warp][2 * lane]) = make_uint2(key[0], key[1]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kPer; j += 4)
+      *reinterpret_cast<uint4*>(&s_key[warp][lane * kPer + j]) = make_uint4(key[j], key[j + 1], key[j + 2], key[j + 3]);
   }
   if (kGroups && a.group_lanes == 0) {
     __syncwarp();
@@ -236,42 +261,44 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const RouteArgs
       }
     }
   }
-  // Lane r learns the r-th chosen key and the lane that held it.
-  uint32_t my_key = 0;
-  int my_lane = lane;
+  // Lane r learns the r-th chosen key and which lanes' heads it was (the
+  // lowest of them gives it up).
+  uint32_t my_key = 0, my_heads = 0;
+  const uint32_t bit = 1u << lane, up_to = bit | (bit - 1u);
   for (int r = 0; r < a.top_k; ++r) {
     const uint32_t best = __reduce_max_sync(kAll, key[0]);
-    const int from = __ffs(__ballot_sync(kAll, key[0] == best)) - 1;
-    if (lane == r) { my_key = best; my_lane = from; }
-    if (lane == from) {
+    const uint32_t heads = __ballot_sync(kAll, key[0] == best);
+    const bool mine = (heads & up_to) == bit;
+    my_key = lane == r ? best : my_key;
+    my_heads = lane == r ? heads : my_heads;
 #pragma unroll
-      for (int j = 0; j + 1 < kPer; ++j) key[j] = key[j + 1];
-      key[kPer - 1] = kOut;
-    }
+    for (int j = 0; j + 1 < kPer; ++j) key[j] = mine ? key[j + 1] : key[j];
+    key[kPer - 1] = mine ? kOut : key[kPer - 1];
   }
-  // Equal keys of one lane were popped in rounds that follow one another; the
-  // n-th of them is the n-th of the lane's experts with that key.
-  const unsigned same = __match_any_sync(kAll, lane < a.top_k ? my_lane : 32 + lane) & __match_any_sync(kAll, my_key);
-  int skip = __popc(same & ((1u << lane) - 1u));
+  // Equal keys of one lane follow one another in the rounds; the n-th of them
+  // is the n-th of the lane's experts with that key.
+  const int from = __ffs(my_heads) - 1;
+  const uint32_t last_key = __shfl_up_sync(kAll, my_key, 1);
+  const int last_from = __shfl_up_sync(kAll, from, 1);
+  const uint32_t again = __ballot_sync(kAll, lane > 0 && lane < a.top_k && my_key == last_key && from == last_from);
+  int skip = __clz(~(again << (31 - lane)));
   __syncwarp();
+  int id = 0;
+  float v = -INFINITY;
   if (lane < a.top_k) {
-    int id = my_lane * kPer;
 #pragma unroll
-    for (int j = kPer - 1; j >= 0; --j) {
-      // number of equal keys before j in the lane
-      int before = 0;
-#pragma unroll
-      for (int i = 0; i < j; ++i) before += s_key[warp][my_lane * kPer + i] == my_key;
-      if (s_key[warp][my_lane * kPer + j] == my_key && before == skip) id = my_lane * kPer + j;
-    }
-    float w = score(load_logit(a, row + id));
-    float total = w;
-    if (a.renorm) {
-      const unsigned chosen = a.top_k == 32 ? kAll : (1u << a.top_k) - 1u;
-      total = 0.f;
-      for (int r = 0; r < a.top_k; ++r) total += __shfl_sync(chosen, w, r);
-      w = total > 0.f ? w / total : 0.f;
-    }
+    for (int j = 0; j < kPer; ++j)
+      if (s_key[warp][from * kPer + j] == my_key && skip-- == 0) id = from * kPer + j;
+    v = load_logit(a, row + id);
+  }
+  if (!a.sigmoid && !full) top = key_value(__reduce_max_sync(kAll, order_key(v)));
+  float w = a.sigmoid ? sigmoid_exact(v) : full ? softmax_term(v, top) / sum : softmax_term(v, top);
+  if (lane >= a.top_k || !(w > 0.f)) w = 0.f;  // 0 / 0: a row that masks every expert
+  if (a.renorm) {
+    const float total = warp_sum(w);
+    w = total > 0.f ? w / total : 0.f;
+  }
+  if (lane < a.top_k) {
     a.weights[int64_t(t) * a.top_k + lane] = w * a.scaling;
     a.ids[int64_t(t) * a.top_k + lane] = id;
   }

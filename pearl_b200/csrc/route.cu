@@ -1,18 +1,16 @@
 // route.cu -- the router of a MoE layer: the top_k experts of every token and
 // their weights from the router's logits (see pb2_route_tokens).
 //
-// A warp per token; lane l holds the kPer = ceil(experts / 32) consecutive
-// experts from l * kPer on, so that the lowest lane with a key holds the
-// lowest expert with it.  Each lane sorts its keys (bare values: min and max
-// only); a round of the choice is then one warp-wide maximum of the lanes'
-// heads, one ballot and a pop in the winner's lane.  Which of the winner's
-// experts a key belongs to is looked up once at the end, one lane per chosen
-// expert, as are the scores: a softmax needs every exponential only for its
-// sum, sigmoids without a bias only those of the chosen.
+// kLanes lanes work on a token (a warp on 32 / kLanes of them); lane l of
+// them holds the kPer consecutive experts from l * kPer on, so that the
+// lowest lane with a key holds the lowest expert with it.  Each lane sorts
+// its keys (bare values: min and max only); a round of the choice is then a
+// maximum over the lanes' heads, one ballot and a pop in the winner's lane.
+// Which of the winner's experts a key belongs to is looked up once at the
+// end, one lane per chosen expert, as are the scores: sigmoids without a
+// bias are taken of the chosen alone, and renormalized softmax weights are a
+// softmax over the chosen, which needs no other exponential.
 //
-// Bound by instruction issue (a few hundred per token), not by the logits'
-// bytes: carrying indices through the rounds and computing all scores took
-// 27 us for 32768 tokens of 128 experts and 19 us for 4099 of 256 in groups.
 #include <algorithm>
 
 #include "pb2_epilogue.cuh"
@@ -47,51 +45,38 @@ __device__ __forceinline__ float load_logit(const RouteArgs& a, int64_t i) {
   return clean(half_at(a.logits, i, a.type == PB2_TYPE_F16));
 }
 
-// This lane's kPer logits of the row starting at element `row` (-inf past
-// the last expert).  a.vec: whole lanes and aligned rows, wide loads.
+// The kPer logits from e0 on of the row starting at element `row` (-inf past
+// the last expert).  a.vec: whole vectors of min(kPer, 4) logits, aligned.
 template <int kPer>
-__device__ __forceinline__ void load_lane(const RouteArgs& a, int64_t row, int lane, float* x) {
-  const int e0 = lane * kPer;
-  if (a.vec && e0 < a.experts) {
-    if (a.type == PB2_TYPE_F32) {
-      const float* p = static_cast<const float*>(a.logits) + row + e0;
-      if constexpr (kPer == 1) {
-        x[0] = p[0];
-      } else if constexpr (kPer == 2) {
-        const float2 v = *reinterpret_cast<const float2*>(p);
-        x[0] = v.x; x[1] = v.y;
-      } else {
+__device__ __forceinline__ void load_lane(const RouteArgs& a, int64_t row, int e0, float* x) {
+  constexpr int kVec = kPer < 4 ? kPer : 4;
+  if (kVec > 1 && a.vec) {
+    const bool f16 = a.type == PB2_TYPE_F16;
 #pragma unroll
-        for (int j = 0; j < kPer; j += 4) {
-          const float4 v = *reinterpret_cast<const float4*>(p + j);
-          x[j] = v.x; x[j + 1] = v.y; x[j + 2] = v.z; x[j + 3] = v.w;
-        }
-      }
-    } else {
-      const uint16_t* p = static_cast<const uint16_t*>(a.logits) + row + e0;
-      const bool f16 = a.type == PB2_TYPE_F16;
-      if constexpr (kPer == 1) {
-        x[0] = half_at(p, 0, f16);
-      } else {
-        uint32_t w[kPer / 2];
-        if constexpr (kPer == 2) {
-          w[0] = *reinterpret_cast<const uint32_t*>(p);
-        } else if constexpr (kPer == 4) {
-          const uint2 v = *reinterpret_cast<const uint2*>(p);
-          w[0] = v.x; w[1] = v.y;
+    for (int j = 0; j < kPer; j += kVec) {
+      float v[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      if (e0 + j < a.experts) {
+        if (a.type == PB2_TYPE_F32) {
+          const float* p = static_cast<const float*>(a.logits) + row + e0 + j;
+          if constexpr (kVec == 4) {
+            const float4 w = *reinterpret_cast<const float4*>(p);
+            v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+          } else {
+            const float2 w = *reinterpret_cast<const float2*>(p);
+            v[0] = w.x; v[1] = w.y;
+          }
         } else {
-          const uint4 v = *reinterpret_cast<const uint4*>(p);
-          w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-        }
-#pragma unroll
-        for (int j = 0; j < kPer / 2; ++j) {
-          const float2 f = unpack_half2(w[j], f16);
-          x[2 * j] = f.x; x[2 * j + 1] = f.y;
+          const uint16_t* p = static_cast<const uint16_t*>(a.logits) + row + e0 + j;
+          uint2 w = make_uint2(0u, 0u);
+          if constexpr (kVec == 4) w = *reinterpret_cast<const uint2*>(p);
+          else w.x = *reinterpret_cast<const uint32_t*>(p);
+          const float2 f = unpack_half2(w.x, f16), g = unpack_half2(w.y, f16);
+          v[0] = f.x; v[1] = f.y; v[2] = g.x; v[3] = g.y;
         }
       }
-    }
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) x[j] = clean(x[j]);
+      for (int i = 0; i < kVec; ++i) x[j + i] = clean(v[i]);
+    }
     return;
   }
 #pragma unroll
@@ -114,123 +99,132 @@ __device__ __forceinline__ float softmax_term(float v, float top) {
   return v == -INFINITY ? 0.f : v == top ? 1.f : __expf(v - top);
 }
 
-__device__ __forceinline__ float warp_sum(float v) {
+// Sum and maximum over the kLanes lanes of a token.
+template <int kLanes>
+__device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+  for (int o = kLanes / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+  return v;
+}
+template <int kLanes>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+  if constexpr (kLanes == 32) return __reduce_max_sync(kAll, v);
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(kAll, v, o));
   return v;
 }
 
-// Keys of a lane in descending order: minimal networks of 0, 1, 5 and 19
-// comparators.
+// Keys of a lane in descending order: Batcher's odd-even merge sort (1, 5,
+// 19, 63 comparators).
 template <int kPer>
-__device__ __forceinline__ void sort_lane(uint32_t* k) {
-  auto order = [&](int i, int j) {
-    const uint32_t hi = max(k[i], k[j]);
-    k[j] = min(k[i], k[j]);
-    k[i] = hi;
-  };
-  if constexpr (kPer == 2) order(0, 1);
-  if constexpr (kPer == 4) { order(0, 2); order(1, 3); order(0, 1); order(2, 3); order(1, 2); }
-  if constexpr (kPer == 8) {
-    order(0, 2); order(1, 3); order(4, 6); order(5, 7);
-    order(0, 4); order(1, 5); order(2, 6); order(3, 7);
-    order(0, 1); order(2, 3); order(4, 5); order(6, 7);
-    order(2, 4); order(3, 5);
-    order(1, 4); order(3, 6);
-    order(1, 2); order(3, 4); order(5, 6);
-  }
+__device__ __forceinline__ void sort_lane(uint32_t* key) {
+#pragma unroll
+  for (int p = 1; p < kPer; p *= 2)
+#pragma unroll
+    for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+      for (int j = k % p; j + k < kPer; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k; ++i)
+          if (i + j + k < kPer && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+            const uint32_t hi = max(key[i + j], key[i + j + k]);
+            key[i + j + k] = min(key[i + j], key[i + j + k]);
+            key[i + j] = hi;
+          }
 }
 
-template <int kPer, bool kGroups>
+template <int kLanes, int kPer, bool kGroups>
 __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const RouteArgs a) {
-  __shared__ __align__(16) uint32_t s_key[kRouteWarps][32 * kPer];
-  __shared__ uint32_t s_group[kRouteWarps][kGroups ? 32 * kPer : 1];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int t = blockIdx.x * kRouteWarps + warp;
+  constexpr int kTokens = 32 / kLanes * kRouteWarps;  // of a CTA
+  constexpr int kKept = kPer < kLanes ? kPer : kLanes;  // top_k <= kLanes: no lane gives up more keys
+  constexpr uint32_t kMask = kLanes == 32 ? kAll : (1u << kLanes) - 1u;
+  __shared__ __align__(16) uint32_t s_key[kTokens][kLanes * kPer];
+  __shared__ uint32_t s_group[kTokens][kGroups ? kLanes * kPer : 1];
+  const int lane = threadIdx.x % kLanes, slot = threadIdx.x / kLanes;
+  const int base = threadIdx.x % 32 - lane;  // the token's first lane in its warp
+  const int t = blockIdx.x * kTokens + slot;
+  const bool live = t < a.tokens;
   griddep_wait();
   griddep_launch_dependents();
-  if (t >= a.tokens) return;
-  const int64_t row = int64_t(t) * a.experts;
+  uint32_t* keys = s_key[slot];
+  const int64_t row = int64_t(live ? t : 0) * a.experts;
   float x[kPer];
-  load_lane<kPer>(a, row, lane, x);
-  // The row's softmax statistics, where they are needed: renormalized
-  // weights are a softmax over the chosen experts alone.
+  load_lane<kPer>(a, row, lane * kPer, x);
+  // The row's softmax statistics, where they are needed.
   float top = -INFINITY, sum = 0.f;
   const bool full = !a.sigmoid && (!a.renorm || a.bias);
   if (full) {
 #pragma unroll
     for (int j = 0; j < kPer; ++j) top = fmaxf(top, x[j]);
-    top = key_value(__reduce_max_sync(kAll, order_key(top)));
+    top = key_value(lanes_max<kLanes>(order_key(top)));
 #pragma unroll
     for (int j = 0; j < kPer; ++j) sum += softmax_term(x[j], top);
-    sum = warp_sum(sum);
+    sum = lanes_sum<kLanes>(sum);
   }
-  auto score = [&](float v) {
-    if (a.sigmoid) return sigmoid_exact(v);
-    return softmax_term(v, top) / sum;
-  };
   uint32_t key[kPer];
   if (a.bias) {
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       const int e = lane * kPer + j;
-      key[j] = e >= a.experts ? kOut : order_key(x[j] == -INFINITY ? x[j] : score(x[j]) + a.bias[e]);
+      float c = x[j];
+      if (c != -INFINITY) c = (a.sigmoid ? sigmoid_exact(c) : softmax_term(c, top) / sum) + a.bias[e];
+      key[j] = e >= a.experts ? kOut : order_key(c);
     }
   } else {
 #pragma unroll
     for (int j = 0; j < kPer; ++j) key[j] = lane * kPer + j >= a.experts ? kOut : order_key(x[j]);
   }
   if constexpr (kPer == 1) {
-    s_key[warp][lane] = key[0];
+    keys[lane] = key[0];
   } else if constexpr (kPer == 2) {
-    *reinterpret_cast<uint2*>(&s_key[warp][2 * lane]) = make_uint2(key[0], key[1]);
+    *reinterpret_cast<uint2*>(keys + 2 * lane) = make_uint2(key[0], key[1]);
   } else {
 #pragma unroll
     for (int j = 0; j < kPer; j += 4)
-      *reinterpret_cast<uint4*>(&s_key[warp][lane * kPer + j]) = make_uint4(key[j], key[j + 1], key[j + 2], key[j + 3]);
+      *reinterpret_cast<uint4*>(keys + lane * kPer + j) = make_uint4(key[j], key[j + 1], key[j + 2], key[j + 3]);
   }
   if (kGroups && a.group_lanes == 0) {
     __syncwarp();
     const int width = a.experts / a.groups;
-    // Group g's value in lane g % 32, element g / 32.
+    uint32_t* kept = s_group[slot];
+    // Group g's value in lane g % kLanes, element g / kLanes.
     uint32_t value[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int g = lane + 32 * i;
+      const int g = lane + kLanes * i;
       value[i] = kOut;
-      s_group[warp][g] = 0u;
+      kept[g] = 0u;
       if (g < a.groups) {
         uint32_t first = kOut, second = kOut;
         for (int j = 0; j < width; ++j) {
-          const uint32_t k = s_key[warp][g * width + j];
+          const uint32_t k = keys[g * width + j];
           second = max(second, min(first, k));
           first = max(first, k);
         }
         value[i] = a.bias && width > 1 ? order_key(key_value(first) + key_value(second)) : first;
       }
     }
-    __syncwarp();
     for (int r = 0; r < a.kept; ++r) {
       uint32_t best = value[0];
 #pragma unroll
       for (int i = 1; i < kPer; ++i) best = max(best, value[i]);
-      best = __reduce_max_sync(kAll, best);
-      unsigned at = 0x7fffffffu;
+      best = lanes_max<kLanes>(best);
+      uint32_t at = 0x7fffffffu;
 #pragma unroll
       for (int i = kPer - 1; i >= 0; --i)
-        if (value[i] == best) at = lane + 32 * i;
-      at = __reduce_min_sync(kAll, at);
+        if (value[i] == best) at = lane + kLanes * i;
+      at = ~lanes_max<kLanes>(~at);  // the lowest
 #pragma unroll
       for (int i = 0; i < kPer; ++i)
-        if (at == unsigned(lane + 32 * i)) { value[i] = kOut; s_group[warp][at] = 1u; }
+        if (at == uint32_t(lane + kLanes * i)) { value[i] = kOut; kept[at] = 1u; }
     }
     __syncwarp();
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       const int e = lane * kPer + j;
-      if (e < a.experts && !s_group[warp][e / width]) {
+      if (e < a.experts && !kept[e / width]) {
         key[j] = kOut;
-        s_key[warp][e] = kOut;
+        keys[e] = kOut;
       }
     }
   }
@@ -249,15 +243,15 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const RouteArgs
     const int group = lane / a.group_lanes;
     bool in = false;
     for (int r = 0; r < a.kept; ++r) {
-      const uint32_t best = __reduce_max_sync(kAll, value);
-      const int from = __ffs(__ballot_sync(kAll, value == best)) - 1;
-      if (from / a.group_lanes == group) { in = true; value = kOut; }
+      const uint32_t best = lanes_max<kLanes>(value);
+      const uint32_t heads = (__ballot_sync(kAll, value == best) >> base) & kMask;
+      if ((__ffs(heads) - 1) / a.group_lanes == group) { in = true; value = kOut; }
     }
     if (!in) {
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
         key[j] = kOut;
-        s_key[warp][lane * kPer + j] = kOut;
+        keys[lane * kPer + j] = kOut;
       }
     }
   }
@@ -266,21 +260,22 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const RouteArgs
   uint32_t my_key = 0, my_heads = 0;
   const uint32_t bit = 1u << lane, up_to = bit | (bit - 1u);
   for (int r = 0; r < a.top_k; ++r) {
-    const uint32_t best = __reduce_max_sync(kAll, key[0]);
-    const uint32_t heads = __ballot_sync(kAll, key[0] == best);
+    const uint32_t best = lanes_max<kLanes>(key[0]);
+    const uint32_t heads = (__ballot_sync(kAll, key[0] == best) >> base) & kMask;
     const bool mine = (heads & up_to) == bit;
     my_key = lane == r ? best : my_key;
     my_heads = lane == r ? heads : my_heads;
 #pragma unroll
-    for (int j = 0; j + 1 < kPer; ++j) key[j] = mine ? key[j + 1] : key[j];
-    key[kPer - 1] = mine ? kOut : key[kPer - 1];
+    for (int j = 0; j + 1 < kKept; ++j) key[j] = mine ? key[j + 1] : key[j];
+    key[kKept - 1] = mine ? kOut : key[kKept - 1];
   }
   // Equal keys of one lane follow one another in the rounds; the n-th of them
   // is the n-th of the lane's experts with that key.
   const int from = __ffs(my_heads) - 1;
-  const uint32_t last_key = __shfl_up_sync(kAll, my_key, 1);
-  const int last_from = __shfl_up_sync(kAll, from, 1);
-  const uint32_t again = __ballot_sync(kAll, lane > 0 && lane < a.top_k && my_key == last_key && from == last_from);
+  const uint32_t last_key = __shfl_up_sync(kAll, my_key, 1, kLanes);
+  const int last_from = __shfl_up_sync(kAll, from, 1, kLanes);
+  const uint32_t again =
+      __ballot_sync(kAll, lane > 0 && lane < a.top_k && my_key == last_key && from == last_from) >> base;
   int skip = __clz(~(again << (31 - lane)));
   __syncwarp();
   int id = 0;
@@ -288,27 +283,33 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const RouteArgs
   if (lane < a.top_k) {
 #pragma unroll
     for (int j = 0; j < kPer; ++j)
-      if (s_key[warp][from * kPer + j] == my_key && skip-- == 0) id = from * kPer + j;
+      if (keys[from * kPer + j] == my_key && skip-- == 0) id = from * kPer + j;
     v = load_logit(a, row + id);
   }
-  if (!a.sigmoid && !full) top = key_value(__reduce_max_sync(kAll, order_key(v)));
+  if (!a.sigmoid && !full) top = key_value(lanes_max<kLanes>(order_key(v)));
   float w = a.sigmoid ? sigmoid_exact(v) : full ? softmax_term(v, top) / sum : softmax_term(v, top);
   if (lane >= a.top_k || !(w > 0.f)) w = 0.f;  // 0 / 0: a row that masks every expert
   if (a.renorm) {
-    const float total = warp_sum(w);
+    const float total = lanes_sum<kLanes>(w);
     w = total > 0.f ? w / total : 0.f;
   }
-  if (lane < a.top_k) {
+  if (live && lane < a.top_k) {
     a.weights[int64_t(t) * a.top_k + lane] = w * a.scaling;
     a.ids[int64_t(t) * a.top_k + lane] = id;
   }
 }
 
-template <int kPer>
-int launch_route(const RouteArgs& a, cudaStream_t s) {
-  const dim3 grid(unsigned((a.tokens + kRouteWarps - 1) / kRouteWarps));
-  if (a.groups > 1) return launch_programmatic(route_kernel<kPer, true>, grid, 32 * kRouteWarps, 0, s, 1, a);
-  return launch_programmatic(route_kernel<kPer, false>, grid, 32 * kRouteWarps, 0, s, 1, a);
+template <int kLanes, int kPer>
+int launch_route(RouteArgs& a, cudaStream_t s) {
+  constexpr int kTokens = 32 / kLanes * kRouteWarps;
+  const int width = a.experts / a.groups, lanes = width / kPer;
+  a.group_lanes = a.groups > 1 && width % kPer == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
+  constexpr int kVec = kPer < 4 ? kPer : 4;
+  a.vec = a.experts % kVec == 0 &&
+          reinterpret_cast<uintptr_t>(a.logits) % (kVec * (a.type == PB2_TYPE_F32 ? 4 : 2)) == 0;
+  const dim3 grid(unsigned((a.tokens + kTokens - 1) / kTokens));
+  if (a.groups > 1) return launch_programmatic(route_kernel<kLanes, kPer, true>, grid, 32 * kRouteWarps, 0, s, 1, a);
+  return launch_programmatic(route_kernel<kLanes, kPer, false>, grid, 32 * kRouteWarps, 0, s, 1, a);
 }
 
 }  // namespace
@@ -346,15 +347,13 @@ extern "C" int pb2_route_tokens(const pb2_route_params* pp, void* stream) {
   a.renorm = p.renormalize;
   a.scaling = p.scaling;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int per = a.experts <= 32 ? 1 : a.experts <= 64 ? 2 : a.experts <= 128 ? 4 : 8;
-  const int lane_bytes = per * (a.type == PB2_TYPE_F32 ? 4 : 2);
-  a.vec = a.experts % per == 0 && reinterpret_cast<uintptr_t>(p.logits) % std::min(lane_bytes, 16) == 0;
-  const int width = a.experts / a.groups, lanes = width / per;
-  a.group_lanes = a.groups > 1 && width % per == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
-  switch (per) {
-    case 1: return launch_route<1>(a, s);
-    case 2: return launch_route<2>(a, s);
-    case 4: return launch_route<4>(a, s);
-    default: return launch_route<8>(a, s);
+  // As few lanes a token as the choice allows (a lane per chosen expert): the
+  // rounds' instructions then serve several tokens at once.
+  if (a.top_k <= 8 && a.experts <= 128) {
+    if (a.experts <= 32) return launch_route<8, 4>(a, s);
+    return a.experts <= 64 ? launch_route<8, 8>(a, s) : launch_route<8, 16>(a, s);
   }
+  if (a.top_k <= 16 && a.experts > 64) return a.experts <= 128 ? launch_route<16, 8>(a, s) : launch_route<16, 16>(a, s);
+  if (a.experts <= 64) return launch_route<32, 2>(a, s);
+  return a.experts <= 128 ? launch_route<32, 4>(a, s) : launch_route<32, 8>(a, s);
 }

@@ -589,8 +589,8 @@ typedef struct pb2_gemm_grouped_params {
 PB2_API int pb2_gemm_grouped(const pb2_gemm_grouped_params* p, void* stream);
 
 /* combine_slots: out[t] = residual[t] + sum over j of topk_weights[t, j] *
- * slots[t * top_k + j], f32 sums in the order of j, rounded once.  A slot
- * whose weight is 0 is not read.  residual may be out. */
+ * slots[t * top_k + j], f32 sums in the order of j, rounded once.  What a
+ * slot of weight 0 holds does not count.  residual may be out. */
 typedef struct pb2_combine_params {
   int device;
   const void* slots;         /* (num_tokens * top_k, n) of type */

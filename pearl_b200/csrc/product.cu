@@ -500,48 +500,60 @@ int run_product(ProductArgs& a, const int8_t* A, const int8_t* B, int device, cu
 }
 
 // out[t] = residual[t] + sum_j w[t, j] * slots[t * top_k + j], f32 sums in
-// slot order; a thread per 8 columns.
+// slot order.  HBM-bound (2 (top_k + 2) bytes a column): a block per token
+// and 256 vectors of eight columns, kCombineBatch slots' loads in flight at a
+// time with the residual's.
 struct CombineArgs {
   const void* slots;
   const float* weights;
   const void* residual;
   void* out;
-  long long tokens;
   int top_k, n, f16, vec;
 };
+constexpr int kCombineBatch = 4;
 
 __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
   griddep_wait();
   griddep_launch_dependents();
-  const int vecs = (a.n + 7) / 8;
-  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  const long long t = i / vecs;
-  if (t >= a.tokens) return;
-  const int col = int(i - t * vecs) * 8;
+  const int64_t t = blockIdx.x;
+  const int col = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
+  if (col >= a.n) return;
   const bool f16 = a.f16;
-  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  auto add = [&](const void* base, long long row, float w) {
+  auto load = [&](const void* base, int64_t row) {
     const uint16_t* p = static_cast<const uint16_t*>(base) + row * a.n + col;
-    if (a.vec) {
-      const uint4 r = *reinterpret_cast<const uint4*>(p);
-      const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
+    if (a.vec) return *reinterpret_cast<const uint4*>(p);
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 f = unpack_half2(rw[j], f16);
-        acc[2 * j] = fmaf(w, f.x, acc[2 * j]);
-        acc[2 * j + 1] = fmaf(w, f.y, acc[2 * j + 1]);
-      }
-    } else {
+    for (int j = 0; j < 8; ++j)
+      if (col + j < a.n) w[j / 2] |= uint32_t(p[j]) << (16 * (j & 1));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  };
+  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  auto add = [&](uint4 r, float w) {
+    const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (col + j < a.n) acc[j] = fmaf(w, half_at(p, j, f16), acc[j]);
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = unpack_half2(rw[j], f16);
+      acc[2 * j] = fmaf(w, f.x, acc[2 * j]);
+      acc[2 * j + 1] = fmaf(w, f.y, acc[2 * j + 1]);
     }
   };
-  for (int j = 0; j < a.top_k; ++j) {
-    const float w = a.weights[t * a.top_k + j];
-    if (w != 0.f) add(a.slots, t * a.top_k + j, w);
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  const uint4 res = a.residual ? load(a.residual, t) : zero;
+  for (int j0 = 0; j0 < a.top_k; j0 += kCombineBatch) {
+    uint4 r[kCombineBatch];
+    float w[kCombineBatch];
+#pragma unroll
+    for (int j = 0; j < kCombineBatch; ++j) {
+      const bool in = j0 + j < a.top_k;
+      r[j] = in ? load(a.slots, t * a.top_k + j0 + j) : zero;
+      w[j] = in ? a.weights[t * a.top_k + j0 + j] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < kCombineBatch; ++j)
+      if (w[j] != 0.f) add(r[j], w[j]);  // whatever a slot without weight holds does not count
   }
-  if (a.residual) add(a.residual, t, 1.0f);
+  if (a.residual) add(res, 1.0f);
   uint16_t* o = static_cast<uint16_t*>(a.out) + t * a.n + col;
   if (a.vec) {
     *reinterpret_cast<uint4*>(o) = make_uint4(pack_half2(acc[0], acc[1], f16), pack_half2(acc[2], acc[3], f16),
@@ -634,8 +646,9 @@ extern "C" int pb2_combine_slots(const pb2_combine_params* pp, void* stream) {
     return PB2_ERR_INVALID_ARGUMENT;
   if (!type16(p.type)) return PB2_ERR_INVALID_ARGUMENT;
   if (p.num_tokens > 0 && (!p.slots || !p.topk_weights || !p.out)) return PB2_ERR_INVALID_ARGUMENT;
-  const int64_t blocks = (p.num_tokens * ((p.n + 7) / 8) + 255) / 256;
-  if (blocks > INT32_MAX) return PB2_ERR_INVALID_ARGUMENT;
+  const int64_t vectors = (p.n + 7) / 8, threads = std::min<int64_t>(256, (vectors + 31) / 32 * 32);
+  const int64_t across = (vectors + threads - 1) / threads;
+  if (across > 65535) return PB2_ERR_INVALID_ARGUMENT;
   int st = set_device(p.device);
   if (st) return st;
   if (p.num_tokens == 0) return PB2_OK;
@@ -644,12 +657,12 @@ extern "C" int pb2_combine_slots(const pb2_combine_params* pp, void* stream) {
   a.weights = p.topk_weights;
   a.residual = p.residual;
   a.out = p.out;
-  a.tokens = p.num_tokens;
   a.top_k = int(p.top_k);
   a.n = int(p.n);
   a.f16 = p.type == PB2_TYPE_F16;
   a.vec = p.n % 8 == 0 && al16(p.slots) && al16(p.out) && al16(p.residual);
-  return launch_programmatic(combine_kernel, dim3(unsigned(blocks)), 256, 0, static_cast<cudaStream_t>(stream), 1, a);
+  return launch_programmatic(combine_kernel, dim3(unsigned(p.num_tokens), unsigned(across)), int(threads), 0,
+                             static_cast<cudaStream_t>(stream), 1, a);
 }
 
 extern "C" int64_t pb2_gated_experts_workspace_bytes(int64_t slots, int64_t inner, int64_t hidden) {

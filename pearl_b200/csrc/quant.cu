@@ -20,6 +20,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "pb2_epilogue.cuh"
 
@@ -215,9 +216,16 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) quant_rows_reg_kern
 }
 
 // act(gate) * up quantized: row i of xq from row index[i] of x, whose rows
-// hold a.n gate values and then a.n up values.  The products of the row stay in registers (kIters vectors of eight a
-// thread) between the max pass and the rounding pass: x is read once and the
-// activation computed once.
+// hold a.n gate values and then a.n up values.
+//
+// Bytes: 4 read and 1 written per product, so HBM bounds long rows as long as
+// the instructions stay few (about 13 per product: the exponential and the
+// reciprocal leave 16 a clock and SM, and rounding is one fma by 1.5 * 2^23,
+// whose sum holds the integer in its low byte).  The products of a row stay in
+// registers (kIters vectors of eight a thread) between the max pass and the
+// rounding pass: x is read once and the activation computed once.  Rows of at
+// most 1024 products take a warp each (no block barrier), longer ones a block
+// of just the threads they need.
 struct GatedArgs {
   QuantArgs q;
   const int32_t* index;
@@ -225,16 +233,14 @@ struct GatedArgs {
 };
 
 template <typename T, int kAct>
-__device__ __forceinline__ void gated_vec(const GatedArgs& a, const T* row, int vec, bool valid, float* v) {
+__device__ __forceinline__ void gated_vec(const GatedArgs& a, int vec, bool valid, uint4 g, uint4 u, float* v) {
+  constexpr bool f16 = std::is_same<T, __half>::value;
+  const uint32_t gw[4] = {g.x, g.y, g.z, g.w}, uw[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = 0.f;
-  if (valid) {
-    const uint4 g = *reinterpret_cast<const uint4*>(row + 8 * vec);
-    const uint4 u = *reinterpret_cast<const uint4*>(row + a.q.n + 8 * vec);
-    const T* ge = reinterpret_cast<const T*>(&g);
-    const T* ue = reinterpret_cast<const T*>(&u);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = activate<kAct>(to_f32<T>(ge[i])) * to_f32<T>(ue[i]);
+  for (int i = 0; i < 4; ++i) {
+    const float2 gf = unpack_half2(gw[i], f16), uf = unpack_half2(uw[i], f16);
+    v[2 * i] = activate<kAct>(gf.x) * uf.x;
+    v[2 * i + 1] = activate<kAct>(gf.y) * uf.y;
   }
   transform_vec(a.q, vec, v);
   if (a.q.smooth && valid) {
@@ -245,65 +251,90 @@ __device__ __forceinline__ void gated_vec(const GatedArgs& a, const T* row, int 
   }
 }
 
-__device__ __forceinline__ void store_quantized(const QuantArgs& a, int64_t row, int vec, const float* v, float inv) {
-  uint32_t packed[2] = {0u, 0u};
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float q = fminf(fmaxf(rintf(v[i] * inv), -a.max_val), a.max_val);
-    packed[i / 4] |= (uint32_t(int32_t(q)) & 0xFFu) << (8 * (i % 4));
-  }
-  *reinterpret_cast<uint2*>(a.xq + row * a.n + 8 * vec) = make_uint2(packed[0], packed[1]);
+// Four products of |v * inv| <= 127.5 as bytes: v * inv + 1.5 * 2^23 is
+// rounded to the nearest integer, ties to even, and keeps it in its low bits.
+__device__ __forceinline__ uint32_t round4(const float* v, float inv) {
+  constexpr float kShift = 12582912.0f;
+  const uint32_t b0 = __float_as_uint(fmaf(v[0], inv, kShift)), b1 = __float_as_uint(fmaf(v[1], inv, kShift));
+  const uint32_t b2 = __float_as_uint(fmaf(v[2], inv, kShift)), b3 = __float_as_uint(fmaf(v[3], inv, kShift));
+  return __byte_perm(__byte_perm(b0, b1, 0x0040), __byte_perm(b2, b3, 0x0040), 0x5410);
 }
 
-// kIters = 0: any row length, the products computed in both passes.
-template <typename T, int kAct, int kIters, int kThreads>
-__global__ void __launch_bounds__(kThreads, 1024 / kThreads) quant_gated_kernel(const GatedArgs a) {
-  __shared__ float warp_max[kThreads / 32];
+constexpr int kGatedIters = 4;
+constexpr int kGatedThreads = 512;
+
+// kWarpRow: a warp per row, else a block per row.  kKeep: the row's products
+// fit in the registers (kGatedIters vectors a thread), else both passes
+// compute them.
+template <typename T, int kAct, bool kWarpRow, bool kKeep>
+__global__ void __launch_bounds__(kWarpRow ? 256 : kGatedThreads, kWarpRow ? 4 : 2) quant_gated_kernel(const GatedArgs a) {
+  __shared__ float warp_max[kGatedThreads / 32];
   griddep_wait();
   griddep_launch_dependents();
-  const int64_t row = blockIdx.x;
+  const int64_t row = kWarpRow ? int64_t(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
+  if (kWarpRow && row >= a.q.m) return;
+  const int threads = kWarpRow ? 32 : blockDim.x, me = kWarpRow ? threadIdx.x % 32 : threadIdx.x;
   const int nvec = a.q.n / 8;
   const int src = a.index ? a.index[row] : int(row);
   const bool in = src >= 0 && src < a.x_rows;
-  const T* x = static_cast<const T*>(a.q.x) + (in ? int64_t(src) * 2 * a.q.n : 0);
+  const uint4* x = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q.x) + (in ? int64_t(src) * 2 * a.q.n : 0));
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
   float amax = 0.f;
-  constexpr int kKept = kIters > 0 ? kIters : 1;
-  float v[kKept][8];
-  const int iters = kIters > 0 ? kIters : (nvec + kThreads - 1) / kThreads;
+  float v[kKeep ? kGatedIters : 1][8];
+  const int iters = kKeep ? kGatedIters : (nvec + threads - 1) / threads;
+  if constexpr (kKeep) {
+    uint4 g[kGatedIters], u[kGatedIters];
+#pragma unroll
+    for (int it = 0; it < kGatedIters; ++it) {  // every load of the row in flight at once
+      const int vec = it * threads + me;
+      const bool valid = in && vec < nvec;
+      g[it] = valid ? x[vec] : zero;
+      u[it] = valid ? x[nvec + vec] : zero;
+    }
+#pragma unroll
+    for (int it = 0; it < kGatedIters; ++it)
+      gated_vec<T, kAct>(a, it * threads + me, it * threads + me < nvec, g[it], u[it], v[it]);
+  }
+  auto again = [&](int it) {  // the products of one vector, without kKeep
+    const int vec = it * threads + me;
+    const bool valid = in && vec < nvec;
+    gated_vec<T, kAct>(a, vec, vec < nvec, valid ? x[vec] : zero, valid ? x[nvec + vec] : zero, v[0]);
+  };
 #pragma unroll
   for (int it = 0; it < iters; ++it) {
-    float(&w)[8] = v[kIters > 0 ? it : 0];
-    const int vec = it * kThreads + threadIdx.x;
-    gated_vec<T, kAct>(a, x, vec, in && vec < nvec, w);
+    if constexpr (!kKeep) again(it);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(w[i]));
+    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[kKeep ? it : 0][i]));
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x / 32] = amax;
-  __syncthreads();
-  amax = 0.f;
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) amax = fmaxf(amax, warp_max[w]);
+  if constexpr (!kWarpRow) {
+    if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x / 32] = amax;
+    __syncthreads();
+    amax = 0.f;
+    for (int w = 0; w < blockDim.x / 32; ++w) amax = fmaxf(amax, warp_max[w]);
+  }
   const float inv = amax > 0.f ? a.q.max_val / amax : 0.f;
-  if (threadIdx.x == 0) a.q.scales[row] = amax * a.q.inv_max_val;
+  if (me == 0) a.q.scales[row] = amax * a.q.inv_max_val;
 #pragma unroll
   for (int it = 0; it < iters; ++it) {
-    float(&w)[8] = v[kIters > 0 ? it : 0];
-    const int vec = it * kThreads + threadIdx.x;
-    if constexpr (kIters == 0) gated_vec<T, kAct>(a, x, vec, in && vec < nvec, w);
-    if (vec < nvec) store_quantized(a.q, row, vec, w, inv);
+    const int vec = it * threads + me;
+    if constexpr (!kKeep) again(it);
+    const float* w = v[kKeep ? it : 0];
+    if (vec < nvec)
+      *reinterpret_cast<uint2*>(a.q.xq + row * a.q.n + 8 * vec) = make_uint2(round4(w, inv), round4(w + 4, inv));
   }
 }
 
 template <typename T, int kAct>
 int launch_gated(const GatedArgs& a, cudaStream_t s) {
   const int nvec = a.q.n / 8;
-  const dim3 grid(unsigned(a.q.m));
-  if (nvec <= 256) return launch_programmatic(quant_gated_kernel<T, kAct, 4, 64>, grid, 64, 0, s, 1, a);
-  if (nvec <= 1024) return launch_programmatic(quant_gated_kernel<T, kAct, 4, 256>, grid, 256, 0, s, 1, a);
-  if (nvec <= 2048) return launch_programmatic(quant_gated_kernel<T, kAct, 4, 512>, grid, 512, 0, s, 1, a);
-  return launch_programmatic(quant_gated_kernel<T, kAct, 0, 512>, grid, 512, 0, s, 1, a);
+  if (nvec <= 32 * kGatedIters)
+    return launch_programmatic(quant_gated_kernel<T, kAct, true, true>, dim3(unsigned((a.q.m + 7) / 8)), 256, 0, s, 1, a);
+  const int threads = ((nvec + kGatedIters - 1) / kGatedIters + 31) / 32 * 32;
+  if (threads <= kGatedThreads)
+    return launch_programmatic(quant_gated_kernel<T, kAct, false, true>, dim3(unsigned(a.q.m)), threads, 0, s, 1, a);
+  return launch_programmatic(quant_gated_kernel<T, kAct, false, false>, dim3(unsigned(a.q.m)), kGatedThreads, 0, s, 1, a);
 }
 
 template <typename T>

@@ -281,8 +281,8 @@ def combine_slots(slots, topk_weights, out, *, residual=None) -> None:
     """out[t] = residual[t] + sum_j topk_weights[t, j] * slots[t * top_k + j]:
     the token's experts added up in float32 in the order of j, rounded once.
     slots (m * top_k, n), out and ``residual`` (m, n), all bf16 or all fp16;
-    topk_weights (m, top_k) float32.  A slot whose weight is 0 is not read;
-    ``residual`` may be out itself."""
+    topk_weights (m, top_k) float32.  What a slot of weight 0 holds does
+    not count; ``residual`` may be out itself."""
     if topk_weights.dim() != 2 or out.dim() != 2:
         _fail("topk_weights and out must be 2D (m, top_k) and (m, n)")
     m, top_k = topk_weights.shape

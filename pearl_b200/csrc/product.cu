@@ -24,12 +24,11 @@ constexpr int kThreads = 32 * (2 + kEpiWarps);
 constexpr int kMaxStages = 10;
 constexpr int kBoxBytes = 32 * 128;  // an epilogue warp's 32 rows x 64 16-bit columns
 constexpr int kMaxGroups = 256;
-constexpr uint16_t kPairMask = 0x3;
 
 enum { kBiasNone = 0, kBiasF32 = 1, kBiasHalf = 2 };  // kBiasHalf: C's type
 
 struct ProductArgs {
-  CUtensorMap tmA;  // A (rows, K) int8
+  CUtensorMap tmA;  // A (rows, K) int8, boxes of box_rows rows
   CUtensorMap tmB;  // B (groups * N, K) int8
   const float* sA;
   const float* sB;
@@ -42,8 +41,11 @@ struct ProductArgs {
   int groups;              // 0: one product of M rows
   const int32_t* ends;     // groups: end row of each group
   const int32_t* c_rows;   // optional: row r of the product goes to row c_rows[r] of C
-  long long c_dst_rows;
-  int a_bytes, stages;     // A bytes of a stage; stages in the ring
+  int c_dst_rows;
+  int tile_rows;           // rows of C per tile
+  int box_rows, a_bytes;   // rows of an A load; A bytes of a stage
+  int stages;
+  int split;               // K ranges, one per CTA (pair) of the cluster
   int vec;                 // rows of C and residual can be moved 16 bytes at a time
   SignalSync* sync;
   long long wait_budget;
@@ -71,7 +73,7 @@ struct Tile {
 
 // Tile t: groups follow one another; inside one, `raster` row tiles walk all
 // column tiles before the next row tiles, so B tiles are read by neighbours.
-template <bool kGrouped, int kRows>
+template <bool kGrouped>
 __device__ __forceinline__ Tile tile_at(const ProductArgs& a, const ProductSmem& S, int t) {
   int g = 0, first = 0, rows = a.M, lt = t;
   if constexpr (kGrouped) {
@@ -85,14 +87,14 @@ __device__ __forceinline__ Tile tile_at(const ProductArgs& a, const ProductSmem&
     rows = S.row0[g + 1] - first;
     lt = t - S.tile0[g];
   }
-  const int tiles_m = (rows + kRows - 1) / kRows;
+  const int tiles_m = (rows + a.tile_rows - 1) / a.tile_rows;
   const int span = min(a.raster, tiles_m);
   const int block = lt / (span * a.tiles_n);
   const int m0 = block * span;
   const int mm = min(span, tiles_m - m0);
   const int in = lt - block * span * a.tiles_n;
   const int tm = m0 + in % mm;
-  return Tile{g, first + tm * kRows, rows - tm * kRows, in / mm};
+  return Tile{g, first + tm * a.tile_rows, rows - tm * a.tile_rows, in / mm};
 }
 
 // One stage of 1-SM int8 MMAs (128 bytes of K) and its commit, from one
@@ -114,6 +116,8 @@ __device__ __forceinline__ void umma_i8_stage_warp(uint32_t d, uint64_t ad, uint
       : "memory");
 }
 
+// act(sum * row scale * column scale + bias) of 32 columns, cols holding
+// {scale, bias} of each.
 template <int kAct>
 __device__ __forceinline__ void finish(uint32_t* v, float rs, const float2* cols) {
 #pragma unroll
@@ -124,34 +128,106 @@ __device__ __forceinline__ void finish(uint32_t* v, float rs, const float2* cols
   }
 }
 
+__device__ __forceinline__ void cp_async16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+template <int kAct>
+__device__ __forceinline__ void activate8(float* f) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = activate<kAct>(f[j]);
+}
+
+// Eight 16-bit elements from element `at` on, of which the row has `left`.
+__device__ __forceinline__ uint4 load8(const void* base, bool vec, int64_t at, int left) {
+  const uint16_t* src = static_cast<const uint16_t*>(base) + at;
+  if (vec) return *reinterpret_cast<const uint4*>(src);
+  uint32_t e[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < left) e[j / 2] |= uint32_t(src[j]) << (16 * (j & 1));
+  return make_uint4(e[0], e[1], e[2], e[3]);
+}
+__device__ __forceinline__ void store8(const ProductArgs& a, int64_t at, int left, uint4 val) {
+  uint16_t* out = static_cast<uint16_t*>(a.C) + at;
+  if (a.vec) {
+    *reinterpret_cast<uint4*>(out) = val;
+    return;
+  }
+  const uint32_t w[4] = {val.x, val.y, val.z, val.w};
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < left) out[j] = uint16_t(w[j / 2] >> (16 * (j & 1)));
+}
+
 // Group boundaries to shared memory: row0 and tile0 (exclusive prefix of the
-// groups' tiles).  Ends are clamped to [0, M] and made non-decreasing, so no
-// table of boundaries leads outside A.
-template <int kRows>
+// groups' tiles), by one warp, eight groups a lane.  Ends are clamped to
+// [0, M] and made non-decreasing, so no table of boundaries leads outside A.
 __device__ __forceinline__ void build_groups(const ProductArgs& a, ProductSmem& S) {
-  for (int g = threadIdx.x; g < a.groups; g += kThreads) S.row0[g + 1] = min(max(a.ends[g], 0), a.M);
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    int row = 0, tile = 0;
-    S.row0[0] = 0;
-    for (int g = 0; g < a.groups; ++g) {
-      const int end = max(S.row0[g + 1], row);
-      S.tile0[g] = tile;
-      tile += (end - row + kRows - 1) / kRows * a.tiles_n;
-      S.row0[g + 1] = row = end;
+  constexpr int kPer = kMaxGroups / 32;
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    int end[kPer], tiles[kPer];
+    int most = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int g = lane * kPer + i;
+      end[i] = g < a.groups ? min(max(a.ends[g], 0), a.M) : 0;
     }
-    S.tile0[a.groups] = tile;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) end[i] = most = max(most, end[i]);
+    int before = most;  // running maximum over the lanes
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before = max(before, v);
+    }
+    before = __shfl_up_sync(0xffffffffu, before, 1);
+    if (lane == 0) before = 0;
+    int sum = 0, begin = before;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      end[i] = max(end[i], before);
+      tiles[i] = sum;
+      sum += (end[i] - begin + a.tile_rows - 1) / a.tile_rows * a.tiles_n;
+      begin = end[i];
+    }
+    int total = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, total, o);
+      if (lane >= o) total += v;
+    }
+    const int base = total - sum;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int g = lane * kPer + i;
+      if (g < a.groups) {
+        S.tile0[g] = base + tiles[i];
+        S.row0[g + 1] = end[i];
+        if (g == a.groups - 1) S.tile0[a.groups] = i + 1 < kPer ? base + tiles[(i + 1) % kPer] : total;
+      }
+    }
+    if (lane == 0) S.row0[0] = 0;
   }
   __syncthreads();
 }
 
-template <bool kPair, int kTN, bool kGrouped>
+// kPair: a tile is worked on by two CTAs (2-SM MMAs, 128 rows of A and half
+// of the tile's rows of B each), else by one.
+//
+// kSplit: the cluster's CTAs (pairs) take a.split ranges of K of one tile and
+// add their int32 sums up through distributed shared memory, each finishing
+// its share of the columns: a product of few tiles then reads its weights
+// through all SMs.  int32 sums are exact, so C does not depend on the split.
+template <bool kPair, int kTN, bool kGrouped, bool kSplit>
 __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ ProductArgs a) {
-  constexpr int kRows = kPair ? 2 * kCtaRows : kCtaRows;  // rows of a tile
-  constexpr int kBRows = kPair ? kTN / 2 : kTN;           // rows of B this CTA loads
+  constexpr int kCtas = kPair ? 2 : 1;
+  constexpr int kBRows = kTN / kCtas;  // rows of B this CTA loads
   constexpr int kBBytes = kBRows * kTileK;
   constexpr int kHalf = kTN / 2;  // columns of an epilogue warp
-  constexpr uint32_t kIdesc = idesc_i8(kRows, kTN);
+  constexpr uint32_t kIdesc = idesc_i8(kCtas * kCtaRows, kTN);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int stage_bytes = a.a_bytes + kBBytes;
@@ -160,8 +236,12 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
   ProductSmem& S = *reinterpret_cast<ProductSmem*>(col_mem + kEpiWarps * kHalf);
   volatile int* abort_flag = &S.abort_flag;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const uint32_t rank = kPair ? cluster_ctarank() : 0;  // 0 issues the MMAs
-  const int first = kPair ? blockIdx.x >> 1 : blockIdx.x, stride = kPair ? gridDim.x >> 1 : gridDim.x;
+  const uint32_t crank = kPair || kSplit ? cluster_ctarank() : 0;
+  const uint32_t rank = kPair ? crank & 1 : 0;  // 0 issues the pair's MMAs
+  const uint32_t lead = crank - rank;           // its cluster rank
+  const uint16_t pair_mask = uint16_t(0x3u << lead);
+  const int split = kSplit ? a.split : 1;
+  const int first = blockIdx.x / (kCtas * split), stride = gridDim.x / (kCtas * split);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < a.stages; ++i) {
@@ -170,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&S.acc_full[i], 1);
-      mbar_init(&S.acc_empty[i], kPair ? 2 * kEpiWarps : kEpiWarps);
+      mbar_init(&S.acc_empty[i], kCtas * kEpiWarps);
     }
     mbar_init(&S.drain, 1);
     S.abort_flag = 0;
@@ -193,10 +273,12 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
   tc_fence_after();
   griddep_wait();
   griddep_launch_dependents();
-  if constexpr (kGrouped) build_groups<kRows>(a, S);
+  if constexpr (kGrouped) build_groups(a, S);
   const uint32_t tmem = S.tmem_base;
-  const int tiles = kGrouped ? S.tile0[a.groups] : (a.M + kRows - 1) / kRows * a.tiles_n;
+  const int tiles = kGrouped ? S.tile0[a.groups] : (a.M + a.tile_rows - 1) / a.tile_rows * a.tiles_n;
   const int kblocks = (a.K + kTileK - 1) / kTileK;
+  const int range = kSplit ? int(crank) / kCtas : 0;
+  const int kb0 = range * kblocks / split, kb1 = (range + 1) * kblocks / split;
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -204,22 +286,32 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
     bool ok = true;
     int st = 0, issued = 0;
     uint32_t phase = 1;
+    const int box_bytes = a.box_rows * kTileK;
     for (int t = first; t < tiles && ok; t += stride) {
-      const Tile w = tile_at<kGrouped, kRows>(a, S, t);
+      const Tile w = tile_at<kGrouped>(a, S, t);
       const int arow = w.row0 + int(rank) * kCtaRows;
       const int brow = w.group * a.N + w.tn * kTN + int(rank) * kBRows;
-      for (int kb = 0; kb < kblocks; ++kb) {
+      // Only loads of A with rows of this tile: the rest of the stage keeps
+      // what it held, and rows past the tile's are never stored.
+      auto boxes_of = [&](int r) {
+        return (min(max(w.rows - r * kCtaRows, 0), min(kCtaRows, a.tile_rows)) + a.box_rows - 1) / a.box_rows;
+      };
+      const int mine = boxes_of(rank);
+      const int bytes = kCtas * kBBytes + (boxes_of(0) + (kPair ? boxes_of(1) : 0)) * box_bytes;
+      for (int kb = kb0; kb < kb1; ++kb) {
         if (!(ok = mbar_wait_warp(&S.empty[st], phase, abort_flag, a.sync, a.wait_budget, a.wait_hint_ns))) break;
         if (leader) {
           uint8_t* sa = ring + st * stage_bytes;
-          if constexpr (kPair) {  // the leader's barrier counts both CTAs' bytes
-            if (rank == 0) mbar_arrive_expect_tx(&S.full[st], 2 * stage_bytes);
-            tma_load_2d_2sm(&a.tmA, &S.full[st], sa, kb * kTileK, arow);
+          // The pair leader's barrier counts both CTAs' bytes.
+          if (rank == 0) mbar_arrive_expect_tx(&S.full[st], bytes);
+          if constexpr (kPair) {
             tma_load_2d_2sm(&a.tmB, &S.full[st], sa + a.a_bytes, kb * kTileK, brow);
+            for (int i = 0; i < mine; ++i)
+              tma_load_2d_2sm(&a.tmA, &S.full[st], sa + i * box_bytes, kb * kTileK, arow + i * a.box_rows);
           } else {
-            mbar_arrive_expect_tx(&S.full[st], stage_bytes);
-            tma_load_2d(&a.tmA, &S.full[st], sa, kb * kTileK, arow);
             tma_load_2d(&a.tmB, &S.full[st], sa + a.a_bytes, kb * kTileK, brow);
+            for (int i = 0; i < mine; ++i)
+              tma_load_2d(&a.tmA, &S.full[st], sa + i * box_bytes, kb * kTileK, arow + i * a.box_rows);
           }
         }
         issued = min(issued + 1, a.stages);
@@ -247,39 +339,38 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         if (!(ok = mbar_wait_warp(&S.acc_empty[slot], ((n >> 1) & 1) ^ 1, abort_flag, a.sync, a.wait_budget, a.wait_hint_ns)))
           break;
         tc_fence_after();
-        for (int kb = 0; kb < kblocks; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!(ok = mbar_wait_warp(&S.full[st], phase, abort_flag, a.sync, a.wait_budget, a.wait_hint_ns))) break;
           tc_fence_after();
           const uint64_t ad = sdesc_sw128(sbase + st * stage_bytes);
           const uint64_t bd = sdesc_sw128(sbase + st * stage_bytes + a.a_bytes);
           if constexpr (kPair)
-            umma_8bit_2sm_stage_warp<4, false>(tmem + slot * kTN, ad, bd, kIdesc, kb != 0, &S.empty[st], kPairMask);
+            umma_8bit_2sm_stage_warp<4, false>(tmem + slot * kTN, ad, bd, kIdesc, kb != kb0, &S.empty[st], pair_mask);
           else
-            umma_i8_stage_warp(tmem + slot * kTN, ad, bd, kIdesc, kb != 0, &S.empty[st]);
+            umma_i8_stage_warp(tmem + slot * kTN, ad, bd, kIdesc, kb != kb0, &S.empty[st]);
           if (++st == a.stages) { st = 0; phase ^= 1; }
         }
         if (ok) {
-          if constexpr (kPair) umma_commit_2sm_warp(&S.acc_full[slot], kPairMask);
+          if constexpr (kPair) umma_commit_2sm_warp(&S.acc_full[slot], pair_mask);
           else umma_commit_warp(&S.acc_full[slot]);
         }
       }
       // Every MMA has retired before TMEM is released.
-      if constexpr (kPair) umma_commit_2sm_warp(&S.drain, 0x1);
+      if constexpr (kPair) umma_commit_2sm_warp(&S.drain, uint16_t(1u << lead));
       else umma_commit_warp(&S.drain);
       const long long t0 = clock64();
       while (!mbar_test(&S.drain, 0) && clock64() - t0 < 100000000LL) {
       }
     }
-  } else {
+  } else if constexpr (!kSplit) {
     // ------------------------------------------------------------ epilogue
     // Warp: TMEM lane quadrant q (32 rows), half h of the tile's columns.
     const int q = warp & 3, ew = warp - 2, h = ew >> 2;
     uint8_t* box = boxes + ew * kBoxBytes;
     float2* cols = col_mem + ew * kHalf;
     const bool f16 = a.c_f16;
-    bool ok = true;
-    int n = 0;
-    const uint32_t leader_empty = kPair ? mapa(&S.acc_empty[0], 0) : 0;
+    const int q0 = int(rank) * kCtaRows + 32 * q;  // the warp's first row in the tile
+    const uint32_t leader_empty = kPair ? mapa(&S.acc_empty[0], lead) : 0;
     auto release = [&](int slot) {  // the warp's loads of the accumulator have completed (wait::ld)
       tc_fence_before();
       __syncwarp();
@@ -288,43 +379,88 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         else mbar_arrive(&S.acc_empty[slot]);
       }
     };
-    for (int t = first; t < tiles && ok; t += stride, ++n) {
-      const Tile w = tile_at<kGrouped, kRows>(a, S, t);
-      const int slot = n & 1;
-      const int q0 = int(rank) * kCtaRows + 32 * q;  // the warp's first row in the tile
-      const int lrow = q0 + lane;
-      const int c0 = w.tn * kTN + h * kHalf;
-      const bool live = q0 < w.rows && c0 < a.N;  // this warp has something to store
-      float rs = 0.f;
-      long long dst = -1;
-      if (live) {
-        if (lrow < w.rows) {
-          const int r = w.row0 + lrow;
-          rs = a.sA[r];
-          dst = r;
-          if (kGrouped && a.c_rows) {
-            dst = a.c_rows[r];
-            if (dst >= a.c_dst_rows) dst = -1;
-          }
-        }
-        __syncwarp();
-        for (int j = lane; j < kHalf; j += 32) {
-          const int c = c0 + j;
-          float2 v = make_float2(0.f, 0.f);
-          if (c < a.N) {
-            v.x = a.sB[int64_t(w.group) * a.N + c];
-            if (!kGrouped && a.bias_kind)
-              v.y = a.bias_kind == kBiasF32 ? static_cast<const float*>(a.bias)[c] : half_at(a.bias, c, f16);
-          }
-          cols[j] = v;
-        }
-        __syncwarp();
+    // What a tile needs beside its accumulator: the row's scale and place in
+    // C (lane = row) and the columns' scales and biases.  Loaded a tile ahead:
+    // with short K the round trip to memory would otherwise be most of a
+    // tile's time.
+    struct Meta {
+      Tile w;
+      bool live;  // this warp has something to store
+      float rs;
+      int dst;
+      float2 col[kHalf / 32];
+    };
+    auto load_meta = [&](int t) {
+      Meta m;
+      m.live = false;
+      m.rs = 0.f;
+      m.dst = -1;
+#pragma unroll
+      for (int j = 0; j < kHalf / 32; ++j) m.col[j] = make_float2(0.f, 0.f);
+      if (t >= tiles) return m;
+      m.w = tile_at<kGrouped>(a, S, t);
+      const int c0 = m.w.tn * kTN + h * kHalf;
+      const int rows = min(m.w.rows, a.tile_rows);
+      m.live = q0 < rows && c0 < a.N;
+      if (!m.live) return m;
+      if (q0 + lane < rows) {
+        const int r = m.w.row0 + q0 + lane;
+        m.rs = a.sA[r];
+        m.dst = kGrouped && a.c_rows ? a.c_rows[r] : r;
       }
+#pragma unroll
+      for (int j = 0; j < kHalf / 32; ++j) {
+        const int c = c0 + 32 * j + lane;
+        if (c < a.N) {
+          m.col[j].x = a.sB[int64_t(m.w.group) * a.N + c];
+          if (!kGrouped && a.bias_kind)
+            m.col[j].y = a.bias_kind == kBiasF32 ? static_cast<const float*>(a.bias)[c] : half_at(a.bias, c, f16);
+        }
+      }
+      return m;
+    };
+    const int piece = lane & 7;
+    bool ok = true;
+    int n = 0;
+    Meta next = load_meta(first);
+    for (int t = first; t < tiles && ok; t += stride, ++n) {
+      const Meta m = next;
+      const int slot = n & 1;
+      const int c0 = m.w.tn * kTN + h * kHalf;
+      const int dst = !kGrouped || m.dst < a.c_dst_rows ? m.dst : -1;
+      // Eight lanes move one 128-byte row of a 64-column chunk, so loads of the
+      // residual and stores of C are whole lines.  Rows change hands through
+      // the warp's box (16-byte piece j of row r at j ^ (r & 7): no bank
+      // conflicts either way), into which the residual is copied
+      // asynchronously while the accumulator is still being computed.
+      auto fetch_residual = [&](int ch) {
+#pragma unroll
+        for (int it = 0; it < 8; ++it) {
+          const int br = 4 * it + (lane >> 3);
+          const int dr = __shfl_sync(0xffffffffu, dst, br);
+          const int col = c0 + 64 * ch + 8 * piece;
+          if (dr >= 0 && col < a.N) {
+            uint8_t* to = box + br * 128 + ((piece ^ (br & 7)) << 4);
+            const int64_t at = int64_t(dr) * a.N + col;
+            if (a.vec)
+              cp_async16(to, static_cast<const uint16_t*>(a.residual) + at);
+            else
+              *reinterpret_cast<uint4*>(to) = load8(a.residual, false, at, a.N - col);
+          }
+        }
+      };
+      if (m.live) {
+#pragma unroll
+        for (int j = 0; j < kHalf / 32; ++j) cols[32 * j + lane] = m.col[j];
+        __syncwarp();
+        if (!kGrouped && a.residual) fetch_residual(0);
+      }
+      next = load_meta(t + stride);
       if (!(ok = mbar_wait_warp(&S.acc_full[slot], (n >> 1) & 1, abort_flag, a.sync, a.wait_budget, a.wait_hint_ns)))
         break;
       tc_fence_after();
       const uint32_t taddr = tmem + slot * kTN + (uint32_t(32 * q) << 16) + h * kHalf;
-      if (!live) {
+      if (!m.live) {
         release(slot);
         continue;
       }
@@ -335,45 +471,18 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         tmem_ld32(taddr + 64 * ch, v);
         tmem_ld32(taddr + 64 * ch + 32, v + 32);
         tmem_wait_ld_into2(v, v + 32);
-        if (ch == kHalf / 64 - 1) {  // the accumulator is free for the tile after next
-          release(slot);
-        }
+        if (ch == kHalf / 64 - 1) release(slot);  // the accumulator is free for the tile after next
         const float2* cc = cols + 64 * ch;
-        const int col0 = c0 + 64 * ch;
         switch (kGrouped ? PB2_ACT_NONE : a.act) {
-          case PB2_ACT_RELU: finish<PB2_ACT_RELU>(v, rs, cc); finish<PB2_ACT_RELU>(v + 32, rs, cc + 32); break;
-          case PB2_ACT_SILU: finish<PB2_ACT_SILU>(v, rs, cc); finish<PB2_ACT_SILU>(v + 32, rs, cc + 32); break;
-          case PB2_ACT_GELU: finish<PB2_ACT_GELU>(v, rs, cc); finish<PB2_ACT_GELU>(v + 32, rs, cc + 32); break;
+          case PB2_ACT_RELU: finish<PB2_ACT_RELU>(v, m.rs, cc); finish<PB2_ACT_RELU>(v + 32, m.rs, cc + 32); break;
+          case PB2_ACT_SILU: finish<PB2_ACT_SILU>(v, m.rs, cc); finish<PB2_ACT_SILU>(v + 32, m.rs, cc + 32); break;
+          case PB2_ACT_GELU: finish<PB2_ACT_GELU>(v, m.rs, cc); finish<PB2_ACT_GELU>(v + 32, m.rs, cc + 32); break;
           case PB2_ACT_GELU_TANH:
-            finish<PB2_ACT_GELU_TANH>(v, rs, cc); finish<PB2_ACT_GELU_TANH>(v + 32, rs, cc + 32); break;
-          default: finish<PB2_ACT_NONE>(v, rs, cc); finish<PB2_ACT_NONE>(v + 32, rs, cc + 32);
+            finish<PB2_ACT_GELU_TANH>(v, m.rs, cc); finish<PB2_ACT_GELU_TANH>(v + 32, m.rs, cc + 32); break;
+          default: finish<PB2_ACT_NONE>(v, m.rs, cc); finish<PB2_ACT_NONE>(v + 32, m.rs, cc + 32);
         }
-        // Rows leave through the warp's box (16-byte chunks, chunk j of row r
-        // at j ^ (r & 7)): eight lanes move one 128-byte row, so stores (and
-        // the residual's loads) are whole lines.
-        const int piece = lane & 7;
         if (!kGrouped && a.residual) {
-#pragma unroll
-          for (int it = 0; it < 8; ++it) {
-            const int br = 4 * it + (lane >> 3);
-            const long long dr = __shfl_sync(0xffffffffu, dst, br);
-            const int col = col0 + 8 * piece;
-            uint4 r = make_uint4(0u, 0u, 0u, 0u);
-            if (dr >= 0 && col < a.N) {
-              const uint16_t* src = static_cast<const uint16_t*>(a.residual) + dr * a.N + col;
-              if (a.vec) {
-                r = *reinterpret_cast<const uint4*>(src);
-              } else {
-                uint16_t e[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                  if (col + j < a.N) e[j] = src[j];
-                r = make_uint4(e[0] | uint32_t(e[1]) << 16, e[2] | uint32_t(e[3]) << 16, e[4] | uint32_t(e[5]) << 16,
-                               e[6] | uint32_t(e[7]) << 16);
-              }
-            }
-            *reinterpret_cast<uint4*>(box + br * 128 + ((piece ^ (br & 7)) << 4)) = r;
-          }
+          cp_async_wait();
           __syncwarp();
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
@@ -400,30 +509,108 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
 #pragma unroll
         for (int it = 0; it < 8; ++it) {
           const int br = 4 * it + (lane >> 3);
-          const long long dr = __shfl_sync(0xffffffffu, dst, br);
-          const int col = col0 + 8 * piece;
+          const int dr = __shfl_sync(0xffffffffu, dst, br);
+          const int col = c0 + 64 * ch + 8 * piece;
           const uint4 val = *reinterpret_cast<const uint4*>(box + br * 128 + ((piece ^ (br & 7)) << 4));
-          if (dr >= 0 && col < a.N) {
-            uint16_t* out = static_cast<uint16_t*>(a.C) + dr * a.N + col;
-            if (a.vec) {
-              *reinterpret_cast<uint4*>(out) = val;
-            } else {
-              const uint32_t w4[4] = {val.x, val.y, val.z, val.w};
-#pragma unroll
-              for (int j = 0; j < 8; ++j)
-                if (col + j < a.N) out[j] = uint16_t(w4[j / 2] >> (16 * (j & 1)));
-            }
-          }
+          if (dr >= 0 && col < a.N) store8(a, int64_t(dr) * a.N + col, a.N - col, val);
         }
         __syncwarp();
+        if (!kGrouped && a.residual && ch + 1 < kHalf / 64) fetch_residual(ch + 1);
       }
     }
   }
-  // Neither CTA of a pair leaves while its peer can still address its
-  // barriers or tensor memory.
+  if constexpr (kSplit) {
+    // ------------------------------------------------------------ join of the K ranges
+    // Each CTA's accumulator goes to its own ring (idle by now) as rows of
+    // kTN int32, 16-byte piece j of row r at j ^ (r & 7); then every CTA
+    // adds up its columns over the ranges.
+    const bool has = first < tiles;
+    const Tile w = has ? tile_at<kGrouped>(a, S, first) : Tile{0, 0, 0, 0};
+    const int live = min(min(max(min(w.rows, a.tile_rows) - int(rank) * kCtaRows, 0), kCtaRows), has ? kCtaRows : 0);
+    if (warp >= 2 && has) {
+      const int q = warp & 3, h = (warp - 2) >> 2;
+      const bool ok = mbar_wait_warp(&S.acc_full[0], 0, abort_flag, a.sync, a.wait_budget, a.wait_hint_ns);
+      tc_fence_after();
+      if (ok && 32 * q < live) {
+#pragma unroll 1
+        for (int ch = 0; ch < kHalf / 32; ++ch) {
+          uint32_t v[32];
+          __syncwarp();
+          tmem_ld32(tmem + (uint32_t(32 * q) << 16) + h * kHalf + 32 * ch, v);
+          tmem_wait_ld_into(v);
+          const int r = 32 * q + lane;
+          if (r < live) {
+            uint4* row = reinterpret_cast<uint4*>(ring + r * kTN * 4);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              row[(h * (kHalf / 4) + 8 * ch + j) ^ (r & 7)] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          }
+        }
+      }
+    }
+    cluster_sync_all();
+    if (warp >= 2 && !*abort_flag) {
+      const bool f16 = a.c_f16;
+      const int width = kTN / split, pieces = width / 8;
+      for (int i = threadIdx.x - 64; i < live * pieces; i += 32 * kEpiWarps) {
+        const int r = i / pieces, lc = range * width + (i - r * pieces) * 8;
+        const int col = w.tn * kTN + lc;
+        if (col >= a.N) continue;
+        const int row = w.row0 + int(rank) * kCtaRows + r;
+        int dst = row;
+        if (kGrouped && a.c_rows) dst = a.c_rows[row];
+        if (dst < 0 || (kGrouped && dst >= a.c_dst_rows)) continue;
+        uint4 res = make_uint4(0u, 0u, 0u, 0u);
+        if (!kGrouped && a.residual) res = load8(a.residual, a.vec, int64_t(dst) * a.N + col, a.N - col);
+        int acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        const uint8_t* p0 = ring + r * kTN * 4 + (((lc / 4) ^ (r & 7)) << 4);
+        const uint8_t* p1 = ring + r * kTN * 4 + (((lc / 4 + 1) ^ (r & 7)) << 4);
+        for (int s = 0; s < split; ++s) {
+          const int4 x = ld_cluster_v4(mapa(p0, s * kCtas + rank)), y = ld_cluster_v4(mapa(p1, s * kCtas + rank));
+          acc[0] += x.x; acc[1] += x.y; acc[2] += x.z; acc[3] += x.w;
+          acc[4] += y.x; acc[5] += y.y; acc[6] += y.z; acc[7] += y.w;
+        }
+        const float rs = a.sA[row];
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float bias = 0.f, sb = 0.f;
+          if (col + j < a.N) {
+            sb = a.sB[int64_t(w.group) * a.N + col + j];
+            if (!kGrouped && a.bias_kind)
+              bias = a.bias_kind == kBiasF32 ? static_cast<const float*>(a.bias)[col + j] : half_at(a.bias, col + j, f16);
+          }
+          f[j] = fmaf(float(acc[j]) * rs, sb, bias);
+        }
+        if constexpr (!kGrouped) {
+          switch (a.act) {
+            case PB2_ACT_RELU: activate8<PB2_ACT_RELU>(f); break;
+            case PB2_ACT_SILU: activate8<PB2_ACT_SILU>(f); break;
+            case PB2_ACT_GELU: activate8<PB2_ACT_GELU>(f); break;
+            case PB2_ACT_GELU_TANH: activate8<PB2_ACT_GELU_TANH>(f); break;
+            default: break;
+          }
+          if (a.residual) {
+            const uint32_t rw[4] = {res.x, res.y, res.z, res.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 g = unpack_half2(rw[j], f16);
+              f[2 * j] += g.x;
+              f[2 * j + 1] += g.y;
+            }
+          }
+        }
+        store8(a, int64_t(dst) * a.N + col, a.N - col,
+               make_uint4(pack_half2(f[0], f[1], f16), pack_half2(f[2], f[3], f16), pack_half2(f[4], f[5], f16),
+                          pack_half2(f[6], f[7], f16)));
+      }
+    }
+  }
+  // No CTA leaves while another of its cluster can still address its
+  // barriers, tensor memory or sums.
   tc_fence_before();
   __syncthreads();
-  if constexpr (kPair) cluster_sync_all();
+  if constexpr (kPair || kSplit) cluster_sync_all();
   tc_fence_after();
   if (warp == 1) {
     __syncwarp();
@@ -461,42 +648,72 @@ int resident_pairs(int device, const void* kern, int smem) {
   return n;
 }
 
-template <bool kPair, int kTN, bool kGrouped>
-int launch_product(ProductArgs& a, const int8_t* A, const int8_t* B, int device, cudaStream_t s) {
-  constexpr int kRows = kPair ? 2 * kCtaRows : kCtaRows;
-  constexpr int kBRows = kPair ? kTN / 2 : kTN;
-  const int box_rows = std::min(kCtaRows, (a.M + 7) / 8 * 8);
+template <bool kPair, int kTN, bool kGrouped, bool kSplit>
+int launch_product(ProductArgs& a, const int8_t* A, const int8_t* B, int cta_rows, int device, cudaStream_t s) {
+  constexpr int kCtas = kPair ? 2 : 1;
+  constexpr int kBRows = kTN / kCtas;
+  a.a_bytes = cta_rows * kTileK;
+  a.tile_rows = kCtas * cta_rows;
+  a.tiles_n = (a.N + kTN - 1) / kTN;
+  a.raster = 8;
   int st;
-  if ((st = make_tmap_2d(&a.tmA, A, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, a.M, kTileK, box_rows,
+  if ((st = make_tmap_2d(&a.tmA, A, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, a.M, kTileK, a.box_rows,
                          CU_TENSOR_MAP_SWIZZLE_128B)) ||
       (st = make_tmap_2d(&a.tmB, B, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, uint64_t(std::max(a.groups, 1)) * a.N, kTileK,
                          kBRows, CU_TENSOR_MAP_SWIZZLE_128B)))
     return st;
-  a.a_bytes = box_rows * kTileK;
-  a.tiles_n = (a.N + kTN - 1) / kTN;
-  a.raster = 8;
   const int fixed = 1024 + kEpiWarps * (kBoxBytes + kTN / 2 * 8) + int(sizeof(ProductSmem));
   a.stages = std::min(kMaxStages, (232448 - fixed) / (a.a_bytes + kBRows * kTileK));
   a.wait_budget = wait_budget_cycles();
   a.wait_hint_ns = suspend_hint_ns(a.wait_budget);
   const int smem = fixed + a.stages * (a.a_bytes + kBRows * kTileK);
-  auto kern = product_kernel<kPair, kTN, kGrouped>;
+  auto kern = product_kernel<kPair, kTN, kGrouped, kSplit>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return launch_status();
   // Row tiles: exact without groups; with them, whose sizes only the device
   // knows, at most one ragged tile a group beyond the whole ones.
-  const int64_t tiles_m = kGrouped ? int64_t(a.M) / kRows + std::min(a.groups, a.M) : (int64_t(a.M) + kRows - 1) / kRows;
-  const int most = kPair ? resident_pairs(device, reinterpret_cast<const void*>(kern), smem)
-                         : std::max(1, sm_count(device));
-  const int64_t ctas = std::min<int64_t>(tiles_m * a.tiles_n, most) * (kPair ? 2 : 1);
-  return launch_programmatic(kern, dim3(unsigned(ctas)), kThreads, smem, s, kPair ? 2 : 1, a);
+  const int64_t tiles_m = kGrouped ? int64_t(a.M) / a.tile_rows + std::min(a.groups, a.M)
+                                   : (int64_t(a.M) + a.tile_rows - 1) / a.tile_rows;
+  int64_t clusters = tiles_m * a.tiles_n;
+  if (!kSplit) {
+    const int most = kPair ? resident_pairs(device, reinterpret_cast<const void*>(kern), smem)
+                           : std::max(1, sm_count(device));
+    clusters = std::min<int64_t>(clusters, most);
+  }
+  const int cluster = kCtas * (kSplit ? a.split : 1);
+  return launch_programmatic(kern, dim3(unsigned(clusters * cluster)), kThreads, smem, s, cluster, a);
+}
+
+// K ranges for a product of `tiles` tiles of `ctas` CTAs: a power of two, at
+// most 8 CTAs to a cluster, as long as the ranges keep all clusters resident
+// and kMinRange K blocks each (a join costs about as much as that many).
+constexpr int kMinRange = 4;
+int split_of(int64_t tiles, int ctas, int kblocks, int sms) {
+  int split = 1;
+  while (2 * split * ctas <= 8 && tiles * ctas * 2 * split <= sms && kblocks / (2 * split) >= kMinRange) split *= 2;
+  return split;
 }
 
 template <bool kGrouped>
 int run_product(ProductArgs& a, const int8_t* A, const int8_t* B, int device, cudaStream_t s) {
-  const int64_t rows = kGrouped ? a.M / a.groups : a.M;
-  if (rows > kCtaRows) return launch_product<true, 256, kGrouped>(a, A, B, device, s);
-  return launch_product<false, 128, kGrouped>(a, A, B, device, s);
+  const int sms = std::max(1, sm_count(device));
+  const int kblocks = (a.K + kTileK - 1) / kTileK;
+  const int64_t rows = kGrouped ? a.M / a.groups : a.M;  // of a group, on average
+  if (rows > kCtaRows) {
+    a.box_rows = kCtaRows;
+    const int64_t tiles = (int64_t(a.M) + 255) / 256 * ((a.N + 255) / 256);
+    a.split = kGrouped ? 1 : split_of(tiles, 2, kblocks, sms);
+    if (a.split > 1) return launch_product<true, 256, kGrouped, true>(a, A, B, kCtaRows, device, s);
+    return launch_product<true, 256, kGrouped, false>(a, A, B, kCtaRows, device, s);
+  }
+  const int cta_rows = std::min(kCtaRows, (a.M + 7) / 8 * 8);
+  a.box_rows = cta_rows;
+  const int64_t tiles_n = (a.N + 127) / 128;
+  const int64_t tiles = (kGrouped ? std::min(a.groups, a.M) : 1) * tiles_n;
+  a.split = split_of(tiles, 1, kblocks, sms);
+  // A K range's sums fit the ring of a CTA whatever its stages (64 KB).
+  if (a.split > 1) return launch_product<false, 128, kGrouped, true>(a, A, B, cta_rows, device, s);
+  return launch_product<false, 128, kGrouped, false>(a, A, B, cta_rows, device, s);
 }
 
 // out[t] = residual[t] + sum_j w[t, j] * slots[t * top_k + j], f32 sums in
@@ -631,7 +848,7 @@ extern "C" int pb2_gemm_grouped(const pb2_gemm_grouped_params* pp, void* stream)
   a.groups = int(p.num_experts);
   a.ends = p.routing_offsets;
   a.c_rows = p.c_row_index;
-  a.c_dst_rows = p.c_row_index ? p.c_rows : p.m;
+  a.c_dst_rows = int(std::min<int64_t>(p.c_row_index ? p.c_rows : p.m, INT32_MAX));
   a.vec = p.n % 8 == 0 && al16(p.C);
   a.sync = static_cast<SignalSync*>(p.host_signal_sync);
   return run_product<true>(a, p.A, p.B, p.device, static_cast<cudaStream_t>(stream));

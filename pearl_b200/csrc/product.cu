@@ -62,6 +62,8 @@ struct ProductSmem {
   int abort_flag;
   int tile0[kMaxGroups + 1];  // first tile of each group
   int row0[kMaxGroups + 1];   // first row of each group
+  float scale[kCtaRows];      // kOnce: the rows' scales and places in C
+  int dst[kCtaRows];
 };
 
 struct Tile {
@@ -97,23 +99,60 @@ __device__ __forceinline__ Tile tile_at(const ProductArgs& a, const ProductSmem&
   return Tile{g, first + tm * a.tile_rows, rows - tm * a.tile_rows, in / mm};
 }
 
-// One stage of 1-SM int8 MMAs (128 bytes of K) and its commit, from one
-// elected lane.
-__device__ __forceinline__ void umma_i8_stage_warp(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc,
-                                                   uint32_t accumulate, uint64_t* bar) {
+// The producer and the issuer are single threads whose loops bound short-tile
+// products (a K stage of a 128-column tile is 256 clocks of MMA), so they keep
+// to 32-bit shared addresses that only step: these are the barrier, TMA and
+// MMA instructions on such addresses.
+__device__ __forceinline__ bool bar_ready(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
   asm volatile(
-      "{\n\t.reg .pred e, p;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t"
-      "setp.eq.u32 p, %4, %4;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::i8 [%0], %5, %6, %3, p;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::i8 [%0], %7, %8, %3, p;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::i8 [%0], %9, %10, %3, p;\n\t"
-      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%11];\n\t}" ::"r"(d),
-      "l"(ad), "l"(bd), "r"(idesc), "r"(accumulate), "l"(ad + 2), "l"(bd + 2), "l"(ad + 4), "l"(bd + 4), "l"(ad + 6),
-      "l"(bd + 6), "r"(smem_u32(bar))
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
       : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// A box to `dst`, counted on `bar`; with kPair on the barrier at this offset
+// in the pair's leader.
+template <bool kPair>
+__device__ __forceinline__ void load_box(const CUtensorMap* map, uint32_t bar, uint32_t dst, int x, int y) {
+  if constexpr (kPair)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar & 0xFEFFFFFFu), "r"(x), "r"(y)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+        : "memory");
+}
+// One stage of int8 MMAs (128 bytes of K) and its commit; the 2-SM commit
+// reaches the barrier in both CTAs of the pair.
+template <bool kPair>
+__device__ __forceinline__ void umma_i8_stage(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t accumulate,
+                                              uint32_t bar, uint16_t pair_mask) {
+  if constexpr (kPair) {
+    umma_i8_2sm(d, ad, bd, idesc, accumulate);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) umma_i8_2sm(d, ad + 2 * i, bd + 2 * i, idesc, 1);
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"(pair_mask)
+        : "memory");
+  } else {
+    umma_i8(d, ad, bd, idesc, accumulate);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) umma_i8(d, ad + 2 * i, bd + 2 * i, idesc, 1);
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  }
 }
 
 // act(sum * row scale * column scale + bias) of 32 columns, cols holding
@@ -217,30 +256,38 @@ __device__ __forceinline__ void build_groups(const ProductArgs& a, ProductSmem& 
 // kPair: a tile is worked on by two CTAs (2-SM MMAs, 128 rows of A and half
 // of the tile's rows of B each), else by one.
 //
-// kSplit: the cluster's CTAs (pairs) take a.split ranges of K of one tile and
-// add their int32 sums up through distributed shared memory, each finishing
-// its share of the columns: a product of few tiles then reads its weights
-// through all SMs.  int32 sums are exact, so C does not depend on the split.
-template <bool kPair, int kTN, bool kGrouped, bool kSplit>
-__global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ ProductArgs a) {
+// kOnce: for products of few tiles, one tile for each CTA (pair), or for a
+// cluster whose CTAs (pairs) take a.split ranges of its K and add their int32
+// sums up through distributed shared memory, each finishing its share of the
+// columns: the weights are then read through all SMs.  int32 sums are exact,
+// so C does not depend on the split.  Half an SM's shared memory, so that the
+// set-up of one product overlaps the end of the one before it.
+// Otherwise the grid is persistent and the accumulator double-buffered.
+template <bool kPair, int kTN, bool kGrouped, bool kOnce>
+__global__ void __launch_bounds__(kThreads, kOnce ? 2 : 1) product_kernel(const __grid_constant__ ProductArgs a) {
   constexpr int kCtas = kPair ? 2 : 1;
   constexpr int kBRows = kTN / kCtas;  // rows of B this CTA loads
   constexpr int kBBytes = kBRows * kTileK;
   constexpr int kHalf = kTN / 2;  // columns of an epilogue warp
   constexpr uint32_t kIdesc = idesc_i8(kCtas * kCtaRows, kTN);
+  // An MMA reads kCtaRows rows of A, however few the stage holds (at least
+  // eight): the read must end inside the stage.  Pairs always hold them all.
+  static_assert(kPair || 8 * kTileK + kBBytes >= kCtaRows * kTileK, "A operand would be read past the stage");
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int stage_bytes = a.a_bytes + kBBytes;
   uint8_t* boxes = ring + a.stages * stage_bytes;
   float2* col_mem = reinterpret_cast<float2*>(boxes + kEpiWarps * kBoxBytes);
-  ProductSmem& S = *reinterpret_cast<ProductSmem*>(col_mem + kEpiWarps * kHalf);
+  // kOnce needs neither boxes nor column scales in shared memory.
+  ProductSmem& S = *reinterpret_cast<ProductSmem*>(kOnce ? boxes : reinterpret_cast<uint8_t*>(col_mem + kEpiWarps * kHalf));
+  constexpr int kTmemCols = kOnce ? kTN : 2 * kTN;
   volatile int* abort_flag = &S.abort_flag;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const uint32_t crank = kPair || kSplit ? cluster_ctarank() : 0;
+  const uint32_t crank = kPair || kOnce ? cluster_ctarank() : 0;
   const uint32_t rank = kPair ? crank & 1 : 0;  // 0 issues the pair's MMAs
   const uint32_t lead = crank - rank;           // its cluster rank
   const uint16_t pair_mask = uint16_t(0x3u << lead);
-  const int split = kSplit ? a.split : 1;
+  const int split = kOnce ? a.split : 1;
   const int first = blockIdx.x / (kCtas * split), stride = gridDim.x / (kCtas * split);
 
   if (threadIdx.x == 0) {
@@ -260,10 +307,10 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
   }
   if (warp == 1) {
     if constexpr (kPair) {
-      tmem_alloc_2sm(&S.tmem_base, 2 * kTN);
+      tmem_alloc_2sm(&S.tmem_base, kTmemCols);
       tmem_relinquish_2sm();
     } else {
-      tmem_alloc(&S.tmem_base, 2 * kTN);
+      tmem_alloc(&S.tmem_base, kTmemCols);
       tmem_relinquish();
     }
   }
@@ -271,98 +318,116 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
   __syncthreads();
   if constexpr (kPair) cluster_sync_all();  // both CTAs' barriers exist before a remote arrive or 2-SM load
   tc_fence_after();
+  const int kblocks = (a.K + kTileK - 1) / kTileK;
+  const int range = kOnce ? int(crank) / kCtas : 0;
+  const int kb0 = range * kblocks / split, kb1 = (range + 1) * kblocks / split;
+  if constexpr (kOnce && !kGrouped) {
+    // The previous kernel is still running: ask L2 for the first stages of B
+    // (a prefetch is coherent with whatever that kernel writes).
+    if (warp == 0 && elect_one()) {
+      const Tile w = tile_at<false>(a, S, first);
+      for (int kb = kb0; kb < min(kb1, kb0 + a.stages); ++kb)
+        tma_prefetch_l2_2d(&a.tmB, kb * kTileK, w.tn * kTN + int(rank) * kBRows);
+    }
+  }
   griddep_wait();
   griddep_launch_dependents();
   if constexpr (kGrouped) build_groups(a, S);
   const uint32_t tmem = S.tmem_base;
   const int tiles = kGrouped ? S.tile0[a.groups] : (a.M + a.tile_rows - 1) / a.tile_rows * a.tiles_n;
-  const int kblocks = (a.K + kTileK - 1) / kTileK;
-  const int range = kSplit ? int(crank) / kCtas : 0;
-  const int kb0 = range * kblocks / split, kb1 = (range + 1) * kblocks / split;
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
-    const bool leader = elect_one();
-    bool ok = true;
-    int st = 0, issued = 0;
-    uint32_t phase = 1;
-    const int box_bytes = a.box_rows * kTileK;
-    for (int t = first; t < tiles && ok; t += stride) {
-      const Tile w = tile_at<kGrouped>(a, S, t);
-      const int arow = w.row0 + int(rank) * kCtaRows;
-      const int brow = w.group * a.N + w.tn * kTN + int(rank) * kBRows;
-      // Only loads of A with rows of this tile: the rest of the stage keeps
-      // what it held, and rows past the tile's are never stored.
-      auto boxes_of = [&](int r) {
-        return (min(max(w.rows - r * kCtaRows, 0), min(kCtaRows, a.tile_rows)) + a.box_rows - 1) / a.box_rows;
-      };
-      const int mine = boxes_of(rank);
-      const int bytes = kCtas * kBBytes + (boxes_of(0) + (kPair ? boxes_of(1) : 0)) * box_bytes;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!(ok = mbar_wait_warp(&S.empty[st], phase, abort_flag, a.sync, a.wait_budget, a.wait_hint_ns))) break;
-        if (leader) {
-          uint8_t* sa = ring + st * stage_bytes;
+    if (elect_one()) {
+      bool ok = true;
+      const uint32_t full0 = smem_u32(S.full), empty0 = smem_u32(S.empty), ring0 = smem_u32(ring);
+      const uint32_t past = 8 * a.stages;
+      uint32_t at = 0, dst = ring0, phase = 1;  // of the stage: barrier offset, address, wait parity
+      const int box_bytes = a.box_rows * kTileK;
+      for (int t = first; t < tiles && ok; t += stride) {
+        const Tile w = tile_at<kGrouped>(a, S, t);
+        const int arow = w.row0 + int(rank) * kCtaRows;
+        const int brow = w.group * a.N + w.tn * kTN + int(rank) * kBRows;
+        // Only loads of A with rows of this tile: the rest of the stage keeps
+        // what it held, and rows past the tile's are never stored.
+        auto boxes_of = [&](int r) {
+          return (min(max(w.rows - r * kCtaRows, 0), min(kCtaRows, a.tile_rows)) + a.box_rows - 1) / a.box_rows;
+        };
+        const int mine = boxes_of(rank);
+        const int bytes = kCtas * kBBytes + (boxes_of(0) + (kPair ? boxes_of(1) : 0)) * box_bytes;
+        const int x1 = kb1 * kTileK;
+        for (int x = kb0 * kTileK; x < x1; x += kTileK) {
+          if (!bar_ready(empty0 + at, phase) &&
+              !(ok = mbar_wait(&S.empty[at / 8], phase, abort_flag, a.sync, a.wait_budget, a.wait_hint_ns)))
+            break;
           // The pair leader's barrier counts both CTAs' bytes.
-          if (rank == 0) mbar_arrive_expect_tx(&S.full[st], bytes);
-          if constexpr (kPair) {
-            tma_load_2d_2sm(&a.tmB, &S.full[st], sa + a.a_bytes, kb * kTileK, brow);
-            for (int i = 0; i < mine; ++i)
-              tma_load_2d_2sm(&a.tmA, &S.full[st], sa + i * box_bytes, kb * kTileK, arow + i * a.box_rows);
+          if (rank == 0) bar_expect(full0 + at, bytes);
+          load_box<kPair>(&a.tmB, full0 + at, dst + a.a_bytes, x, brow);
+          if (mine == 1) {
+            load_box<kPair>(&a.tmA, full0 + at, dst, x, arow);
           } else {
-            tma_load_2d(&a.tmB, &S.full[st], sa + a.a_bytes, kb * kTileK, brow);
-            for (int i = 0; i < mine; ++i)
-              tma_load_2d(&a.tmA, &S.full[st], sa + i * box_bytes, kb * kTileK, arow + i * a.box_rows);
+            for (int i = 0; i < mine; ++i) load_box<kPair>(&a.tmA, full0 + at, dst + i * box_bytes, x, arow + i * a.box_rows);
           }
+          at += 8;
+          dst += stage_bytes;
+          if (at == past) { at = 0; dst = ring0; phase ^= 1; }
         }
-        issued = min(issued + 1, a.stages);
-        if (++st == a.stages) { st = 0; phase ^= 1; }
+      }
+      // Every load in flight has landed and been consumed before the CTA ends
+      // (bounded).  The next wait of each stage in turn is for just that; on a
+      // stage that was never filled it returns at once.
+      for (int i = 0; i < a.stages; ++i) {
+        const long long t0 = clock64();
+        while (!bar_ready(empty0 + at, phase) && clock64() - t0 < 100000000LL) {
+        }
+        at += 8;
+        if (at == past) { at = 0; phase ^= 1; }
       }
     }
-    // Every load in flight has landed and been consumed before the CTA ends
-    // (bounded).
-    for (int i = 0; i < issued; ++i) {
-      st = st == 0 ? a.stages - 1 : st - 1;
-      if (st == a.stages - 1) phase ^= 1;
-      const long long t0 = clock64();
-      while (!mbar_test(&S.empty[st], phase ^ 1) && clock64() - t0 < 100000000LL) {
-      }
-    }
+    __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (the pair's leader)
-    if (rank == 0) {
+    if (rank == 0 && elect_one()) {
       bool ok = true;
-      int st = 0, n = 0;
-      uint32_t phase = 0;
-      const uint32_t sbase = smem_u32(ring);
+      int n = 0;
+      const uint32_t full0 = smem_u32(S.full), empty0 = smem_u32(S.empty);
+      const uint32_t past = 8 * a.stages;
+      const uint64_t desc0 = sdesc_sw128(smem_u32(ring));  // address field: the low 14 bits, in 16 bytes
+      const uint32_t step = stage_bytes >> 4, b_off = a.a_bytes >> 4;
+      uint32_t at = 0, phase = 0;
+      uint64_t ad = desc0;
       for (int t = first; t < tiles && ok; t += stride, ++n) {
         const int slot = n & 1;
-        if (!(ok = mbar_wait_warp(&S.acc_empty[slot], ((n >> 1) & 1) ^ 1, abort_flag, a.sync, a.wait_budget, a.wait_hint_ns)))
+        if (!(ok = mbar_wait(&S.acc_empty[slot], ((n >> 1) & 1) ^ 1, abort_flag, a.sync, a.wait_budget, a.wait_hint_ns)))
           break;
         tc_fence_after();
+        const uint32_t d = tmem + slot * kTN;
+        uint32_t accumulate = 0;
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (!(ok = mbar_wait_warp(&S.full[st], phase, abort_flag, a.sync, a.wait_budget, a.wait_hint_ns))) break;
+          if (!bar_ready(full0 + at, phase) &&
+              !(ok = mbar_wait(&S.full[at / 8], phase, abort_flag, a.sync, a.wait_budget, a.wait_hint_ns)))
+            break;
           tc_fence_after();
-          const uint64_t ad = sdesc_sw128(sbase + st * stage_bytes);
-          const uint64_t bd = sdesc_sw128(sbase + st * stage_bytes + a.a_bytes);
-          if constexpr (kPair)
-            umma_8bit_2sm_stage_warp<4, false>(tmem + slot * kTN, ad, bd, kIdesc, kb != kb0, &S.empty[st], pair_mask);
-          else
-            umma_i8_stage_warp(tmem + slot * kTN, ad, bd, kIdesc, kb != kb0, &S.empty[st]);
-          if (++st == a.stages) { st = 0; phase ^= 1; }
+          umma_i8_stage<kPair>(d, ad, ad + b_off, kIdesc, accumulate, empty0 + at, pair_mask);
+          accumulate = 1;
+          at += 8;
+          ad += step;
+          if (at == past) { at = 0; ad = desc0; phase ^= 1; }
         }
         if (ok) {
-          if constexpr (kPair) umma_commit_2sm_warp(&S.acc_full[slot], pair_mask);
-          else umma_commit_warp(&S.acc_full[slot]);
+          if constexpr (kPair) umma_commit_2sm(&S.acc_full[slot], pair_mask);
+          else umma_commit(&S.acc_full[slot]);
         }
       }
       // Every MMA has retired before TMEM is released.
-      if constexpr (kPair) umma_commit_2sm_warp(&S.drain, uint16_t(1u << lead));
-      else umma_commit_warp(&S.drain);
+      if constexpr (kPair) umma_commit_2sm(&S.drain, uint16_t(1u << lead));
+      else umma_commit(&S.drain);
       const long long t0 = clock64();
       while (!mbar_test(&S.drain, 0) && clock64() - t0 < 100000000LL) {
       }
     }
-  } else if constexpr (!kSplit) {
+    __syncwarp();
+  } else if constexpr (!kOnce) {
     // ------------------------------------------------------------ epilogue
     // Warp: TMEM lane quadrant q (32 rows), half h of the tile's columns.
     const int q = warp & 3, ew = warp - 2, h = ew >> 2;
@@ -519,17 +584,67 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       }
     }
   }
-  if constexpr (kSplit) {
+  if constexpr (kOnce) {
     // ------------------------------------------------------------ join of the K ranges
     // Each CTA's accumulator goes to its own ring (idle by now) as rows of
     // kTN int32, 16-byte piece j of row r at j ^ (r & 7); then every CTA
-    // adds up its columns over the ranges.
+    // adds up its columns over the ranges, a thread eight of them.
     const bool has = first < tiles;
     const Tile w = has ? tile_at<kGrouped>(a, S, first) : Tile{0, 0, 0, 0};
-    const int live = min(min(max(min(w.rows, a.tile_rows) - int(rank) * kCtaRows, 0), kCtaRows), has ? kCtaRows : 0);
-    if (warp >= 2 && has) {
+    const int live = has ? min(max(min(w.rows, a.tile_rows) - int(rank) * kCtaRows, 0), kCtaRows) : 0;
+    const bool f16 = a.c_f16;
+    const int width = kTN / split, pieces = width / 8;  // powers of two, at most 32 pieces
+    // A thread keeps its piece of eight columns over all its rows.
+    const int et = threadIdx.x - 64, step = 32 * kEpiWarps / pieces;
+    const int r0 = et / pieces, lc = range * width + (et - r0 * pieces) * 8;
+    const int col = w.tn * kTN + lc;
+    const bool cols_in = et >= 0 && has && col < a.N;
+    float sb[8], bias[8];
+    auto load_residual = [&](int r) {
+      const int dst = r < live && cols_in ? S.dst[r] : -1;
+      return dst >= 0 ? load8(a.residual, a.vec, int64_t(dst) * a.N + col, a.N - col) : make_uint4(0u, 0u, 0u, 0u);
+    };
+    uint4 res;
+    if (warp >= 2) {
+      // What does not wait for the products: scales, places, the residual.
+      if (et < live) {
+        const int row = w.row0 + int(rank) * kCtaRows + et;
+        S.scale[et] = a.sA[row];
+        int dst = row;
+        if (kGrouped && a.c_rows) dst = a.c_rows[row] < a.c_dst_rows ? a.c_rows[row] : -1;
+        S.dst[et] = dst;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sb[j] = bias[j] = 0.f;
+      if (cols_in) {
+        const float* p = a.sB + int64_t(w.group) * a.N + col;
+        if (a.vec) {
+          *reinterpret_cast<float4*>(sb) = *reinterpret_cast<const float4*>(p);
+          *reinterpret_cast<float4*>(sb + 4) = *reinterpret_cast<const float4*>(p + 4);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (col + j < a.N) sb[j] = p[j];
+        }
+        if (!kGrouped && a.bias_kind == kBiasF32) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (col + j < a.N) bias[j] = static_cast<const float*>(a.bias)[col + j];
+        } else if (!kGrouped && a.bias_kind) {
+          const uint4 u = load8(a.bias, a.vec, col, a.N - col);
+          const uint32_t uw[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 g = unpack_half2(uw[j], f16);
+            bias[2 * j] = g.x;
+            bias[2 * j + 1] = g.y;
+          }
+        }
+      }
+      named_barrier_sync(1, 32 * kEpiWarps);  // S.scale and S.dst are in
+      if (!kGrouped && a.residual) res = load_residual(r0);
       const int q = warp & 3, h = (warp - 2) >> 2;
-      const bool ok = mbar_wait_warp(&S.acc_full[0], 0, abort_flag, a.sync, a.wait_budget, a.wait_hint_ns);
+      const bool ok = has && mbar_wait_warp(&S.acc_full[0], 0, abort_flag, a.sync, a.wait_budget, a.wait_hint_ns);
       tc_fence_after();
       if (ok && 32 * q < live) {
 #pragma unroll 1
@@ -548,40 +663,36 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         }
       }
     }
-    cluster_sync_all();
-    if (warp >= 2 && !*abort_flag) {
-      const bool f16 = a.c_f16;
-      const int width = kTN / split, pieces = width / 8;
-      for (int i = threadIdx.x - 64; i < live * pieces; i += 32 * kEpiWarps) {
-        const int r = i / pieces, lc = range * width + (i - r * pieces) * 8;
-        const int col = w.tn * kTN + lc;
-        if (col >= a.N) continue;
-        const int row = w.row0 + int(rank) * kCtaRows + r;
-        int dst = row;
-        if (kGrouped && a.c_rows) dst = a.c_rows[row];
-        if (dst < 0 || (kGrouped && dst >= a.c_dst_rows)) continue;
-        uint4 res = make_uint4(0u, 0u, 0u, 0u);
-        if (!kGrouped && a.residual) res = load8(a.residual, a.vec, int64_t(dst) * a.N + col, a.N - col);
+    if (split > 1) cluster_sync_all();
+    else __syncthreads();
+    if (cols_in && !*abort_flag) {
+      for (int r = r0; r < live; r += step) {
+        const int dst = S.dst[r];
         int acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        const uint8_t* p0 = ring + r * kTN * 4 + (((lc / 4) ^ (r & 7)) << 4);
-        const uint8_t* p1 = ring + r * kTN * 4 + (((lc / 4 + 1) ^ (r & 7)) << 4);
-        for (int s = 0; s < split; ++s) {
-          const int4 x = ld_cluster_v4(mapa(p0, s * kCtas + rank)), y = ld_cluster_v4(mapa(p1, s * kCtas + rank));
+        auto add = [&](int4 x, int4 y) {
           acc[0] += x.x; acc[1] += x.y; acc[2] += x.z; acc[3] += x.w;
           acc[4] += y.x; acc[5] += y.y; acc[6] += y.z; acc[7] += y.w;
+        };
+        const uint8_t* p0 = ring + r * kTN * 4 + (((lc / 4) ^ (r & 7)) << 4);
+        const uint8_t* p1 = ring + r * kTN * 4 + (((lc / 4 + 1) ^ (r & 7)) << 4);
+        if (split == 1) {
+          add(*reinterpret_cast<const int4*>(p0), *reinterpret_cast<const int4*>(p1));
+        } else {
+          for (int s = 0; s < split; s += 2) {  // split is even: four loads in flight
+            const uint32_t c = s * kCtas + rank;
+            const int4 x0 = ld_cluster_v4(mapa(p0, c)), y0 = ld_cluster_v4(mapa(p1, c));
+            const int4 x1 = ld_cluster_v4(mapa(p0, c + kCtas)), y1 = ld_cluster_v4(mapa(p1, c + kCtas));
+            add(x0, y0);
+            add(x1, y1);
+          }
         }
-        const float rs = a.sA[row];
+        const uint4 mine = res;
+        if (!kGrouped && a.residual) res = load_residual(r + step);
+        if (dst < 0) continue;
+        const float rs = S.scale[r];
         float f[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          float bias = 0.f, sb = 0.f;
-          if (col + j < a.N) {
-            sb = a.sB[int64_t(w.group) * a.N + col + j];
-            if (!kGrouped && a.bias_kind)
-              bias = a.bias_kind == kBiasF32 ? static_cast<const float*>(a.bias)[col + j] : half_at(a.bias, col + j, f16);
-          }
-          f[j] = fmaf(float(acc[j]) * rs, sb, bias);
-        }
+        for (int j = 0; j < 8; ++j) f[j] = fmaf(float(acc[j]) * rs, sb[j], bias[j]);
         if constexpr (!kGrouped) {
           switch (a.act) {
             case PB2_ACT_RELU: activate8<PB2_ACT_RELU>(f); break;
@@ -591,7 +702,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
             default: break;
           }
           if (a.residual) {
-            const uint32_t rw[4] = {res.x, res.y, res.z, res.w};
+            const uint32_t rw[4] = {mine.x, mine.y, mine.z, mine.w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const float2 g = unpack_half2(rw[j], f16);
@@ -610,12 +721,12 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
   // barriers, tensor memory or sums.
   tc_fence_before();
   __syncthreads();
-  if constexpr (kPair || kSplit) cluster_sync_all();
+  if (kPair || split > 1) cluster_sync_all();
   tc_fence_after();
   if (warp == 1) {
     __syncwarp();
-    if constexpr (kPair) tmem_dealloc_2sm(tmem, 2 * kTN);
-    else tmem_dealloc(tmem, 2 * kTN);
+    if constexpr (kPair) tmem_dealloc_2sm(tmem, kTmemCols);
+    else tmem_dealloc(tmem, kTmemCols);
   }
 }
 
@@ -648,7 +759,10 @@ int resident_pairs(int device, const void* kern, int smem) {
   return n;
 }
 
-template <bool kPair, int kTN, bool kGrouped, bool kSplit>
+// Shared memory of a CTA that leaves room for another on its SM.
+constexpr int kHalfSm = 115712;
+
+template <bool kPair, int kTN, bool kGrouped, bool kOnce>
 int launch_product(ProductArgs& a, const int8_t* A, const int8_t* B, int cta_rows, int device, cudaStream_t s) {
   constexpr int kCtas = kPair ? 2 : 1;
   constexpr int kBRows = kTN / kCtas;
@@ -662,12 +776,16 @@ int launch_product(ProductArgs& a, const int8_t* A, const int8_t* B, int cta_row
       (st = make_tmap_2d(&a.tmB, B, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, uint64_t(std::max(a.groups, 1)) * a.N, kTileK,
                          kBRows, CU_TENSOR_MAP_SWIZZLE_128B)))
     return st;
-  const int fixed = 1024 + kEpiWarps * (kBoxBytes + kTN / 2 * 8) + int(sizeof(ProductSmem));
-  a.stages = std::min(kMaxStages, (232448 - fixed) / (a.a_bytes + kBRows * kTileK));
+  const int fixed = 1024 + int(sizeof(ProductSmem)) + (kOnce ? 0 : kEpiWarps * (kBoxBytes + kTN / 2 * 8));
+  a.stages = std::min(kMaxStages, ((kOnce ? kHalfSm : 232448) - fixed) / (a.a_bytes + kBRows * kTileK));
+  // Whole loads of A in a stage, and with kOnce a tile's sums in the ring.
+  if (cta_rows % a.box_rows || cta_rows > kCtaRows || (kPair && cta_rows != kCtaRows) ||
+      (kOnce && cta_rows * kTN * 4 > a.stages * (a.a_bytes + kBRows * kTileK)))
+    return PB2_ERR_UNSUPPORTED_CONFIG;
   a.wait_budget = wait_budget_cycles();
   a.wait_hint_ns = suspend_hint_ns(a.wait_budget);
   const int smem = fixed + a.stages * (a.a_bytes + kBRows * kTileK);
-  auto kern = product_kernel<kPair, kTN, kGrouped, kSplit>;
+  auto kern = product_kernel<kPair, kTN, kGrouped, kOnce>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return launch_status();
   // Row tiles: exact without groups; with them, whose sizes only the device
@@ -675,12 +793,12 @@ int launch_product(ProductArgs& a, const int8_t* A, const int8_t* B, int cta_row
   const int64_t tiles_m = kGrouped ? int64_t(a.M) / a.tile_rows + std::min(a.groups, a.M)
                                    : (int64_t(a.M) + a.tile_rows - 1) / a.tile_rows;
   int64_t clusters = tiles_m * a.tiles_n;
-  if (!kSplit) {
+  if (!kOnce) {
     const int most = kPair ? resident_pairs(device, reinterpret_cast<const void*>(kern), smem)
                            : std::max(1, sm_count(device));
     clusters = std::min<int64_t>(clusters, most);
   }
-  const int cluster = kCtas * (kSplit ? a.split : 1);
+  const int cluster = kCtas * (kOnce ? a.split : 1);
   return launch_programmatic(kern, dim3(unsigned(clusters * cluster)), kThreads, smem, s, cluster, a);
 }
 
@@ -703,7 +821,7 @@ int run_product(ProductArgs& a, const int8_t* A, const int8_t* B, int device, cu
     a.box_rows = kCtaRows;
     const int64_t tiles = (int64_t(a.M) + 255) / 256 * ((a.N + 255) / 256);
     a.split = kGrouped ? 1 : split_of(tiles, 2, kblocks, sms);
-    if (a.split > 1) return launch_product<true, 256, kGrouped, true>(a, A, B, kCtaRows, device, s);
+    if (a.split > 1) return launch_product<true, 128, kGrouped, true>(a, A, B, kCtaRows, device, s);
     return launch_product<true, 256, kGrouped, false>(a, A, B, kCtaRows, device, s);
   }
   const int cta_rows = std::min(kCtaRows, (a.M + 7) / 8 * 8);
@@ -816,7 +934,7 @@ extern "C" int pb2_gemm_epilogue(const pb2_gemm_epilogue_params* pp, void* strea
   a.M = int(p.m);
   a.N = int(p.n);
   a.K = int(p.k);
-  a.vec = p.n % 8 == 0 && al16(p.C) && al16(p.residual);
+  a.vec = p.n % 8 == 0 && al16(p.C) && al16(p.residual) && al16(p.B_scales) && al16(p.bias);
   a.sync = static_cast<SignalSync*>(p.host_signal_sync);
   return run_product<false>(a, p.A, p.B, p.device, static_cast<cudaStream_t>(stream));
 }
@@ -849,7 +967,7 @@ extern "C" int pb2_gemm_grouped(const pb2_gemm_grouped_params* pp, void* stream)
   a.ends = p.routing_offsets;
   a.c_rows = p.c_row_index;
   a.c_dst_rows = int(std::min<int64_t>(p.c_row_index ? p.c_rows : p.m, INT32_MAX));
-  a.vec = p.n % 8 == 0 && al16(p.C);
+  a.vec = p.n % 8 == 0 && al16(p.C) && al16(p.B_scales);
   a.sync = static_cast<SignalSync*>(p.host_signal_sync);
   return run_product<true>(a, p.A, p.B, p.device, static_cast<cudaStream_t>(stream));
 }

@@ -260,9 +260,7 @@ __device__ __forceinline__ void build_groups(const ProductArgs& a, ProductSmem& 
 // cluster whose CTAs (pairs) take a.split ranges of its K and add their int32
 // sums up through distributed shared memory, each finishing its share of the
 // columns: the weights are then read through all SMs.  int32 sums are exact,
-// so C does not depend on the split.  Half an SM's shared memory, so that the
-// set-up of one product overlaps the end of the one before it.
-// Otherwise the grid is persistent and the accumulator double-buffered.
+// so C does not depend on the split.  Otherwise the grid is persistent and the accumulator double-buffered.
 template <bool kPair, int kTN, bool kGrouped, bool kOnce>
 __global__ void __launch_bounds__(kThreads, kOnce ? 2 : 1) product_kernel(const __grid_constant__ ProductArgs a) {
   constexpr int kCtas = kPair ? 2 : 1;
@@ -759,7 +757,10 @@ int resident_pairs(int device, const void* kern, int smem) {
   return n;
 }
 
-// Shared memory of a CTA that leaves room for another on its SM.
+// Shared memory of a CTA that leaves room for another on its SM: for short K
+// ranges, so that the set-up of one product overlaps the end of the one before
+// it (1 x 4096 x 4096 in ranges of 8 blocks 6.7 us, 7.0 with a full ring;
+// 64 x 4096 x 14336 in ranges of 28 blocks 18.6, 16.4 with a full ring).
 constexpr int kHalfSm = 115712;
 
 template <bool kPair, int kTN, bool kGrouped, bool kOnce>
@@ -777,7 +778,8 @@ int launch_product(ProductArgs& a, const int8_t* A, const int8_t* B, int cta_row
                          kBRows, CU_TENSOR_MAP_SWIZZLE_128B)))
     return st;
   const int fixed = 1024 + int(sizeof(ProductSmem)) + (kOnce ? 0 : kEpiWarps * (kBoxBytes + kTN / 2 * 8));
-  a.stages = std::min(kMaxStages, ((kOnce ? kHalfSm : 232448) - fixed) / (a.a_bytes + kBRows * kTileK));
+  const bool half = kOnce && (a.K + kTileK - 1) / kTileK <= 8 * a.split;
+  a.stages = std::min(kMaxStages, ((half ? kHalfSm : 232448) - fixed) / (a.a_bytes + kBRows * kTileK));
   // Whole loads of A in a stage, and with kOnce a tile's sums in the ring.
   if (cta_rows % a.box_rows || cta_rows > kCtaRows || (kPair && cta_rows != kCtaRows) ||
       (kOnce && cta_rows * kTN * 4 > a.stages * (a.a_bytes + kBRows * kTileK)))
@@ -802,36 +804,79 @@ int launch_product(ProductArgs& a, const int8_t* A, const int8_t* B, int cta_row
   return launch_programmatic(kern, dim3(unsigned(clusters * cluster)), kThreads, smem, s, cluster, a);
 }
 
-// K ranges for a product of `tiles` tiles of `ctas` CTAs: a power of two, at
-// most 8 CTAs to a cluster, as long as the ranges keep all clusters resident
-// and kMinRange K blocks each (a join costs about as much as that many).
-constexpr int kMinRange = 4;
-int split_of(int64_t tiles, int ctas, int kblocks, int sms) {
-  int split = 1;
-  while (2 * split * ctas <= 8 && tiles * ctas * 2 * split <= sms && kblocks / (2 * split) >= kMinRange) split *= 2;
-  return split;
+// The variant for a product is the one with the smallest estimate of its
+// time, in us: a start and end, and for each K block of a CTA's tiles what a
+// stage of that tile takes.  Fitted to products of 1 to 2048 rows, 2048 to
+// 14336 columns and 1040 to 14336 of K, whose measured times it meets within
+// about 15% and whose order it keeps; the measured pairs beside the rules
+// are us.
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+int run_linear(ProductArgs& a, const int8_t* A, const int8_t* B, int device, cudaStream_t s) {
+  const int64_t sms = std::max(1, sm_count(device)), pairs = sms / 2;
+  const int64_t kblocks = ceil_div(a.K, kTileK), m = a.M, n = a.N;
+  const int cta_rows = int(std::min<int64_t>(kCtaRows, ceil_div(m, 8) * 8));
+  a.box_rows = cta_rows;
+  // Persistent: 256 x 256 tiles of CTA pairs, 256 x 128 of pairs, 128 x 128.
+  // (1024 x 4096 x 4096: 18.7 | 19.5 | 20.7; 512 x 4096 x 14336: 41 | 28 | 32;
+  // 777 x 2048 x 2048: 11 | 8.8 | 8.2.)
+  const double wide = 8.0 + 0.33 * double(ceil_div(ceil_div(m, 256) * ceil_div(n, 256), pairs) * kblocks);
+  const double pair = 6.0 + 0.20 * double(ceil_div(ceil_div(m, 256) * ceil_div(n, 128), pairs) * kblocks);
+  const double single = 4.5 + 0.25 * double(ceil_div(ceil_div(m, 128) * ceil_div(n, 128), sms) * kblocks);
+  // One tile a cluster, K split over it as far as the SMs, a cluster of four
+  // CTAs (of eight, most have to wait for a second round) and kMinRange K
+  // blocks a range allow.  (1 x 4096 x 4096: 6.5, unsplit 10.7;
+  // 256 x 4096 x 14336: 22 in pairs, unsplit 27.)
+  constexpr int kMinRange = 4;
+  auto split_of = [&](int64_t tiles, int ctas) {
+    int split = 1;
+    while (2 * split * ctas <= 4 && tiles * ctas * 2 * split <= sms && kblocks / (2 * split) >= kMinRange) split *= 2;
+    return split;
+  };
+  const int split1 = split_of(ceil_div(m, 128) * ceil_div(n, 128), 1), split2 = split_of(ceil_div(m, 256) * ceil_div(n, 128), 2);
+  const double join = 5.0 + 0.035 * double(std::min<int64_t>(m, 128)), never = 1e30;
+  const double once1 = split1 > 1 ? join + 0.25 * double(ceil_div(kblocks, split1)) : never;
+  const double once2 = split2 > 1 && m > kCtaRows ? join + 0.20 * double(ceil_div(kblocks, split2)) : never;
+  const double best = std::min({m > kCtaRows ? std::min(wide, pair) : never, single, once1, once2});
+  if (best == once1 || best == once2) {
+    a.split = best == once1 ? split1 : split2;
+    if (best == once1) return launch_product<false, 128, false, true>(a, A, B, cta_rows, device, s);
+    return launch_product<true, 128, false, true>(a, A, B, cta_rows, device, s);
+  }
+  a.split = 1;
+  if (best == single) return launch_product<false, 128, false, false>(a, A, B, cta_rows, device, s);
+  if (best == pair) return launch_product<true, 128, false, false>(a, A, B, cta_rows, device, s);
+  return launch_product<true, 256, false, false>(a, A, B, cta_rows, device, s);
 }
 
-template <bool kGrouped>
-int run_product(ProductArgs& a, const int8_t* A, const int8_t* B, int device, cudaStream_t s) {
-  const int sms = std::max(1, sm_count(device));
-  const int kblocks = (a.K + kTileK - 1) / kTileK;
-  const int64_t rows = kGrouped ? a.M / a.groups : a.M;  // of a group, on average
-  if (rows > kCtaRows) {
+int run_grouped(ProductArgs& a, const int8_t* A, const int8_t* B, int device, cudaStream_t s) {
+  const int64_t sms = std::max(1, sm_count(device));
+  const int64_t kblocks = ceil_div(a.K, kTileK), average = a.M / a.groups;
+  a.split = 1;
+  // Groups of more rows than a CTA's tile: pairs (16 groups of 256 rows,
+  // 4096 x 4096: 85, single CTAs 94; of 128 rows 64, single CTAs 62).
+  if (average > kCtaRows + kCtaRows / 4) {
     a.box_rows = kCtaRows;
-    const int64_t tiles = (int64_t(a.M) + 255) / 256 * ((a.N + 255) / 256);
-    a.split = kGrouped ? 1 : split_of(tiles, 2, kblocks, sms);
-    if (a.split > 1) return launch_product<true, 128, kGrouped, true>(a, A, B, kCtaRows, device, s);
-    return launch_product<true, 256, kGrouped, false>(a, A, B, kCtaRows, device, s);
+    return launch_product<true, 256, true, false>(a, A, B, kCtaRows, device, s);
   }
-  const int cta_rows = std::min(kCtaRows, (a.M + 7) / 8 * 8);
-  a.box_rows = cta_rows;
-  const int64_t tiles_n = (a.N + 127) / 128;
-  const int64_t tiles = (kGrouped ? std::min(a.groups, a.M) : 1) * tiles_n;
-  a.split = split_of(tiles, 1, kblocks, sms);
-  // A K range's sums fit the ring of a CTA whatever its stages (64 KB).
-  if (a.split > 1) return launch_product<false, 128, kGrouped, true>(a, A, B, cta_rows, device, s);
-  return launch_product<false, 128, kGrouped, false>(a, A, B, cta_rows, device, s);
+  // The weights bound what is left: a stage holds no more rows of A than
+  // groups of this size need, so that more of it is weights in flight (60
+  // groups of 22 rows: 34 with 64 rows a stage, 38 with 128).
+  int cta_rows = average <= 16 ? 32 : average <= 64 ? 64 : kCtaRows;
+  cta_rows = int(std::min<int64_t>(cta_rows, ceil_div(a.M, 8) * 8));
+  a.box_rows = std::min(cta_rows, 32);
+  cta_rows = int(ceil_div(cta_rows, a.box_rows)) * a.box_rows;
+  const int64_t used = std::min<int64_t>(a.groups, a.M);
+  const int64_t tiles_m = used + a.M / (2 * cta_rows);  // about
+  const int64_t narrow = tiles_m * ceil_div(a.N, 128), broad = tiles_m * ceil_div(a.N, 256);
+  while (narrow * 2 * a.split <= sms && 2 * a.split <= 4 && kblocks / (2 * a.split) >= 4) a.split *= 2;
+  if (a.split > 1) return launch_product<false, 128, true, true>(a, A, B, cta_rows, device, s);
+  // 128 columns a tile, or 256 with half the loads of A (128 groups of 128
+  // rows: 63 | 55; 20 groups of one row or two, 2048 x 1408: 14.3 | 15.6).
+  const double full = cta_rows == kCtaRows ? 1.0 : 0.9;
+  if (0.22 * full * double(ceil_div(narrow, sms)) < 0.32 * double(ceil_div(broad, sms)))
+    return launch_product<false, 128, true, false>(a, A, B, cta_rows, device, s);
+  return launch_product<false, 256, true, false>(a, A, B, cta_rows, device, s);
 }
 
 // out[t] = residual[t] + sum_j w[t, j] * slots[t * top_k + j], f32 sums in
@@ -936,7 +981,7 @@ extern "C" int pb2_gemm_epilogue(const pb2_gemm_epilogue_params* pp, void* strea
   a.K = int(p.k);
   a.vec = p.n % 8 == 0 && al16(p.C) && al16(p.residual) && al16(p.B_scales) && al16(p.bias);
   a.sync = static_cast<SignalSync*>(p.host_signal_sync);
-  return run_product<false>(a, p.A, p.B, p.device, static_cast<cudaStream_t>(stream));
+  return run_linear(a, p.A, p.B, p.device, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int pb2_gemm_grouped(const pb2_gemm_grouped_params* pp, void* stream) {
@@ -969,7 +1014,7 @@ extern "C" int pb2_gemm_grouped(const pb2_gemm_grouped_params* pp, void* stream)
   a.c_dst_rows = int(std::min<int64_t>(p.c_row_index ? p.c_rows : p.m, INT32_MAX));
   a.vec = p.n % 8 == 0 && al16(p.C) && al16(p.B_scales);
   a.sync = static_cast<SignalSync*>(p.host_signal_sync);
-  return run_product<true>(a, p.A, p.B, p.device, static_cast<cudaStream_t>(stream));
+  return run_grouped(a, p.A, p.B, p.device, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int pb2_combine_slots(const pb2_combine_params* pp, void* stream) {

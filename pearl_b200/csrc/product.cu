@@ -46,6 +46,7 @@ struct ProductArgs {
   int box_rows, a_bytes;   // rows of an A load; A bytes of a stage
   int stages;
   int split;               // K ranges, one per CTA (pair) of the cluster
+  int early;               // only A and sA come from the kernel before this one (see the start of the kernel)
   int vec;                 // rows of C and residual can be moved 16 bytes at a time
   SignalSync* sync;
   long long wait_budget;
@@ -328,7 +329,11 @@ __global__ void __launch_bounds__(kThreads, kOnce ? 2 : 1) product_kernel(const 
         tma_prefetch_l2_2d(&a.tmB, kb * kTileK, w.tn * kTN + int(rank) * kBRows);
     }
   }
-  griddep_wait();
+  // Programmatic dependent launch: with a.early everything but A and sA was
+  // complete before the kernel before this one could let it start (that
+  // kernel waits for its own predecessors first), so the groups and the first
+  // stages of B are read while it is still running.
+  if (!kGrouped || !a.early) griddep_wait();
   griddep_launch_dependents();
   if constexpr (kGrouped) build_groups(a, S);
   const uint32_t tmem = S.tmem_base;
@@ -342,6 +347,7 @@ __global__ void __launch_bounds__(kThreads, kOnce ? 2 : 1) product_kernel(const 
       const uint32_t past = 8 * a.stages;
       uint32_t at = 0, dst = ring0, phase = 1;  // of the stage: barrier offset, address, wait parity
       const int box_bytes = a.box_rows * kTileK;
+      bool early = kGrouped && a.early;
       for (int t = first; t < tiles && ok; t += stride) {
         const Tile w = tile_at<kGrouped>(a, S, t);
         const int arow = w.row0 + int(rank) * kCtaRows;
@@ -354,18 +360,36 @@ __global__ void __launch_bounds__(kThreads, kOnce ? 2 : 1) product_kernel(const 
         const int mine = boxes_of(rank);
         const int bytes = kCtas * kBBytes + (boxes_of(0) + (kPair ? boxes_of(1) : 0)) * box_bytes;
         const int x1 = kb1 * kTileK;
-        for (int x = kb0 * kTileK; x < x1; x += kTileK) {
+        int x = kb0 * kTileK;
+        auto load_a = [&](uint32_t bar, uint32_t to, int k) {
+          if (mine == 1) {
+            load_box<kPair>(&a.tmA, bar, to, k, arow);
+          } else {
+            for (int i = 0; i < mine; ++i) load_box<kPair>(&a.tmA, bar, to + i * box_bytes, k, arow + i * a.box_rows);
+          }
+        };
+        if (kGrouped && early) {  // the ring is empty: B of its first round, then the wait, then A
+          early = false;
+          const int n = min(a.stages, kb1 - kb0);
+          for (int i = 0; i < n; ++i) {
+            if (rank == 0) bar_expect(full0 + 8 * i, bytes);
+            load_box<kPair>(&a.tmB, full0 + 8 * i, ring0 + i * stage_bytes + a.a_bytes, x + i * kTileK, brow);
+          }
+          griddep_wait();
+          for (int i = 0; i < n; ++i) load_a(full0 + 8 * i, ring0 + i * stage_bytes, x + i * kTileK);
+          x += n * kTileK;
+          at = 8 * n;
+          dst = ring0 + n * stage_bytes;
+          if (at == past) { at = 0; dst = ring0; phase ^= 1; }
+        }
+        for (; x < x1; x += kTileK) {
           if (!bar_ready(empty0 + at, phase) &&
               !(ok = mbar_wait(&S.empty[at / 8], phase, abort_flag, a.sync, a.wait_budget, a.wait_hint_ns)))
             break;
           // The pair leader's barrier counts both CTAs' bytes.
           if (rank == 0) bar_expect(full0 + at, bytes);
           load_box<kPair>(&a.tmB, full0 + at, dst + a.a_bytes, x, brow);
-          if (mine == 1) {
-            load_box<kPair>(&a.tmA, full0 + at, dst, x, arow);
-          } else {
-            for (int i = 0; i < mine; ++i) load_box<kPair>(&a.tmA, full0 + at, dst + i * box_bytes, x, arow + i * a.box_rows);
-          }
+          load_a(full0 + at, dst, x);
           at += 8;
           dst += stage_bytes;
           if (at == past) { at = 0; dst = ring0; phase ^= 1; }
@@ -485,6 +509,7 @@ __global__ void __launch_bounds__(kThreads, kOnce ? 2 : 1) product_kernel(const 
     const int piece = lane & 7;
     bool ok = true;
     int n = 0;
+    if (kGrouped && a.early) griddep_wait();
     Meta next = load_meta(first);
     for (int t = first; t < tiles && ok; t += stride, ++n) {
       const Meta m = next;
@@ -604,6 +629,7 @@ __global__ void __launch_bounds__(kThreads, kOnce ? 2 : 1) product_kernel(const 
     };
     uint4 res;
     if (warp >= 2) {
+      if (kGrouped && a.early) griddep_wait();
       // What does not wait for the products: scales, places, the residual.
       if (et < live) {
         const int row = w.row0 + int(rank) * kCtaRows + et;
@@ -984,11 +1010,9 @@ extern "C" int pb2_gemm_epilogue(const pb2_gemm_epilogue_params* pp, void* strea
   return run_linear(a, p.A, p.B, p.device, static_cast<cudaStream_t>(stream));
 }
 
-extern "C" int pb2_gemm_grouped(const pb2_gemm_grouped_params* pp, void* stream) {
-  pb2::NvtxRange nvtx_range("pb2_gemm_grouped");
-  using namespace pb2;
-  if (!pp) return PB2_ERR_INVALID_ARGUMENT;
-  const pb2_gemm_grouped_params& p = *pp;
+namespace pb2 {
+// `early`: see ProductArgs.
+int gemm_grouped(const pb2_gemm_grouped_params& p, bool early, cudaStream_t stream) {
   if (p.m < 0 || p.n <= 0 || p.k <= 0 || p.m > INT32_MAX || p.k > INT32_MAX) return PB2_ERR_INVALID_ARGUMENT;
   if (p.num_experts <= 0 || p.num_experts > kMaxGroups || p.n > INT32_MAX / p.num_experts) return PB2_ERR_INVALID_ARGUMENT;
   if (!type16(p.c_type)) return PB2_ERR_INVALID_ARGUMENT;
@@ -1014,7 +1038,15 @@ extern "C" int pb2_gemm_grouped(const pb2_gemm_grouped_params* pp, void* stream)
   a.c_dst_rows = int(std::min<int64_t>(p.c_row_index ? p.c_rows : p.m, INT32_MAX));
   a.vec = p.n % 8 == 0 && al16(p.C) && al16(p.B_scales);
   a.sync = static_cast<SignalSync*>(p.host_signal_sync);
-  return run_grouped(a, p.A, p.B, p.device, static_cast<cudaStream_t>(stream));
+  a.early = early;
+  return run_grouped(a, p.A, p.B, p.device, stream);
+}
+}  // namespace pb2
+
+extern "C" int pb2_gemm_grouped(const pb2_gemm_grouped_params* pp, void* stream) {
+  pb2::NvtxRange nvtx_range("pb2_gemm_grouped");
+  if (!pp) return PB2_ERR_INVALID_ARGUMENT;
+  return pb2::gemm_grouped(*pp, false, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int pb2_combine_slots(const pb2_combine_params* pp, void* stream) {
@@ -1113,7 +1145,8 @@ extern "C" int pb2_gated_experts(const pb2_gated_experts_params* pp, void* strea
     return PB2_ERR_INVALID_ARGUMENT;
   if (p.inner % 16 != 0) return PB2_ERR_UNSUPPORTED_CONFIG;
   int st = pb2_quantize_gated(&q, stream);
-  if (!st) st = pb2_gemm_grouped(&g, stream);
+  // The quantizer writes A and its scales; weights and routing are older.
+  if (!st) st = gemm_grouped(g, true, static_cast<cudaStream_t>(stream));
   if (!st) st = pb2_combine_slots(&c, stream);
   return st;
 }

@@ -431,3 +431,34 @@ def test_gated_experts_is_its_three_steps(m, E, k, hidden, inner, dtype, residua
         total, mag = total + r.double(), mag + r.double().abs()
     # each slot's product is rounded to the type before the sum
     within(out, total, mag * (HALF_ULP[dtype] * 1.01 + 2.0 ** -19) + k * 2.0 ** -25, dtype)
+
+
+@pytest.mark.parametrize("m,E,k,hidden,inner", [(8, 8, 2, 4096, 2048), (2, 8, 2, 512, 4096), (900, 64, 4, 512, 768), (1500, 4, 2, 1024, 512)])
+def test_gated_experts_back_to_back(m, E, k, hidden, inner):
+    """Calls queued one behind the other, each with inputs written just before
+    it on the same stream: the product's early loads take none of them."""
+    g = gen(m + inner)
+    w, ids = route(randn(g, m, E), k)
+    slots = m * k
+    data, slot, ends = (torch.empty(s, dtype=torch.int32, device="cuda") for s in (slots, slots, E))
+    scratch = torch.empty(pg.moe.get_build_routing_data_scratchpad_bytes(slots), dtype=torch.uint8, device="cuda")
+    pg.moe.build_routing_data(ids, data, slot, ends, scratch, E)
+    W, ws = int8(g, E, hidden, inner), (torch.rand(E, hidden, generator=g, device="cuda") + 0.5) * 1e-3
+    xs = [randn(g, slots, 2 * inner).to(BF16) for _ in range(12)]
+    x = torch.empty_like(xs[0])
+    space = torch.empty(pg.moe.get_gated_experts_workspace_bytes(slots, inner, hidden), dtype=torch.uint8, device="cuda")
+    outs = [torch.empty(m, hidden, dtype=BF16, device="cuda") for _ in xs]
+    torch.cuda.synchronize()
+    for src, out in zip(xs, outs):
+        x.copy_(src)
+        pg.moe.gated_experts(x, W, ws, out, slot, ends, w, workspace=space)
+    torch.cuda.synchronize()
+    for src, out in zip(xs, outs):
+        q, sc = torch.empty(slots, inner, dtype=torch.int8, device="cuda"), torch.empty(slots, device="cuda")
+        y, want = torch.empty(slots, hidden, dtype=BF16, device="cuda"), torch.empty_like(out)
+        for step in (lambda: pg.quantization.quantize_gated(src, q, sc, row_index=slot),
+                     lambda: pg.moe.gemm_grouped(q, W, sc, ws, y, ends, c_row_index=slot),
+                     lambda: pg.moe.combine_slots(y, w, want)):
+            step()
+            torch.cuda.synchronize()
+        assert torch.equal(out, want)

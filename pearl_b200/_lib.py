@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -232,6 +233,18 @@ def load() -> ctypes.CDLL:
         L.pb2_rcp_approx_f32.argtypes = [ctypes.c_int, _vp, _vp, _i64, _vp]
         _lib = L
     return _lib
+
+
+_FORMAT = {ctypes.c_int: "i", ctypes.c_int64: "q", ctypes.c_void_p: "P", ctypes.c_float: "f"}
+
+
+def packer(params):
+    """A function that takes a parameter struct's fields in order (addresses
+    as integers, 0 for NULL) and gives its bytes, for an entry point's
+    argument: a third of the time it takes to fill a ctypes structure."""
+    layout = struct.Struct("@" + "".join(_FORMAT[t] for _, t in params._fields_))
+    assert layout.size == ctypes.sizeof(params)
+    return layout.pack
 
 
 _functions: dict = {}

@@ -10,6 +10,7 @@
 // tensor memory) is being filled.  int32 sums are exact; the epilogue works
 // in f32 and rounds once.
 #include <algorithm>
+#include <atomic>
 #include <cstring>
 
 #include "pb2_epilogue.cuh"
@@ -814,8 +815,11 @@ int launch_product(ProductArgs& a, const int8_t* A, const int8_t* B, int cta_row
   a.wait_hint_ns = suspend_hint_ns(a.wait_budget);
   const int smem = fixed + a.stages * (a.a_bytes + kBRows * kTileK);
   auto kern = product_kernel<kPair, kTN, kGrouped, kOnce>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return launch_status();
+  static std::atomic<bool> allowed[64];  // the attribute holds for the process: set once a device
+  if (!allowed[device & 63].load(std::memory_order_relaxed)) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448) != cudaSuccess) return launch_status();
+    allowed[device & 63].store(true, std::memory_order_relaxed);
+  }
   // Row tiles: exact without groups; with them, whose sizes only the device
   // knows, at most one ragged tile a group beyond the whole ones.
   const int64_t tiles_m = kGrouped ? int64_t(a.M) / a.tile_rows + std::min(a.groups, a.M)

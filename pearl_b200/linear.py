@@ -12,6 +12,8 @@ from .pearl_gemm_interface import _call_on, _fail
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_INT8, _INT32, _FLOAT = (torch.int8,), (torch.int32,), (torch.float32,)
+_PACK = _lib.packer(_lib.GemmEpilogueParams)
 
 
 def _activation(name: str) -> int:
@@ -21,19 +23,20 @@ def _activation(name: str) -> int:
     return code
 
 
-def _operand(t, name: str, shape: tuple, dtypes: tuple, device) -> int:
-    """Address of a contiguous tensor of this shape, type and device."""
+def _operand(t, name: str, shape: tuple, dtypes: tuple, index: int) -> int:
+    """Address of a contiguous tensor of this shape and type on device
+    ``index``."""
+    if t.get_device() == index >= 0 and t.is_contiguous() and t.dtype in dtypes and t.shape == shape:
+        return t.data_ptr()
     if not t.is_cuda:
         _fail(f"{name} must be on CUDA")
-    if t.device != device:
-        _fail(f"{name} must be on {device}, got {t.device}")
+    if t.get_device() != index:
+        _fail(f"{name} must be on cuda:{index}, got {t.device}")
     if not t.is_contiguous():
         _fail(f"{name} must be contiguous")
     if t.dtype not in dtypes:
         _fail(f"expected dtype: {' or '.join(str(d) for d in dtypes)} but got this dtype: {t.dtype} ({name})")
-    if t.shape != shape:
-        _fail(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    return t.data_ptr()
+    _fail(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
 def _half_type(t, name: str) -> int:
@@ -42,9 +45,9 @@ def _half_type(t, name: str) -> int:
     return _TYPES[t.dtype]
 
 
-def _sync_word(sync):
+def _sync_word(sync) -> int:
     if sync is None:
-        return None
+        return 0
     if not sync.is_cuda or sync.numel() != _lib.HOST_SIGNAL_SYNC_SIZE:
         _fail(f"host_signal_sync must be a {_lib.HOST_SIGNAL_SYNC_SIZE}-byte CUDA buffer")
     return sync.data_ptr()
@@ -64,23 +67,18 @@ def gemm_epilogue(A, B, A_scales, B_scales, C, *, bias=None, activation: str = "
         _fail("A and B must be 2-D")
     m, k = A.shape
     n = B.shape[0]
-    dev = A.device
+    at = A.get_device()
     if k % 16:
         _fail(f"k must be a multiple of 16, got {k}")
     half = _half_type(C, "C")
-    p = _lib.GemmEpilogueParams()
-    p.A = _operand(A, "A", (m, k), (torch.int8,), dev)
-    p.B = _operand(B, "B", (n, k), (torch.int8,), dev)
-    p.A_scales = _operand(A_scales, "A_scales", (m,), (torch.float32,), dev)
-    p.B_scales = _operand(B_scales, "B_scales", (n,), (torch.float32,), dev)
-    p.C = _operand(C, "C", (m, n), (C.dtype,), dev)
-    if bias is not None:
-        p.bias, p.bias_type = _operand(bias, "bias", (n,), (torch.float32, C.dtype), dev), _TYPES[bias.dtype]
-    if residual is not None:
-        p.residual = _operand(residual, "residual", (m, n), (C.dtype,), dev)
-    p.m, p.n, p.k, p.c_type, p.activation = m, n, k, half, _activation(activation)
-    p.host_signal_sync = _sync_word(host_signal_sync)
-    _call_on(dev, "pb2_gemm_epilogue", p, "gemm_epilogue")
+    _call_on(at, "pb2_gemm_epilogue", _PACK(
+        at, m, n, k, _operand(A, "A", (m, k), _INT8, at), _operand(B, "B", (n, k), _INT8, at),
+        _operand(A_scales, "A_scales", (m,), _FLOAT, at), _operand(B_scales, "B_scales", (n,), _FLOAT, at),
+        _operand(C, "C", (m, n), (C.dtype,), at), half,
+        0 if bias is None else _operand(bias, "bias", (n,), (C.dtype, torch.float32), at),
+        0 if bias is None else _TYPES[bias.dtype], _activation(activation),
+        0 if residual is None else _operand(residual, "residual", (m, n), (C.dtype,), at),
+        _sync_word(host_signal_sync)), "gemm_epilogue")
 
 
 __all__ = ["ACTIVATIONS", "gemm_epilogue"]

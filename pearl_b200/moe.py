@@ -7,12 +7,14 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .linear import _activation, _half_type, _operand, _sync_word
+from .linear import _FLOAT, _INT8, _INT32, _TYPES, _activation, _half_type, _operand, _sync_word
 from .pearl_gemm_interface import _call_on, _device_index, _fail, _stream
 from .quantization import _check_block
 
 _SCORING = {"softmax": 0, "sigmoid": 1}
-_LOGIT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_LOGIT_TYPES = tuple(_TYPES)
+_PACK_ROUTE, _PACK_GROUPED = _lib.packer(_lib.RouteParams), _lib.packer(_lib.GemmGroupedParams)
+_PACK_COMBINE, _PACK_EXPERTS = _lib.packer(_lib.CombineParams), _lib.packer(_lib.GatedExpertsParams)
 MAX_EXPERTS = 256  # the routing order sorts 8-bit expert ids
 MAX_TOP_K = 32
 
@@ -219,7 +221,7 @@ def route_tokens(logits, topk_weights, topk_ids, *, scoring: str = "softmax", bi
         _fail("logits and topk_ids must be 2D (m, num_experts) and (m, top_k)")
     m, experts = logits.shape
     top_k = topk_ids.shape[1]
-    dev = logits.device
+    at = logits.get_device()
     if scoring not in _SCORING:
         _fail(f"scoring must be 'softmax' or 'sigmoid', got {scoring!r}")
     if not 1 <= experts <= MAX_EXPERTS:
@@ -229,16 +231,12 @@ def route_tokens(logits, topk_weights, topk_ids, *, scoring: str = "softmax", bi
               f"{num_groups} and {topk_groups}")
     if not 1 <= top_k <= min(MAX_TOP_K, topk_groups * (experts // num_groups)):
         _fail(f"top_k must be in 1..{min(MAX_TOP_K, topk_groups * (experts // num_groups))}, got {top_k}")
-    p = _lib.RouteParams()
-    p.logits = _operand(logits, "logits", (m, experts), tuple(_LOGIT_TYPES), dev)
-    p.topk_weights = _operand(topk_weights, "topk_weights", (m, top_k), (torch.float32,), dev)
-    p.topk_ids = _operand(topk_ids, "topk_ids", (m, top_k), (torch.int32,), dev)
-    if bias is not None:
-        p.bias = _operand(bias, "bias", (experts,), (torch.float32,), dev)
-    p.logits_type, p.num_tokens, p.num_experts, p.top_k = _LOGIT_TYPES[logits.dtype], m, experts, top_k
-    p.scoring, p.num_groups, p.topk_groups = _SCORING[scoring], num_groups, topk_groups
-    p.renormalize, p.scaling = bool(renormalize), scaling
-    _call_on(dev, "pb2_route_tokens", p, "route_tokens")
+    _call_on(at, "pb2_route_tokens", _PACK_ROUTE(
+        at, _operand(logits, "logits", (m, experts), _LOGIT_TYPES, at), _TYPES[logits.dtype], m, experts, top_k,
+        _SCORING[scoring], 0 if bias is None else _operand(bias, "bias", (experts,), _FLOAT, at), num_groups,
+        topk_groups, bool(renormalize), scaling,
+        _operand(topk_weights, "topk_weights", (m, top_k), _FLOAT, at),
+        _operand(topk_ids, "topk_ids", (m, top_k), _INT32, at)), "route_tokens")
 
 
 def gemm_grouped(A, B, A_scales, B_scales, C, routing_offsets, *, c_row_index=None, host_signal_sync=None) -> None:
@@ -256,25 +254,20 @@ def gemm_grouped(A, B, A_scales, B_scales, C, routing_offsets, *, c_row_index=No
         _fail("A and C must be 2-D and B 3-D (num_experts, n, k)")
     m, k = A.shape
     experts, n, _ = B.shape
-    dev = A.device
+    at = A.get_device()
     if k % 16:
         _fail(f"k must be a multiple of 16, got {k}")
     if not 1 <= experts <= MAX_EXPERTS:
         _fail(f"num_experts must be in 1..{MAX_EXPERTS}, got {experts}")
     half = _half_type(C, "C")
-    p = _lib.GemmGroupedParams()
-    p.A = _operand(A, "A", (m, k), (torch.int8,), dev)
-    p.B = _operand(B, "B", (experts, n, k), (torch.int8,), dev)
-    p.A_scales = _operand(A_scales, "A_scales", (m,), (torch.float32,), dev)
-    p.B_scales = _operand(B_scales, "B_scales", (experts, n), (torch.float32,), dev)
-    p.C = _operand(C, "C", (m if c_row_index is None else C.shape[0], n), (C.dtype,), dev)
-    p.routing_offsets = _operand(routing_offsets, "routing_offsets", (experts,), (torch.int32,), dev)
-    if c_row_index is not None:
-        p.c_row_index = _operand(c_row_index, "c_row_index", (m,), (torch.int32,), dev)
-        p.c_rows = C.shape[0]
-    p.m, p.n, p.k, p.num_experts, p.c_type = m, n, k, experts, half
-    p.host_signal_sync = _sync_word(host_signal_sync)
-    _call_on(dev, "pb2_gemm_grouped", p, "gemm_grouped")
+    rows = m if c_row_index is None else C.shape[0]
+    _call_on(at, "pb2_gemm_grouped", _PACK_GROUPED(
+        at, m, n, k, _operand(A, "A", (m, k), _INT8, at), _operand(B, "B", (experts, n, k), _INT8, at),
+        _operand(A_scales, "A_scales", (m,), _FLOAT, at), _operand(B_scales, "B_scales", (experts, n), _FLOAT, at),
+        _operand(C, "C", (rows, n), (C.dtype,), at), half, experts,
+        _operand(routing_offsets, "routing_offsets", (experts,), _INT32, at),
+        0 if c_row_index is None else _operand(c_row_index, "c_row_index", (m,), _INT32, at), rows,
+        _sync_word(host_signal_sync)), "gemm_grouped")
 
 
 def combine_slots(slots, topk_weights, out, *, residual=None) -> None:
@@ -287,16 +280,13 @@ def combine_slots(slots, topk_weights, out, *, residual=None) -> None:
         _fail("topk_weights and out must be 2D (m, top_k) and (m, n)")
     m, top_k = topk_weights.shape
     n = out.shape[1]
-    dev = out.device
+    at = out.get_device()
     half = _half_type(out, "out")
-    p = _lib.CombineParams()
-    p.slots = _operand(slots, "slots", (m * top_k, n), (out.dtype,), dev)
-    p.topk_weights = _operand(topk_weights, "topk_weights", (m, top_k), (torch.float32,), dev)
-    p.out = _operand(out, "out", (m, n), (out.dtype,), dev)
-    if residual is not None:
-        p.residual = _operand(residual, "residual", (m, n), (out.dtype,), dev)
-    p.type, p.num_tokens, p.top_k, p.n = half, m, top_k, n
-    _call_on(dev, "pb2_combine_slots", p, "combine_slots")
+    _call_on(at, "pb2_combine_slots", _PACK_COMBINE(
+        at, _operand(slots, "slots", (m * top_k, n), (out.dtype,), at),
+        _operand(topk_weights, "topk_weights", (m, top_k), _FLOAT, at),
+        0 if residual is None else _operand(residual, "residual", (m, n), (out.dtype,), at),
+        _operand(out, "out", (m, n), (out.dtype,), at), half, m, top_k, n), "combine_slots")
 
 
 def get_gated_experts_workspace_bytes(slots: int, inner: int, hidden: int) -> int:
@@ -323,7 +313,7 @@ def gated_experts(x, w, w_scales, out, slot_indices, routing_offsets, topk_weigh
     experts, hidden, inner = w.shape
     m, top_k = topk_weights.shape
     slots = m * top_k
-    dev = x.device
+    at = x.get_device()
     if inner % 16:
         _fail(f"inner must be a multiple of 16, got {inner}")
     if not 1 <= experts <= MAX_EXPERTS:
@@ -332,26 +322,21 @@ def gated_experts(x, w, w_scales, out, slot_indices, routing_offsets, topk_weigh
         _fail(f"max_val must be in 1..127, got {max_val}")
     _check_block(block_size, inner)
     half = _half_type(x, "x")
-    p = _lib.GatedExpertsParams()
-    p.x = _operand(x, "x", (slots, 2 * inner), (x.dtype,), dev)
-    p.w = _operand(w, "w", (experts, hidden, inner), (torch.int8,), dev)
-    p.w_scales = _operand(w_scales, "w_scales", (experts, hidden), (torch.float32,), dev)
-    p.out = _operand(out, "out", (m, hidden), (x.dtype,), dev)
-    p.slot_indices = _operand(slot_indices, "slot_indices", (slots,), (torch.int32,), dev)
-    p.routing_offsets = _operand(routing_offsets, "routing_offsets", (experts,), (torch.int32,), dev)
-    p.topk_weights = _operand(topk_weights, "topk_weights", (m, top_k), (torch.float32,), dev)
-    if residual is not None:
-        p.residual = _operand(residual, "residual", (m, hidden), (x.dtype,), dev)
-    if smooth_scale is not None:
-        p.smooth = _operand(smooth_scale, "smooth_scale", (1, inner) if smooth_scale.dim() == 2 else (inner,),
-                            (torch.float32,), dev)
     need = get_gated_experts_workspace_bytes(slots, inner, hidden)
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    elif not workspace.is_cuda or workspace.device != dev or workspace.dtype != torch.uint8 or workspace.numel() < need:
-        _fail(f"workspace must be a uint8 tensor on {dev} of at least {need} bytes")
-    p.workspace, p.workspace_bytes = workspace.data_ptr(), workspace.numel()
-    p.type, p.num_tokens, p.top_k, p.num_experts, p.inner, p.hidden = half, m, top_k, experts, inner, hidden
-    p.activation, p.max_val, p.block_size = _activation(activation), max_val, block_size
-    p.host_signal_sync = _sync_word(host_signal_sync)
-    _call_on(dev, "pb2_gated_experts", p, "gated_experts")
+        workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+    elif workspace.get_device() != at or workspace.dtype != torch.uint8 or workspace.numel() < need:
+        _fail(f"workspace must be a uint8 tensor on {x.device} of at least {need} bytes")
+    _call_on(at, "pb2_gated_experts", _PACK_EXPERTS(
+        at, _operand(x, "x", (slots, 2 * inner), (x.dtype,), at), half, m, top_k, experts, inner, hidden,
+        _activation(activation),
+        0 if smooth_scale is None else _operand(
+            smooth_scale, "smooth_scale", (1, inner) if smooth_scale.dim() == 2 else (inner,), _FLOAT, at),
+        max_val, block_size, _operand(w, "w", (experts, hidden, inner), _INT8, at),
+        _operand(w_scales, "w_scales", (experts, hidden), _FLOAT, at),
+        _operand(slot_indices, "slot_indices", (slots,), _INT32, at),
+        _operand(routing_offsets, "routing_offsets", (experts,), _INT32, at),
+        _operand(topk_weights, "topk_weights", (m, top_k), _FLOAT, at),
+        0 if residual is None else _operand(residual, "residual", (m, hidden), (x.dtype,), at),
+        _operand(out, "out", (m, hidden), (x.dtype,), at), workspace.data_ptr(), workspace.numel(),
+        _sync_word(host_signal_sync)), "gated_experts")

@@ -61,18 +61,17 @@ def _device_index(t: torch.Tensor) -> int:
     return t.device.index if t.device.index is not None else torch.cuda.current_device()
 
 
-def _call_on(device: torch.device, name: str, params, op: str) -> None:
-    """Queue a C-ABI call on ``device``'s current stream, with the caller's
-    current device left as it was.  The raw stream handle and no device
-    switch where none is needed: both show in a call of a few microseconds."""
-    index = device.index
-    params.device = index
+def _call_on(index: int, name: str, params: bytes, op: str) -> None:
+    """Queue a C-ABI call (its packed parameters) on the current stream of
+    device ``index``, with the caller's current device left as it was.  The
+    raw stream handle and no device switch where none is needed: both show in
+    a call of a few microseconds."""
     stream = torch._C._cuda_getCurrentRawStream(index)
     if torch.cuda.current_device() == index:
-        status = _lib.function(name)(ctypes.byref(params), stream)
+        status = _lib.function(name)(params, stream)
     else:
         with torch.cuda.device(index):
-            status = _lib.function(name)(ctypes.byref(params), stream)
+            status = _lib.function(name)(params, stream)
     if status:
         _lib.check(status, op)
 

@@ -11,6 +11,7 @@ import torch
 from . import _lib
 from .pearl_gemm_interface import _call_on, _device_index, _fail, _stream
 
+_PACK_GATED = _lib.packer(_lib.GatedQuantParams)
 DEFAULT_HADAMARD_BLOCK_SIZE = 16  # hadamard.py:520
 
 
@@ -80,31 +81,27 @@ def quantize_gated(x, xq, xq_scales, *, activation: str = "silu", row_index=None
     ((M,) int32) row i of the result is row row_index[i] of x -- a MoE
     layer's slots in expert order -- and an index outside x gives a row of
     zeros; without it M = rows."""
-    from .linear import _activation, _half_type, _operand
+    from .linear import _FLOAT, _INT8, _INT32, _activation, _half_type, _operand
 
     if x.dim() != 2 or x.shape[1] % 2:
         _fail("x must be 2D (M, 2 N): gate values, then up values")
     rows, N = x.shape[0], x.shape[1] // 2
-    dev = x.device
+    at = x.get_device()
     half = _half_type(x, "x")
     M = rows if row_index is None else row_index.numel()
-    p = _lib.GatedQuantParams()
-    p.x = _operand(x, "x", (rows, 2 * N), (x.dtype,), dev)
-    p.xq = _operand(xq, "xq", (M, N), (torch.int8,), dev)
-    p.scales = _operand(xq_scales, "xq_scales", (M, 1) if xq_scales.dim() == 2 else (M,), (torch.float32,), dev)
-    if row_index is not None:
-        p.row_index = _operand(row_index, "row_index", (M,), (torch.int32,), dev)
-    if smooth_scale is not None:
-        p.smooth = _operand(smooth_scale, "smooth_scale", (1, N) if smooth_scale.dim() == 2 else (N,),
-                            (torch.float32,), dev)
     if N % 8:
         _fail(f"the row length must be a multiple of 8, got {N}")
     if not 0 < max_val <= 127:
         _fail(f"max_val must be in 1..127, got {max_val}")
     _check_block(block_size, N)
-    p.x_type, p.m, p.n, p.x_rows, p.activation = half, M, N, rows, _activation(activation)
-    p.max_val, p.block_size = max_val, block_size
-    _call_on(dev, "pb2_quantize_gated", p, "quantize_gated")
+    _call_on(at, "pb2_quantize_gated", _PACK_GATED(
+        at, _operand(x, "x", (rows, 2 * N), (x.dtype,), at), half, M, N, rows, _activation(activation),
+        0 if row_index is None else _operand(row_index, "row_index", (M,), _INT32, at),
+        0 if smooth_scale is None else _operand(
+            smooth_scale, "smooth_scale", (1, N) if smooth_scale.dim() == 2 else (N,), _FLOAT, at),
+        _operand(xq, "xq", (M, N), _INT8, at),
+        _operand(xq_scales, "xq_scales", (M, 1) if xq_scales.dim() == 2 else (M,), _FLOAT, at),
+        max_val, block_size), "quantize_gated")
 
 
 def _check_block(block_size: int, n: int) -> None:

@@ -13,6 +13,10 @@ reference's order and with the reference's arguments:
 * ``PearlLinear.apply_weights``: the mining / non-mining branches of
   vllm_kernels.py:154-247.
 
+``PearlLinear.apply_fused`` and ``moe_layer`` go on where the reference hands
+over to vLLM: the linear layer with its bias, activation and residual, and a
+whole MoE layer from router logits to the combined output.
+
 What sits outside the GPU path is passed in rather than fetched: the
 gateway's mining job becomes a ``MiningJob`` value (its hash key, adjusted
 target and seed derivation), and the asynchronous proof submission is left to
@@ -26,10 +30,13 @@ from collections import OrderedDict
 from dataclasses import dataclass, field
 
 import torch
+import torch.nn.functional as F
 
 from . import pearl_gemm_interface as P
 from .helpers import HostSignalHeaderPinnedPool, get_host_signal_sync_fields
-from .moe import build_routing_data, get_build_routing_data_scratchpad_bytes, scatter_rows
+from .linear import _activation, gemm_epilogue
+from .moe import (build_routing_data, gated_experts, gemm_grouped, get_build_routing_data_scratchpad_bytes, route_tokens,
+                  scatter_rows)
 from .moe import noisy_gemm_grouped as grouped_noisy_gemm
 from .quantization import quantize
 
@@ -317,6 +324,32 @@ class PearlLinear:
         return pearl_gemm_vanilla(x_q.contiguous(), w_q.contiguous(), x_s.squeeze(-1),
                                   w_s.reshape(-1), x.dtype, self.config)
 
+    def apply_fused(self, layer, x: torch.Tensor, bias: torch.Tensor | None = None, activation: str = "none",
+                    residual: torch.Tensor | None = None) -> torch.Tensor:
+        """act(x . W^T + bias) + residual for x (m, k) bf16 or fp16: the same
+        quantization and choice of mining as apply_weights, with the rest in
+        the product's epilogue.  A mined product, whose kernel ends at the
+        scales, gets it in elementwise steps behind it."""
+        k, n = x.shape[-1], layer.weight.shape[0]
+        m = x.numel() // k
+        mines = self.mining_enabled and self.job is not None and self.config.should_use_noisy_gemm(m, n, k)
+        if mines and x.dtype is torch.bfloat16:  # the mined product writes bf16
+            _activation(activation)
+            y = self.apply_weights(layer, x).float()
+            y = _ELEMENTWISE[activation](y if bias is None else y + bias.float())
+            return (y if residual is None else y + residual.float()).to(x.dtype)
+        quant = quant_7bit if self.mining_enabled else quant_8bit
+        x_q, x_s, _ = quant(x, smooth_scale=getattr(layer, "smooth_quant_scale", None),
+                            block_size=int(getattr(layer, "hadamard_block_size", NO_HADAMARD_BLOCK_SIZE)))
+        C = torch.empty((m, n), dtype=x.dtype, device=x.device)
+        gemm_epilogue(x_q, layer.weight.contiguous(), x_s.squeeze(-1), layer.weight_scale.reshape(-1), C, bias=bias,
+                      activation=activation, residual=residual)
+        return C
+
+
+_ELEMENTWISE = {"none": lambda y: y, "relu": F.relu, "silu": F.silu, "gelu": F.gelu,
+                "gelu_tanh": lambda y: F.gelu(y, approximate="tanh")}
+
 
 # --------------------------------------------------------------------- MoE --
 @dataclass
@@ -502,3 +535,43 @@ def moe_gemm1(A_q, A_scales, topk_ids, w1, w1_scale, job: MiningJob,
         scatter_rows(C_e, out, layout.slot_indices[start:start + count])
         res.per_expert[e] = MinedGemm(header, sync, ctx.commitment_hash_A, ctx.commitment_hash_B, hits)
     return out, res
+
+
+def moe_layer(x, router_logits, w1, w1_scale, w2, w2_scale, top_k: int, *, job: MiningJob | None = None,
+              config: MiningConfig = MiningConfig(), residual=None, smooth1=None, smooth2=None, activation: str = "silu",
+              **routing):
+    """A MoE layer from its input and its router's logits to its output:
+
+        ids, weights = route_tokens(router_logits)          (**routing: its keyword arguments)
+        h[slot] = x[token] . w1[expert]^T                   mined when there is a job and the layer is large enough
+        out[token] = residual + sum weights * (act(gate) * up of h[slot]) . w2[expert]^T
+
+    x (m, K) bf16 or fp16 (a mined first product needs bf16); w1 (E, 2 I, K)
+    int8 -- int7 where it is mined -- with the gate rows first, w2 (E, K_out,
+    I) int8, scales (E, 2 I) and (E, K_out) float32.  Without a mined product
+    nothing here waits for the device.  Returns (out, MoEGemm1Result or None)."""
+    m, K = x.shape
+    E, N, _ = w1.shape
+    device = x.device
+    ids = torch.empty((m, top_k), dtype=torch.int32, device=device)
+    weights = torch.empty((m, top_k), dtype=torch.float32, device=device)
+    route_tokens(router_logits, weights, ids, **routing)
+    mined = None
+    if job is not None and x.dtype is torch.bfloat16 and config.should_use_noisy_gemm(m, N, K):
+        x_q, x_s, _ = quant_7bit(x, smooth_scale=smooth1)
+        h, mined = moe_gemm1(x_q, x_s, ids, w1, w1_scale, job, config)
+        slot_indices, offsets = mined.ctx.routing_layout.slot_indices, mined.ctx.routing_layout.routing_offsets
+    else:
+        x_q, x_s, _ = quant_8bit(x, smooth_scale=smooth1)
+        slots = m * top_k
+        tokens, slot_indices = (torch.empty(slots, dtype=torch.int32, device=device) for _ in range(2))
+        offsets = torch.empty(E, dtype=torch.int32, device=device)
+        scratch = torch.empty(get_build_routing_data_scratchpad_bytes(slots), dtype=torch.uint8, device=device)
+        build_routing_data(ids, tokens, slot_indices, offsets, scratch, E)
+        h = torch.empty((slots, N), dtype=x.dtype, device=device)
+        gemm_grouped(x_q[tokens], w1, x_s.squeeze(-1)[tokens], w1_scale.reshape(E, N), h, offsets,
+                     c_row_index=slot_indices)
+    out = torch.empty((m, w2.shape[1]), dtype=x.dtype, device=device)
+    gated_experts(h, w2, w2_scale.reshape(E, -1), out, slot_indices, offsets, weights, residual=residual,
+                  smooth_scale=smooth2, activation=activation)
+    return out, mined

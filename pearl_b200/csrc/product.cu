@@ -258,11 +258,11 @@ __device__ __forceinline__ void build_groups(const ProductArgs& a, ProductSmem& 
 // kPair: a tile is worked on by two CTAs (2-SM MMAs, 128 rows of A and half
 // of the tile's rows of B each), else by one.
 //
-// kOnce: for products of few tiles, one tile for each CTA (pair), or for a
-// cluster whose CTAs (pairs) take a.split ranges of its K and add their int32
-// sums up through distributed shared memory, each finishing its share of the
-// columns: the weights are then read through all SMs.  int32 sums are exact,
-// so C does not depend on the split.  Otherwise the grid is persistent and the accumulator double-buffered.
+// kOnce: for products of few tiles, one tile for each cluster, whose CTAs
+// (pairs) take a.split ranges of its K and add their int32 sums up through
+// distributed shared memory, each finishing its share of the columns: the
+// weights are then read through all SMs.  int32 sums are exact, so C does not
+// depend on the split.  Otherwise the grid is persistent and the accumulator double-buffered.
 template <bool kPair, int kTN, bool kGrouped, bool kOnce>
 __global__ void __launch_bounds__(kThreads, kOnce ? 2 : 1) product_kernel(const __grid_constant__ ProductArgs a) {
   constexpr int kCtas = kPair ? 2 : 1;
@@ -617,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, kOnce ? 2 : 1) product_kernel(const 
     const Tile w = has ? tile_at<kGrouped>(a, S, first) : Tile{0, 0, 0, 0};
     const int live = has ? min(max(min(w.rows, a.tile_rows) - int(rank) * kCtaRows, 0), kCtaRows) : 0;
     const bool f16 = a.c_f16;
-    const int width = kTN / split, pieces = width / 8;  // powers of two, at most 32 pieces
+    const int width = kTN / split, pieces = width / 8;  // 64 or 32 columns
     // A thread keeps its piece of eight columns over all its rows.
     const int et = threadIdx.x - 64, step = 32 * kEpiWarps / pieces;
     const int r0 = et / pieces, lc = range * width + (et - r0 * pieces) * 8;
@@ -688,8 +688,7 @@ __global__ void __launch_bounds__(kThreads, kOnce ? 2 : 1) product_kernel(const 
         }
       }
     }
-    if (split > 1) cluster_sync_all();
-    else __syncthreads();
+    cluster_sync_all();
     if (cols_in && !*abort_flag) {
       for (int r = r0; r < live; r += step) {
         const int dst = S.dst[r];
@@ -700,16 +699,12 @@ __global__ void __launch_bounds__(kThreads, kOnce ? 2 : 1) product_kernel(const 
         };
         const uint8_t* p0 = ring + r * kTN * 4 + (((lc / 4) ^ (r & 7)) << 4);
         const uint8_t* p1 = ring + r * kTN * 4 + (((lc / 4 + 1) ^ (r & 7)) << 4);
-        if (split == 1) {
-          add(*reinterpret_cast<const int4*>(p0), *reinterpret_cast<const int4*>(p1));
-        } else {
-          for (int s = 0; s < split; s += 2) {  // split is even: four loads in flight
-            const uint32_t c = s * kCtas + rank;
-            const int4 x0 = ld_cluster_v4(mapa(p0, c)), y0 = ld_cluster_v4(mapa(p1, c));
-            const int4 x1 = ld_cluster_v4(mapa(p0, c + kCtas)), y1 = ld_cluster_v4(mapa(p1, c + kCtas));
-            add(x0, y0);
-            add(x1, y1);
-          }
+        for (int s = 0; s < split; s += 2) {  // split is even: four loads in flight
+          const uint32_t c = s * kCtas + rank;
+          const int4 x0 = ld_cluster_v4(mapa(p0, c)), y0 = ld_cluster_v4(mapa(p1, c));
+          const int4 x1 = ld_cluster_v4(mapa(p0, c + kCtas)), y1 = ld_cluster_v4(mapa(p1, c + kCtas));
+          add(x0, y0);
+          add(x1, y1);
         }
         const uint4 mine = res;
         if (!kGrouped && a.residual) res = load_residual(r + step);
@@ -746,7 +741,7 @@ __global__ void __launch_bounds__(kThreads, kOnce ? 2 : 1) product_kernel(const 
   // barriers, tensor memory or sums.
   tc_fence_before();
   __syncthreads();
-  if (kPair || split > 1) cluster_sync_all();
+  if constexpr (kPair || kOnce) cluster_sync_all();
   tc_fence_after();
   if (warp == 1) {
     __syncwarp();
@@ -809,7 +804,7 @@ int launch_product(ProductArgs& a, const int8_t* A, const int8_t* B, int cta_row
   a.stages = std::min(kMaxStages, ((half ? kHalfSm : 232448) - fixed) / (a.a_bytes + kBRows * kTileK));
   // Whole loads of A in a stage, and with kOnce a tile's sums in the ring.
   if (cta_rows % a.box_rows || cta_rows > kCtaRows || (kPair && cta_rows != kCtaRows) ||
-      (kOnce && cta_rows * kTN * 4 > a.stages * (a.a_bytes + kBRows * kTileK)))
+      (kOnce && (a.split < 2 || cta_rows * kTN * 4 > a.stages * (a.a_bytes + kBRows * kTileK))))
     return PB2_ERR_UNSUPPORTED_CONFIG;
   a.wait_budget = wait_budget_cycles();
   a.wait_hint_ns = suspend_hint_ns(a.wait_budget);
@@ -825,6 +820,7 @@ int launch_product(ProductArgs& a, const int8_t* A, const int8_t* B, int cta_row
   const int64_t tiles_m = kGrouped ? int64_t(a.M) / a.tile_rows + std::min(a.groups, a.M)
                                    : (int64_t(a.M) + a.tile_rows - 1) / a.tile_rows;
   int64_t clusters = tiles_m * a.tiles_n;
+  if (clusters > INT32_MAX / 8) return PB2_ERR_INVALID_ARGUMENT;
   if (!kOnce) {
     const int most = kPair ? resident_pairs(device, reinterpret_cast<const void*>(kern), smem)
                            : std::max(1, sm_count(device));

@@ -71,8 +71,8 @@ PB2_API int pb2_abi_version(void);
  * word of host_signal_sync and unwinds, so a stalled pipeline ends the
  * kernel with a status instead of holding the GPU.
  * pb2_set_wait_budget_cycles sets the budget that later launches of the
- * mined GEMM's main kernel (pb2_noisy_gemm, pb2_gemm) take, for the whole
- * process; cycles <= 0 restores the default (about one second).  Returns the
+ * mined GEMM's main kernel (pb2_noisy_gemm, pb2_gemm) and the un-mined
+ * products (pb2_gemm_epilogue, pb2_gemm_grouped) take, for the whole process; cycles <= 0 restores the default (about one second).  Returns the
  * previous budget.  Launches already queued keep the budget they were
  * given.  The noising kernels always keep the default: their K-split
  * clusters read one another's shared memory until an exit handshake, which a

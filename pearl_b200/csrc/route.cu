@@ -11,6 +11,13 @@
 // bias are taken of the chosen alone, and renormalized softmax weights are a
 // softmax over the chosen, which needs no other exponential.
 //
+// What bounds it is instruction issue, not the logits: 11.4 us for 32768
+// tokens of 128 f32 logits (1.7 TB/s of 6.5).  A warp per token with indices
+// carried through the rounds and all scores computed took 27 us, bare keys
+// 20, no exponentials beside the chosen 16, eight lanes a token 11.4.  4099
+// tokens of 256 experts in 8 groups with a bias: 9.1 us, mostly the latency
+// of one token's chain (sixteen exact sigmoids a lane, four group rounds,
+// eight expert rounds); 4 tokens of 8 experts: 2.1 us.
 #include <algorithm>
 
 #include "pb2_epilogue.cuh"

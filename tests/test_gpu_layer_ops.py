@@ -175,6 +175,30 @@ def test_linear_on_another_stream_and_in_a_graph():
     assert torch.equal(C, D)
 
 
+@pytest.mark.parametrize("m,n,k", [(128, 128, 262144), (600, 512, 131072)])
+def test_linear_wait_budget(m, n, k):
+    """A budget that the epilogue's wait for its sums outlasts ends the kernel
+    with a status, and the next call finds everything as it was."""
+    g = gen(m)
+    A, B = int8(g, m, k), int8(g, n, k)
+    sa, sb = torch.ones(m, device="cuda"), torch.full((n,), 1e-6, device="cuda")
+    C = torch.empty(m, n, dtype=BF16, device="cuda")
+    sync = torch.zeros(pg.get_host_signal_sync_size(), dtype=torch.int8, device="cuda")
+    before = pg.device_waits.set_wait_budget_cycles(64)
+    try:
+        pg.gemm_epilogue(A, B, sa, sb, C, host_signal_sync=sync)
+        torch.cuda.synchronize()
+    finally:
+        pg.device_waits.set_wait_budget_cycles(before)
+    assert pg.get_host_signal_sync_fields(sync)["error"] == pg._lib.PB2_ERR_DEVICE_TIMEOUT
+    sync.zero_()
+    pg.gemm_epilogue(A, B, sa, sb, C, host_signal_sync=sync)
+    torch.cuda.synchronize()
+    assert pg.get_host_signal_sync_fields(sync)["error"] == 0
+    want, slack = linear64(A, B, sa, sb, None, "none", None)
+    within(C, want, slack, BF16)
+
+
 # ------------------------------------------------------------------ router --
 def route(logits, top_k, **kw):
     m = logits.shape[0]

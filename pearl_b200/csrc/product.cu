@@ -28,10 +28,13 @@ namespace {
 
 constexpr int kCtaRows = 128;  // rows of C per CTA
 constexpr int kTileK = 128;     // bytes of K per stage
-constexpr int kEpiWarps = 8;
-constexpr int kThreads = 32 * (2 + kEpiWarps);
+// Epilogue warps: a persistent CTA's 16 hide each other's latency (eight took
+// 5.7 kclocks for a tile of 128 x 256, twice its MMAs at K = 768); where two
+// CTAs share an SM, eight fit.
+constexpr int epi_warps(bool once) { return once ? 8 : 16; }
+constexpr int product_threads(bool once) { return 32 * (2 + epi_warps(once)); }
 constexpr int kMaxStages = 10;
-constexpr int kBoxBytes = 32 * 128;  // an epilogue warp's 32 rows x 64 16-bit columns
+constexpr int kBoxBytes = 32 * 64;  // an epilogue warp's 32 rows x 32 16-bit columns
 constexpr int kMaxGroups = 256;
 
 enum { kBiasNone = 0, kBiasF32 = 1, kBiasHalf = 2 };  // kBiasHalf: C's type
@@ -46,7 +49,7 @@ struct ProductArgs {
   const void* residual;
   int c_f16, bias_kind, act;
   int M, N, K;
-  int tiles_n, raster;
+  int tiles_m, tiles_n;    // of the whole product (tiles_m: without groups)
   int groups;              // 0: one product of M rows
   const int32_t* ends;     // groups: end row of each group
   const int32_t* c_rows;   // optional: row r of the product goes to row c_rows[r] of C
@@ -72,6 +75,7 @@ struct ProductSmem {
   int abort_flag;
   int tile0[kMaxGroups + 1];  // first tile of each group
   int row0[kMaxGroups + 1];   // first row of each group
+  int tiles_m[kMaxGroups];    // row tiles of each group
   float scale[kCtaRows];      // kOnce: the rows' scales and places in C
   int dst[kCtaRows];
 };
@@ -83,30 +87,44 @@ struct Tile {
   int tn;
 };
 
-// Tile t: groups follow one another; inside one, `raster` row tiles walk all
-// column tiles before the next row tiles, so B tiles are read by neighbours.
+// Tile t, asked by a whole warp: groups follow one another; inside one,
+// kRaster row tiles walk all column tiles before the next row tiles, so B
+// tiles are read by neighbours.  Divisions are kept off the common path (a
+// tile of few K blocks is over in 1500 clocks, and so was a binary search
+// with four divisions).
+constexpr int kRaster = 8;
 template <bool kGrouped>
 __device__ __forceinline__ Tile tile_at(const ProductArgs& a, const ProductSmem& S, int t) {
-  int g = 0, first = 0, rows = a.M, lt = t;
+  int g = 0, first = 0, rows = a.M, lt = t, tiles_m = a.tiles_m;
   if constexpr (kGrouped) {
-    int lo = 0, hi = a.groups;  // the last group whose first tile is <= t
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (S.tile0[mid] <= t) lo = mid; else hi = mid;
-    }
-    g = lo;
+    // The last group whose first tile is <= t: by eights, then among eight.
+    const int lane = threadIdx.x % 32;
+    const bool by8 = 8 * lane < a.groups && S.tile0[8 * lane] <= t;
+    const int base = 8 * (__popc(__ballot_sync(0xffffffffu, by8)) - 1);
+    const bool by1 = lane < 8 && base + lane < a.groups && S.tile0[base + lane] <= t;
+    g = base + __popc(__ballot_sync(0xffffffffu, by1)) - 1;
     first = S.row0[g];
     rows = S.row0[g + 1] - first;
     lt = t - S.tile0[g];
+    tiles_m = S.tiles_m[g];
   }
-  const int tiles_m = (rows + a.tile_rows - 1) / a.tile_rows;
-  const int span = min(a.raster, tiles_m);
-  const int block = lt / (span * a.tiles_n);
-  const int m0 = block * span;
-  const int mm = min(span, tiles_m - m0);
-  const int in = lt - block * span * a.tiles_n;
-  const int tm = m0 + in % mm;
-  return Tile{g, first + tm * a.tile_rows, rows - tm * a.tile_rows, in / mm};
+  int m0 = 0, mm = min(kRaster, tiles_m), in = lt;
+  if (in >= mm * a.tiles_n) {
+    const int block = lt / (kRaster * a.tiles_n);
+    m0 = block * kRaster;
+    mm = min(kRaster, tiles_m - m0);
+    in = lt - block * kRaster * a.tiles_n;
+  }
+  int tm = 0, tn = in;
+  if (mm == kRaster) {
+    tn = in / kRaster;
+    tm = in % kRaster;
+  } else if (mm > 1) {
+    tn = in / mm;
+    tm = in - tn * mm;
+  }
+  tm += m0;
+  return Tile{g, first + tm * a.tile_rows, rows - tm * a.tile_rows, tn};
 }
 
 // The producer and the issuer are single threads whose loops bound short-tile
@@ -239,7 +257,9 @@ __device__ __forceinline__ void build_groups(const ProductArgs& a, ProductSmem& 
     for (int i = 0; i < kPer; ++i) {
       end[i] = max(end[i], before);
       tiles[i] = sum;
-      sum += (end[i] - begin + a.tile_rows - 1) / a.tile_rows * a.tiles_n;
+      const int tiles_m = (end[i] - begin + a.tile_rows - 1) / a.tile_rows;
+      if (lane * kPer + i < a.groups) S.tiles_m[lane * kPer + i] = tiles_m;
+      sum += tiles_m * a.tiles_n;
       begin = end[i];
     }
     int total = sum;
@@ -272,11 +292,12 @@ __device__ __forceinline__ void build_groups(const ProductArgs& a, ProductSmem& 
 // weights are then read through all SMs.  int32 sums are exact, so C does not
 // depend on the split.  Otherwise the grid is persistent and the accumulator double-buffered.
 template <bool kPair, int kTN, bool kGrouped, bool kOnce>
-__global__ void __launch_bounds__(kThreads, kOnce ? 2 : 1) product_kernel(const __grid_constant__ ProductArgs a) {
+__global__ void __launch_bounds__(product_threads(kOnce), kOnce ? 2 : 1) product_kernel(const __grid_constant__ ProductArgs a) {
   constexpr int kCtas = kPair ? 2 : 1;
   constexpr int kBRows = kTN / kCtas;  // rows of B this CTA loads
   constexpr int kBBytes = kBRows * kTileK;
-  constexpr int kHalf = kTN / 2;  // columns of an epilogue warp
+  constexpr int kEpiWarps = epi_warps(kOnce);
+  constexpr int kCols = kTN / (kEpiWarps / 4);  // columns of an epilogue warp
   constexpr uint32_t kIdesc = idesc_i8(kCtas * kCtaRows, kTN);
   // An MMA reads kCtaRows rows of A, however few the stage holds (at least
   // eight): the read must end inside the stage.  Pairs always hold them all.
@@ -287,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, kOnce ? 2 : 1) product_kernel(const 
   uint8_t* boxes = ring + a.stages * stage_bytes;
   float2* col_mem = reinterpret_cast<float2*>(boxes + kEpiWarps * kBoxBytes);
   // kOnce needs neither boxes nor column scales in shared memory.
-  ProductSmem& S = *reinterpret_cast<ProductSmem*>(kOnce ? boxes : reinterpret_cast<uint8_t*>(col_mem + kEpiWarps * kHalf));
+  ProductSmem& S = *reinterpret_cast<ProductSmem*>(kOnce ? boxes : reinterpret_cast<uint8_t*>(col_mem + kEpiWarps * kCols));
   constexpr int kTmemCols = kOnce ? kTN : 2 * kTN;
   volatile int* abort_flag = &S.abort_flag;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -332,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, kOnce ? 2 : 1) product_kernel(const 
   if constexpr (kOnce && !kGrouped) {
     // The previous kernel is still running: ask L2 for the first stages of B
     // (a prefetch is coherent with whatever that kernel writes).
-    if (warp == 0 && elect_one()) {
+    if (warp == 0 && lane == 0) {
       const Tile w = tile_at<false>(a, S, first);
       for (int kb = kb0; kb < min(kb1, kb0 + a.stages); ++kb)
         tma_prefetch_l2_2d(&a.tmB, kb * kTileK, w.tn * kTN + int(rank) * kBRows);
@@ -346,19 +367,21 @@ __global__ void __launch_bounds__(kThreads, kOnce ? 2 : 1) product_kernel(const 
   griddep_launch_dependents();
   if constexpr (kGrouped) build_groups(a, S);
   const uint32_t tmem = S.tmem_base;
-  const int tiles = kGrouped ? S.tile0[a.groups] : (a.M + a.tile_rows - 1) / a.tile_rows * a.tiles_n;
+  const int tiles = kGrouped ? S.tile0[a.groups] : a.tiles_m * a.tiles_n;
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
-    if (elect_one()) {
-      bool ok = true;
-      const uint32_t full0 = smem_u32(S.full), empty0 = smem_u32(S.empty), ring0 = smem_u32(ring);
-      const uint32_t past = 8 * a.stages;
-      uint32_t at = 0, dst = ring0, phase = 1;  // of the stage: barrier offset, address, wait parity
-      const int box_bytes = a.box_rows * kTileK;
-      bool early = kGrouped && a.early;
-      for (int t = first; t < tiles && ok; t += stride) {
-        const Tile w = tile_at<kGrouped>(a, S, t);
+    // The warp finds each tile; one thread issues its loads.
+    const bool leader = elect_one();
+    bool ok = true;
+    const uint32_t full0 = smem_u32(S.full), empty0 = smem_u32(S.empty), ring0 = smem_u32(ring);
+    const uint32_t past = 8 * a.stages;
+    uint32_t at = 0, dst = ring0, phase = 1;  // of the stage: barrier offset, address, wait parity
+    const int box_bytes = a.box_rows * kTileK;
+    bool early = kGrouped && a.early;
+    for (int t = first; t < tiles; t += stride) {
+      const Tile w = tile_at<kGrouped>(a, S, t);
+      if (leader && ok) {
         const int arow = w.row0 + int(rank) * kCtaRows;
         const int brow = w.group * a.N + w.tn * kTN + int(rank) * kBRows;
         // Only loads of A with rows of this tile: the rest of the stage keeps
@@ -404,6 +427,9 @@ __global__ void __launch_bounds__(kThreads, kOnce ? 2 : 1) product_kernel(const 
           if (at == past) { at = 0; dst = ring0; phase ^= 1; }
         }
       }
+      __syncwarp();
+    }
+    if (leader) {
       // Every load in flight has landed and been consumed before the CTA ends
       // (bounded).  The next wait of each stage in turn is for just that; on a
       // stage that was never filled it returns at once.
@@ -460,10 +486,10 @@ __global__ void __launch_bounds__(kThreads, kOnce ? 2 : 1) product_kernel(const 
     __syncwarp();
   } else if constexpr (!kOnce) {
     // ------------------------------------------------------------ epilogue
-    // Warp: TMEM lane quadrant q (32 rows), half h of the tile's columns.
+    // Warp: TMEM lane quadrant q (32 rows), strip h of the tile's columns.
     const int q = warp & 3, ew = warp - 2, h = ew >> 2;
     uint8_t* box = boxes + ew * kBoxBytes;
-    float2* cols = col_mem + ew * kHalf;
+    float2* cols = col_mem + ew * kCols;
     const bool f16 = a.c_f16;
     const int q0 = int(rank) * kCtaRows + 32 * q;  // the warp's first row in the tile
     const uint32_t leader_empty = kPair ? mapa(&S.acc_empty[0], lead) : 0;
@@ -480,42 +506,50 @@ __global__ void __launch_bounds__(kThreads, kOnce ? 2 : 1) product_kernel(const 
     // with short K the round trip to memory would otherwise be most of a
     // tile's time.
     struct Meta {
-      Tile w;
+      int tn;
       bool live;  // this warp has something to store
       float rs;
       int dst;
-      float2 col[kHalf / 32];
+      float2 col[kCols / 32];
     };
     auto load_meta = [&](int t) {
       Meta m;
       m.live = false;
+      m.tn = 0;
       m.rs = 0.f;
       m.dst = -1;
 #pragma unroll
-      for (int j = 0; j < kHalf / 32; ++j) m.col[j] = make_float2(0.f, 0.f);
+      for (int j = 0; j < kCols / 32; ++j) m.col[j] = make_float2(0.f, 0.f);
       if (t >= tiles) return m;
-      m.w = tile_at<kGrouped>(a, S, t);
-      const int c0 = m.w.tn * kTN + h * kHalf;
-      const int rows = min(m.w.rows, a.tile_rows);
+      const Tile w = tile_at<kGrouped>(a, S, t);
+      m.tn = w.tn;
+      const int c0 = w.tn * kTN + h * kCols;
+      const int rows = min(w.rows, a.tile_rows);
       m.live = q0 < rows && c0 < a.N;
       if (!m.live) return m;
       if (q0 + lane < rows) {
-        const int r = m.w.row0 + q0 + lane;
+        const int r = w.row0 + q0 + lane;
         m.rs = a.sA[r];
         m.dst = kGrouped && a.c_rows ? a.c_rows[r] : r;
       }
 #pragma unroll
-      for (int j = 0; j < kHalf / 32; ++j) {
+      for (int j = 0; j < kCols / 32; ++j) {
         const int c = c0 + 32 * j + lane;
         if (c < a.N) {
-          m.col[j].x = a.sB[int64_t(m.w.group) * a.N + c];
+          m.col[j].x = a.sB[int64_t(w.group) * a.N + c];
           if (!kGrouped && a.bias_kind)
             m.col[j].y = a.bias_kind == kBiasF32 ? static_cast<const float*>(a.bias)[c] : half_at(a.bias, c, f16);
         }
       }
       return m;
     };
-    const int piece = lane & 7;
+    // Four lanes move one 64-byte row of a 32-column chunk, eight rows an
+    // instruction, so loads of the residual and stores of C are whole sectors.
+    // Rows change hands through the warp's box (16-byte piece j of row r at
+    // j ^ (r / 2 % 4): no bank conflicts either way), into which the residual
+    // is copied asynchronously while the accumulator is still being computed.
+    const int piece = lane & 3, sub = lane >> 2;
+    auto place = [&](int row, int j) { return box + row * 64 + ((j ^ ((row >> 1) & 3)) << 4); };
     bool ok = true;
     int n = 0;
     if (kGrouped && a.early) griddep_wait();
@@ -523,22 +557,20 @@ __global__ void __launch_bounds__(kThreads, kOnce ? 2 : 1) product_kernel(const 
     for (int t = first; t < tiles && ok; t += stride, ++n) {
       const Meta m = next;
       const int slot = n & 1;
-      const int c0 = m.w.tn * kTN + h * kHalf;
-      const int dst = !kGrouped || m.dst < a.c_dst_rows ? m.dst : -1;
-      // Eight lanes move one 128-byte row of a 64-column chunk, so loads of the
-      // residual and stores of C are whole lines.  Rows change hands through
-      // the warp's box (16-byte piece j of row r at j ^ (r & 7): no bank
-      // conflicts either way), into which the residual is copied
-      // asynchronously while the accumulator is still being computed.
-      auto fetch_residual = [&](int ch) {
+      const int c0 = m.tn * kTN + h * kCols;
+      int dst[4];  // the rows of C this lane moves pieces of
+      {
+        const int mine = !kGrouped || m.dst < a.c_dst_rows ? m.dst : -1;
 #pragma unroll
-        for (int it = 0; it < 8; ++it) {
-          const int br = 4 * it + (lane >> 3);
-          const int dr = __shfl_sync(0xffffffffu, dst, br);
-          const int col = c0 + 64 * ch + 8 * piece;
-          if (dr >= 0 && col < a.N) {
-            uint8_t* to = box + br * 128 + ((piece ^ (br & 7)) << 4);
-            const int64_t at = int64_t(dr) * a.N + col;
+        for (int it = 0; it < 4; ++it) dst[it] = __shfl_sync(0xffffffffu, mine, 8 * it + sub);
+      }
+      auto fetch_residual = [&](int ch) {
+        const int col = c0 + 32 * ch + 8 * piece;
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+          if (dst[it] >= 0 && col < a.N) {
+            uint8_t* to = place(8 * it + sub, piece);
+            const int64_t at = int64_t(dst[it]) * a.N + col;
             if (a.vec)
               cp_async16(to, static_cast<const uint16_t*>(a.residual) + at);
             else
@@ -548,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, kOnce ? 2 : 1) product_kernel(const 
       };
       if (m.live) {
 #pragma unroll
-        for (int j = 0; j < kHalf / 32; ++j) cols[32 * j + lane] = m.col[j];
+        for (int j = 0; j < kCols / 32; ++j) cols[32 * j + lane] = m.col[j];
         __syncwarp();
         if (!kGrouped && a.residual) fetch_residual(0);
       }
@@ -556,34 +588,32 @@ __global__ void __launch_bounds__(kThreads, kOnce ? 2 : 1) product_kernel(const 
       if (!(ok = mbar_wait_warp(&S.acc_full[slot], (n >> 1) & 1, abort_flag, a.sync, a.wait_budget, a.wait_hint_ns)))
         break;
       tc_fence_after();
-      const uint32_t taddr = tmem + slot * kTN + (uint32_t(32 * q) << 16) + h * kHalf;
+      const uint32_t taddr = tmem + slot * kTN + (uint32_t(32 * q) << 16) + h * kCols;
       if (!m.live) {
         release(slot);
         continue;
       }
 #pragma unroll 1
-      for (int ch = 0; ch < kHalf / 64; ++ch) {
-        uint32_t v[64];
+      for (int ch = 0; ch < kCols / 32; ++ch) {
+        uint32_t v[32];
         __syncwarp();
-        tmem_ld32(taddr + 64 * ch, v);
-        tmem_ld32(taddr + 64 * ch + 32, v + 32);
-        tmem_wait_ld_into2(v, v + 32);
-        if (ch == kHalf / 64 - 1) release(slot);  // the accumulator is free for the tile after next
-        const float2* cc = cols + 64 * ch;
+        tmem_ld32(taddr + 32 * ch, v);
+        tmem_wait_ld_into(v);
+        if (ch == kCols / 32 - 1) release(slot);  // the accumulator is free for the tile after next
+        const float2* cc = cols + 32 * ch;
         switch (kGrouped ? PB2_ACT_NONE : a.act) {
-          case PB2_ACT_RELU: finish<PB2_ACT_RELU>(v, m.rs, cc); finish<PB2_ACT_RELU>(v + 32, m.rs, cc + 32); break;
-          case PB2_ACT_SILU: finish<PB2_ACT_SILU>(v, m.rs, cc); finish<PB2_ACT_SILU>(v + 32, m.rs, cc + 32); break;
-          case PB2_ACT_GELU: finish<PB2_ACT_GELU>(v, m.rs, cc); finish<PB2_ACT_GELU>(v + 32, m.rs, cc + 32); break;
-          case PB2_ACT_GELU_TANH:
-            finish<PB2_ACT_GELU_TANH>(v, m.rs, cc); finish<PB2_ACT_GELU_TANH>(v + 32, m.rs, cc + 32); break;
-          default: finish<PB2_ACT_NONE>(v, m.rs, cc); finish<PB2_ACT_NONE>(v + 32, m.rs, cc + 32);
+          case PB2_ACT_RELU: finish<PB2_ACT_RELU>(v, m.rs, cc); break;
+          case PB2_ACT_SILU: finish<PB2_ACT_SILU>(v, m.rs, cc); break;
+          case PB2_ACT_GELU: finish<PB2_ACT_GELU>(v, m.rs, cc); break;
+          case PB2_ACT_GELU_TANH: finish<PB2_ACT_GELU_TANH>(v, m.rs, cc); break;
+          default: finish<PB2_ACT_NONE>(v, m.rs, cc);
         }
         if (!kGrouped && a.residual) {
           cp_async_wait();
           __syncwarp();
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const uint4 r = *reinterpret_cast<const uint4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4));
+          for (int j = 0; j < 4; ++j) {
+            const uint4 r = *reinterpret_cast<const uint4*>(place(lane, j));
             const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
             for (int p = 0; p < 4; ++p) {
@@ -595,24 +625,25 @@ __global__ void __launch_bounds__(kThreads, kOnce ? 2 : 1) product_kernel(const 
           __syncwarp();
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < 4; ++j) {
           uint32_t o[4];
 #pragma unroll
           for (int p = 0; p < 4; ++p)
             o[p] = pack_half2(__uint_as_float(v[8 * j + 2 * p]), __uint_as_float(v[8 * j + 2 * p + 1]), f16);
-          *reinterpret_cast<uint4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(place(lane, j)) = make_uint4(o[0], o[1], o[2], o[3]);
         }
         __syncwarp();
+        uint4 out[4];
 #pragma unroll
-        for (int it = 0; it < 8; ++it) {
-          const int br = 4 * it + (lane >> 3);
-          const int dr = __shfl_sync(0xffffffffu, dst, br);
-          const int col = c0 + 64 * ch + 8 * piece;
-          const uint4 val = *reinterpret_cast<const uint4*>(box + br * 128 + ((piece ^ (br & 7)) << 4));
-          if (dr >= 0 && col < a.N) store8(a, int64_t(dr) * a.N + col, a.N - col, val);
+        for (int it = 0; it < 4; ++it) out[it] = *reinterpret_cast<const uint4*>(place(8 * it + sub, piece));
+        const int col = c0 + 32 * ch + 8 * piece;
+        if (col < a.N) {
+#pragma unroll
+          for (int it = 0; it < 4; ++it)
+            if (dst[it] >= 0) store8(a, int64_t(dst[it]) * a.N + col, a.N - col, out[it]);
         }
         __syncwarp();
-        if (!kGrouped && a.residual && ch + 1 < kHalf / 64) fetch_residual(ch + 1);
+        if (!kGrouped && a.residual && ch + 1 < kCols / 32) fetch_residual(ch + 1);
       }
     }
   }
@@ -681,17 +712,17 @@ __global__ void __launch_bounds__(kThreads, kOnce ? 2 : 1) product_kernel(const 
       tc_fence_after();
       if (ok && 32 * q < live) {
 #pragma unroll 1
-        for (int ch = 0; ch < kHalf / 32; ++ch) {
+        for (int ch = 0; ch < kCols / 32; ++ch) {
           uint32_t v[32];
           __syncwarp();
-          tmem_ld32(tmem + (uint32_t(32 * q) << 16) + h * kHalf + 32 * ch, v);
+          tmem_ld32(tmem + (uint32_t(32 * q) << 16) + h * kCols + 32 * ch, v);
           tmem_wait_ld_into(v);
           const int r = 32 * q + lane;
           if (r < live) {
             uint4* row = reinterpret_cast<uint4*>(ring + r * kTN * 4);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-              row[(h * (kHalf / 4) + 8 * ch + j) ^ (r & 7)] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+              row[(h * (kCols / 4) + 8 * ch + j) ^ (r & 7)] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
           }
         }
       }
@@ -768,7 +799,7 @@ int resident_pairs(int device, const void* kern, int smem) {
   if (n == 0) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2, 1, 1);
-    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.blockDim = dim3(product_threads(false), 1, 1);
     cfg.dynamicSmemBytes = size_t(smem);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -791,7 +822,7 @@ int resident_pairs(int device, const void* kern, int smem) {
 // ranges, so that the set-up of one product overlaps the end of the one before
 // it (1 x 4096 x 4096 in ranges of 8 blocks 6.7 us, 7.0 with a full ring;
 // 64 x 4096 x 14336 in ranges of 28 blocks 18.6, 16.4 with a full ring).
-constexpr int kHalfSm = 115712;
+constexpr int kColsSm = 115712;
 
 template <bool kPair, int kTN, bool kGrouped, bool kOnce>
 int launch_product(ProductArgs& a, const int8_t* A, const int8_t* B, int cta_rows, int device, cudaStream_t s) {
@@ -799,17 +830,17 @@ int launch_product(ProductArgs& a, const int8_t* A, const int8_t* B, int cta_row
   constexpr int kBRows = kTN / kCtas;
   a.a_bytes = cta_rows * kTileK;
   a.tile_rows = kCtas * cta_rows;
+  a.tiles_m = int((int64_t(a.M) + a.tile_rows - 1) / a.tile_rows);
   a.tiles_n = (a.N + kTN - 1) / kTN;
-  a.raster = 8;
   int st;
   if ((st = make_tmap_2d(&a.tmA, A, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, a.M, kTileK, a.box_rows,
                          CU_TENSOR_MAP_SWIZZLE_128B)) ||
       (st = make_tmap_2d(&a.tmB, B, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, uint64_t(std::max(a.groups, 1)) * a.N, kTileK,
                          kBRows, CU_TENSOR_MAP_SWIZZLE_128B)))
     return st;
-  const int fixed = 1024 + int(sizeof(ProductSmem)) + (kOnce ? 0 : kEpiWarps * (kBoxBytes + kTN / 2 * 8));
+  const int fixed = 1024 + int(sizeof(ProductSmem)) + (kOnce ? 0 : epi_warps(false) * kBoxBytes + 4 * kTN * 8);
   const bool half = kOnce && (a.K + kTileK - 1) / kTileK <= 8 * a.split;
-  a.stages = std::min(kMaxStages, ((half ? kHalfSm : 232448) - fixed) / (a.a_bytes + kBRows * kTileK));
+  a.stages = std::min(kMaxStages, ((half ? kColsSm : 232448) - fixed) / (a.a_bytes + kBRows * kTileK));
   // Whole loads of A in a stage, and with kOnce a tile's sums in the ring.
   if (cta_rows % a.box_rows || cta_rows > kCtaRows || (kPair && cta_rows != kCtaRows) ||
       (kOnce && (a.split < 2 || cta_rows * kTN * 4 > a.stages * (a.a_bytes + kBRows * kTileK))))
@@ -835,7 +866,7 @@ int launch_product(ProductArgs& a, const int8_t* A, const int8_t* B, int cta_row
     clusters = std::min<int64_t>(clusters, most);
   }
   const int cluster = kCtas * (kOnce ? a.split : 1);
-  return launch_programmatic(kern, dim3(unsigned(clusters * cluster)), kThreads, smem, s, cluster, a);
+  return launch_programmatic(kern, dim3(unsigned(clusters * cluster)), product_threads(kOnce), smem, s, cluster, a);
 }
 
 // The variant for a product is the one with the smallest estimate of its

@@ -569,8 +569,8 @@ PB2_API int pb2_quantize_gated(const pb2_gated_quant_params* p, void* stream);
  *   C[row] = A_scales[row] * B_scales[e] * (A[row] . B[e]^T),
  * written to row c_row_index[row] of C's c_rows rows when the index is given
  * (rows outside are skipped).  Rows past the last expert's end are not
- * written.  num_experts <= 256; types, alignment and host_signal_sync as for
- * pb2_gemm_epilogue. */
+ * written.  num_experts <= 256; C of
+ * f32, bf16 or f16; alignment and host_signal_sync as for pb2_gemm_epilogue. */
 typedef struct pb2_gemm_grouped_params {
   int device;
   int64_t m, n, k;
@@ -593,7 +593,8 @@ PB2_API int pb2_gemm_grouped(const pb2_gemm_grouped_params* p, void* stream);
  * slot of weight 0 holds does not count.  residual may be out. */
 typedef struct pb2_combine_params {
   int device;
-  const void* slots;         /* (num_tokens * top_k, n) of type */
+  const void* slots;         /* (num_tokens * top_k, n) of slots_type */
+  int slots_type;            /* type or PB2_TYPE_F32 */
   const float* topk_weights; /* (num_tokens, top_k) */
   const void* residual;      /* (num_tokens, n), optional */
   void* out;                 /* (num_tokens, n) */
@@ -606,8 +607,8 @@ PB2_API int pb2_combine_slots(const pb2_combine_params* p, void* stream);
  * quantize_gated of x (slots = num_tokens * top_k rows in slot order) into
  * expert order (slot_indices), gemm_grouped with w back to slot order,
  * combine_slots.  workspace: pb2_gated_experts_workspace_bytes(slots, inner,
- * hidden) bytes, 16-byte aligned.  The slots' products are rounded to `type`
- * between the last two steps. */
+ * hidden) bytes, 16-byte aligned.  Between the last two steps the slots'
+ * products are f32 where they fit in 32 MB, else rounded to `type`. */
 typedef struct pb2_gated_experts_params {
   int device;
   const void* x; /* (slots, 2 inner) of type */

@@ -166,7 +166,8 @@ class GemmGroupedParams(ctypes.Structure):
 
 
 class CombineParams(ctypes.Structure):
-    _fields_ = [("device", ctypes.c_int), ("slots", _vp), ("topk_weights", _vp), ("residual", _vp), ("out", _vp),
+    _fields_ = [("device", ctypes.c_int), ("slots", _vp), ("slots_type", ctypes.c_int), ("topk_weights", _vp),
+                ("residual", _vp), ("out", _vp),
                 ("type", ctypes.c_int), ("num_tokens", _i64), ("top_k", _i64), ("n", _i64)]
 
 

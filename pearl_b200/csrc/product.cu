@@ -47,7 +47,7 @@ struct ProductArgs {
   void* C;
   const void* bias;
   const void* residual;
-  int c_f16, bias_kind, act;
+  int c_f16, c_f32, bias_kind, act;  // C: bf16, f16 or, of groups only, f32
   int M, N, K;
   int tiles_m, tiles_n;    // of the whole product (tiles_m: without groups)
   int groups;              // 0: one product of M rows
@@ -226,6 +226,18 @@ __device__ __forceinline__ void store8(const ProductArgs& a, int64_t at, int lef
 #pragma unroll
   for (int j = 0; j < 8; ++j)
     if (j < left) out[j] = uint16_t(w[j / 2] >> (16 * (j & 1)));
+}
+// Four f32 elements.
+__device__ __forceinline__ void store4(const ProductArgs& a, int64_t at, int left, uint4 val) {
+  uint32_t* out = static_cast<uint32_t*>(a.C) + at;
+  if (a.vec) {
+    *reinterpret_cast<uint4*>(out) = val;
+    return;
+  }
+  const uint32_t w[4] = {val.x, val.y, val.z, val.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (j < left) out[j] = w[j];
 }
 
 // Group boundaries to shared memory: row0 and tile0 (exclusive prefix of the
@@ -624,6 +636,24 @@ __global__ void __launch_bounds__(product_threads(kOnce), kOnce ? 2 : 1) product
           }
           __syncwarp();
         }
+        if (kGrouped && a.c_f32) {
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {  // 16 columns are a box's 64-byte rows
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              *reinterpret_cast<uint4*>(place(lane, j)) =
+                  make_uint4(v[16 * part + 4 * j], v[16 * part + 4 * j + 1], v[16 * part + 4 * j + 2], v[16 * part + 4 * j + 3]);
+            __syncwarp();
+            const int col = c0 + 32 * ch + 16 * part + 4 * piece;
+#pragma unroll
+            for (int it = 0; it < 4; ++it) {
+              const uint4 val = *reinterpret_cast<const uint4*>(place(8 * it + sub, piece));
+              if (dst[it] >= 0 && col < a.N) store4(a, int64_t(dst[it]) * a.N + col, a.N - col, val);
+            }
+            __syncwarp();
+          }
+          continue;
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           uint32_t o[4];
@@ -769,6 +799,15 @@ __global__ void __launch_bounds__(product_threads(kOnce), kOnce ? 2 : 1) product
               f[2 * j + 1] += g.y;
             }
           }
+        }
+        if (kGrouped && a.c_f32) {
+#pragma unroll
+          for (int j = 0; j < 8; j += 4)
+            if (col + j < a.N)
+              store4(a, int64_t(dst) * a.N + col + j, a.N - col - j,
+                     make_uint4(__float_as_uint(f[j]), __float_as_uint(f[j + 1]), __float_as_uint(f[j + 2]),
+                                __float_as_uint(f[j + 3])));
+          continue;
         }
         store8(a, int64_t(dst) * a.N + col, a.N - col,
                make_uint4(pack_half2(f[0], f[1], f16), pack_half2(f[2], f[3], f16), pack_half2(f[4], f[5], f16),
@@ -957,25 +996,42 @@ struct CombineArgs {
   int top_k, n, f16, vec;
 };
 constexpr int kCombineBatch = 4;
+// Eight columns of a slot.
+struct Eight {
+  uint4 lo, hi;  // hi: of f32 slots
+};
 
+template <bool kSlotF32>
 __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
   griddep_wait();
   griddep_launch_dependents();
   const int64_t t = blockIdx.x;
   const int col = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
   if (col >= a.n) return;
+  const int left = a.n - col;
   const bool f16 = a.f16;
-  auto load = [&](const void* base, int64_t row) {
-    const uint16_t* p = static_cast<const uint16_t*>(base) + row * a.n + col;
-    if (a.vec) return *reinterpret_cast<const uint4*>(p);
-    uint32_t w[4] = {0u, 0u, 0u, 0u};
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  auto load_slot = [&](int64_t row) {
+    Eight e;
+    if constexpr (kSlotF32) {
+      const uint32_t* p = static_cast<const uint32_t*>(a.slots) + row * a.n + col;
+      if (a.vec) {
+        e.lo = *reinterpret_cast<const uint4*>(p);
+        e.hi = *reinterpret_cast<const uint4*>(p + 4);
+      } else {
+        uint32_t w[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (col + j < a.n) w[j / 2] |= uint32_t(p[j]) << (16 * (j & 1));
-    return make_uint4(w[0], w[1], w[2], w[3]);
+        for (int j = 0; j < 8; ++j) w[j] = j < left ? p[j] : 0u;
+        e.lo = make_uint4(w[0], w[1], w[2], w[3]);
+        e.hi = make_uint4(w[4], w[5], w[6], w[7]);
+      }
+    } else {
+      e.lo = load8(a.slots, a.vec, row * a.n + col, left);
+    }
+    return e;
   };
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  auto add = [&](uint4 r, float w) {
+  auto add16 = [&](uint4 r, float w) {
     const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -984,22 +1040,30 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
       acc[2 * j + 1] = fmaf(w, f.y, acc[2 * j + 1]);
     }
   };
-  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-  const uint4 res = a.residual ? load(a.residual, t) : zero;
+  auto add = [&](const Eight& e, float w) {
+    if constexpr (kSlotF32) {
+      const uint32_t x[8] = {e.lo.x, e.lo.y, e.lo.z, e.lo.w, e.hi.x, e.hi.y, e.hi.z, e.hi.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] = fmaf(w, __uint_as_float(x[j]), acc[j]);
+    } else {
+      add16(e.lo, w);
+    }
+  };
+  const uint4 res = a.residual ? load8(a.residual, a.vec, t * a.n + col, left) : zero;
   for (int j0 = 0; j0 < a.top_k; j0 += kCombineBatch) {
-    uint4 r[kCombineBatch];
+    Eight r[kCombineBatch];
     float w[kCombineBatch];
 #pragma unroll
     for (int j = 0; j < kCombineBatch; ++j) {
       const bool in = j0 + j < a.top_k;
-      r[j] = in ? load(a.slots, t * a.top_k + j0 + j) : zero;
+      if (in) r[j] = load_slot(t * a.top_k + j0 + j);
       w[j] = in ? a.weights[t * a.top_k + j0 + j] : 0.f;
     }
 #pragma unroll
     for (int j = 0; j < kCombineBatch; ++j)
       if (w[j] != 0.f) add(r[j], w[j]);  // whatever a slot without weight holds does not count
   }
-  if (a.residual) add(res, 1.0f);
+  if (a.residual) add16(res, 1.0f);
   uint16_t* o = static_cast<uint16_t*>(a.out) + t * a.n + col;
   if (a.vec) {
     *reinterpret_cast<uint4*>(o) = make_uint4(pack_half2(acc[0], acc[1], f16), pack_half2(acc[2], acc[3], f16),
@@ -1007,9 +1071,17 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (col + j < a.n) o[j] = half_bits(acc[j], f16);
+      if (j < left) o[j] = half_bits(acc[j], f16);
   }
 }
+
+// The type gated_experts keeps the slots' products in between its product and
+// its combination: f32 while they stay in L2 beside what else passes through
+// it, else the output's 16 bits, whose rounding then is as large as the
+// output's own (the error against 64 bits 1.4 times that of one rounding; f32
+// would double the 134 MB each way of 16384 slots of 4096).
+constexpr int64_t kSlotF32Bytes = 32 << 20;
+bool slots_f32(int64_t slots, int64_t hidden) { return slots * hidden * 4 <= kSlotF32Bytes; }
 
 bool type16(int t) { return t == PB2_TYPE_BF16 || t == PB2_TYPE_F16; }
 
@@ -1055,7 +1127,7 @@ namespace pb2 {
 int gemm_grouped(const pb2_gemm_grouped_params& p, bool early, cudaStream_t stream) {
   if (p.m < 0 || p.n <= 0 || p.k <= 0 || p.m > INT32_MAX || p.k > INT32_MAX) return PB2_ERR_INVALID_ARGUMENT;
   if (p.num_experts <= 0 || p.num_experts > kMaxGroups || p.n > INT32_MAX / p.num_experts) return PB2_ERR_INVALID_ARGUMENT;
-  if (!type16(p.c_type)) return PB2_ERR_INVALID_ARGUMENT;
+  if (!type16(p.c_type) && p.c_type != PB2_TYPE_F32) return PB2_ERR_INVALID_ARGUMENT;
   if (p.k % 16 != 0) return PB2_ERR_UNSUPPORTED_CONFIG;
   if (p.c_row_index && p.c_rows < 0) return PB2_ERR_INVALID_ARGUMENT;
   if (p.m > 0 && (!p.A || !p.B || !p.A_scales || !p.B_scales || !p.C || !p.routing_offsets || !al16(p.A) || !al16(p.B)))
@@ -1069,6 +1141,7 @@ int gemm_grouped(const pb2_gemm_grouped_params& p, bool early, cudaStream_t stre
   a.sB = p.B_scales;
   a.C = p.C;
   a.c_f16 = p.c_type == PB2_TYPE_F16;
+  a.c_f32 = p.c_type == PB2_TYPE_F32;
   a.M = int(p.m);
   a.N = int(p.n);
   a.K = int(p.k);
@@ -1096,7 +1169,7 @@ extern "C" int pb2_combine_slots(const pb2_combine_params* pp, void* stream) {
   const pb2_combine_params& p = *pp;
   if (p.num_tokens < 0 || p.top_k <= 0 || p.n <= 0 || p.num_tokens > INT32_MAX || p.top_k > INT32_MAX || p.n > INT32_MAX)
     return PB2_ERR_INVALID_ARGUMENT;
-  if (!type16(p.type)) return PB2_ERR_INVALID_ARGUMENT;
+  if (!type16(p.type) || (p.slots_type != p.type && p.slots_type != PB2_TYPE_F32)) return PB2_ERR_INVALID_ARGUMENT;
   if (p.num_tokens > 0 && (!p.slots || !p.topk_weights || !p.out)) return PB2_ERR_INVALID_ARGUMENT;
   const int64_t vectors = (p.n + 7) / 8, threads = std::min<int64_t>(256, (vectors + 31) / 32 * 32);
   const int64_t across = (vectors + threads - 1) / threads;
@@ -1113,14 +1186,16 @@ extern "C" int pb2_combine_slots(const pb2_combine_params* pp, void* stream) {
   a.n = int(p.n);
   a.f16 = p.type == PB2_TYPE_F16;
   a.vec = p.n % 8 == 0 && al16(p.slots) && al16(p.out) && al16(p.residual);
-  return launch_programmatic(combine_kernel, dim3(unsigned(p.num_tokens), unsigned(across)), int(threads), 0,
-                             static_cast<cudaStream_t>(stream), 1, a);
+  const dim3 grid(unsigned(p.num_tokens), static_cast<unsigned>(across));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (p.slots_type == PB2_TYPE_F32) return launch_programmatic(combine_kernel<true>, grid, int(threads), 0, s, 1, a);
+  return launch_programmatic(combine_kernel<false>, grid, int(threads), 0, s, 1, a);
 }
 
 extern "C" int64_t pb2_gated_experts_workspace_bytes(int64_t slots, int64_t inner, int64_t hidden) {
   if (slots <= 0 || inner <= 0 || hidden <= 0) return 0;
   auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
-  return up(slots * inner) + up(slots * 4) + up(slots * hidden * 2);
+  return up(slots * inner) + up(slots * 4) + up(slots * hidden * (pb2::slots_f32(slots, hidden) ? 4 : 2));
 }
 
 extern "C" int pb2_gated_experts(const pb2_gated_experts_params* pp, void* stream) {
@@ -1162,7 +1237,7 @@ extern "C" int pb2_gated_experts(const pb2_gated_experts_params* pp, void* strea
   g.A_scales = q.scales;
   g.B_scales = p.w_scales;
   g.C = ws + up(slots * p.inner) + up(slots * 4);
-  g.c_type = p.type;
+  g.c_type = slots_f32(slots, p.hidden) ? PB2_TYPE_F32 : p.type;
   g.num_experts = p.num_experts;
   g.routing_offsets = p.routing_offsets;
   g.c_row_index = p.slot_indices;
@@ -1172,6 +1247,7 @@ extern "C" int pb2_gated_experts(const pb2_gated_experts_params* pp, void* strea
   std::memset(&c, 0, sizeof(c));
   c.device = p.device;
   c.slots = g.C;
+  c.slots_type = g.c_type;
   c.topk_weights = p.topk_weights;
   c.residual = p.residual;
   c.out = p.out;

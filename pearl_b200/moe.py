@@ -245,7 +245,7 @@ def gemm_grouped(A, B, A_scales, B_scales, C, routing_offsets, *, c_row_index=No
     (build_routing_data's, read on the device: no host copy of the counts),
     against ``B`` (E, n, k) int8; A_scales (m,), B_scales (E, n) float32;
 
-        C[i] = A_scales[i] * B_scales[e] * (A[i] . B[e]^T)   (bf16 or fp16)
+        C[i] = A_scales[i] * B_scales[e] * (A[i] . B[e]^T)   (float32, bf16 or fp16)
 
     With ``c_row_index`` ((m,) int32, e.g. slot_indices) row i goes to row
     c_row_index[i] of C instead; rows outside C are skipped.  Rows past the
@@ -259,12 +259,11 @@ def gemm_grouped(A, B, A_scales, B_scales, C, routing_offsets, *, c_row_index=No
         _fail(f"k must be a multiple of 16, got {k}")
     if not 1 <= experts <= MAX_EXPERTS:
         _fail(f"num_experts must be in 1..{MAX_EXPERTS}, got {experts}")
-    half = _half_type(C, "C")
     rows = m if c_row_index is None else C.shape[0]
     _call_on(at, "pb2_gemm_grouped", _PACK_GROUPED(
         at, m, n, k, _operand(A, "A", (m, k), _INT8, at), _operand(B, "B", (experts, n, k), _INT8, at),
         _operand(A_scales, "A_scales", (m,), _FLOAT, at), _operand(B_scales, "B_scales", (experts, n), _FLOAT, at),
-        _operand(C, "C", (rows, n), (C.dtype,), at), half, experts,
+        _operand(C, "C", (rows, n), tuple(_TYPES), at), _TYPES[C.dtype], experts,
         _operand(routing_offsets, "routing_offsets", (experts,), _INT32, at),
         0 if c_row_index is None else _operand(c_row_index, "c_row_index", (m,), _INT32, at), rows,
         _sync_word(host_signal_sync)), "gemm_grouped")
@@ -273,8 +272,8 @@ def gemm_grouped(A, B, A_scales, B_scales, C, routing_offsets, *, c_row_index=No
 def combine_slots(slots, topk_weights, out, *, residual=None) -> None:
     """out[t] = residual[t] + sum_j topk_weights[t, j] * slots[t * top_k + j]:
     the token's experts added up in float32 in the order of j, rounded once.
-    slots (m * top_k, n), out and ``residual`` (m, n), all bf16 or all fp16;
-    topk_weights (m, top_k) float32.  What a slot of weight 0 holds does
+    slots (m * top_k, n), out and ``residual`` (m, n), all bf16 or all fp16, or
+    the slots float32; topk_weights (m, top_k) float32.  What a slot of weight 0 holds does
     not count; ``residual`` may be out itself."""
     if topk_weights.dim() != 2 or out.dim() != 2:
         _fail("topk_weights and out must be 2D (m, top_k) and (m, n)")
@@ -283,7 +282,7 @@ def combine_slots(slots, topk_weights, out, *, residual=None) -> None:
     at = out.get_device()
     half = _half_type(out, "out")
     _call_on(at, "pb2_combine_slots", _PACK_COMBINE(
-        at, _operand(slots, "slots", (m * top_k, n), (out.dtype,), at),
+        at, _operand(slots, "slots", (m * top_k, n), (out.dtype, torch.float32), at), _TYPES[slots.dtype],
         _operand(topk_weights, "topk_weights", (m, top_k), _FLOAT, at),
         0 if residual is None else _operand(residual, "residual", (m, n), (out.dtype,), at),
         _operand(out, "out", (m, n), (out.dtype,), at), half, m, top_k, n), "combine_slots")
@@ -306,8 +305,8 @@ def gated_experts(x, w, w_scales, out, slot_indices, routing_offsets, topk_weigh
     top_k) route_tokens'.  x, out and ``residual`` are all bf16 or all fp16;
     ``smooth_scale`` (1, inner) or (inner,) float32.  ``workspace`` (uint8,
     get_gated_experts_workspace_bytes) is taken from torch's allocator when
-    not given.  The slots' products are rounded to out's type before they are
-    added up."""
+    not given.  Before they are added up the slots' products are float32 where
+    they fit in 32 MB, else rounded to out's type."""
     if w.dim() != 3 or topk_weights.dim() != 2:
         _fail("w must be 3-D (num_experts, hidden, inner) and topk_weights 2D (m, top_k)")
     experts, hidden, inner = w.shape

@@ -17,7 +17,8 @@ import pearl_b200 as pg
 pytestmark = pytest.mark.gpu
 
 ACC = 2.0 ** -20
-HALF_ULP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}  # 8 and 11 significant bits
+# 8, 11 and 24 significant bits
+HALF_ULP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 
 
@@ -363,7 +364,8 @@ COUNTS = [[1], [0, 1, 0], [5, 0, 3], [0, 0, 130, 7, 0], [128, 128], [129, 1, 255
 
 
 @pytest.mark.parametrize("counts", COUNTS, ids=lambda c: f"{len(c)}x{sum(c)}")
-@pytest.mark.parametrize("n,k,dtype", [(8, 16, BF16), (264, 144, F16), (129, 272, BF16), (1000, 1360, F16)])
+@pytest.mark.parametrize("n,k,dtype", [(8, 16, BF16), (264, 144, F16), (129, 272, BF16), (1000, 1360, F16), (200, 400, F32),
+                                       (131, 96, F32)])
 def test_gemm_grouped(counts, n, k, dtype):
     g = gen(sum(counts) * 31 + n)
     E, m = len(counts), sum(counts)
@@ -400,10 +402,11 @@ def test_gemm_grouped_rows_past_the_last_expert_stay():
 
 @pytest.mark.parametrize("m,k,n", [(1, 1, 8), (1, 2, 4096), (5, 3, 17), (33, 8, 264), (7, 32, 1001)])
 @pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("slots_f32", [False, True])
 @pytest.mark.parametrize("residual", [False, True])
-def test_combine_slots(m, k, n, dtype, residual):
+def test_combine_slots(m, k, n, dtype, slots_f32, residual):
     g = gen(m + k + n)
-    y = randn(g, m * k, n).to(dtype)
+    y = randn(g, m * k, n).to(F32 if slots_f32 else dtype)
     w = torch.rand(m, k, generator=g, device="cuda")
     if k > 1:
         w[m // 2, 0] = 0
@@ -423,7 +426,8 @@ def test_combine_slots(m, k, n, dtype, residual):
 
 @pytest.mark.parametrize("m,E,k,hidden,inner,dtype", [
     (1, 4, 1, 64, 32, BF16), (1, 8, 2, 4096, 1024, BF16), (3, 60, 4, 2040, 1360, F16), (40, 16, 8, 136, 272, F16),
-    (300, 8, 2, 1000, 528, BF16), (700, 4, 3, 264, 2048, BF16)])
+    (300, 8, 2, 1000, 528, BF16), (700, 4, 3, 264, 2048, BF16),
+    (1500, 8, 6, 1024, 64, F16)])
 @pytest.mark.parametrize("residual,smooth", [(False, False), (True, True)])
 def test_gated_experts_is_its_three_steps(m, E, k, hidden, inner, dtype, residual, smooth):
     g = gen(m + hidden)
@@ -440,7 +444,8 @@ def test_gated_experts_is_its_three_steps(m, E, k, hidden, inner, dtype, residua
     pg.moe.gated_experts(x, W, ws, out, slot, ends, w, residual=r, smooth_scale=s)
     q, sc = torch.empty(slots, inner, dtype=torch.int8, device="cuda"), torch.empty(slots, device="cuda")
     pg.quantization.quantize_gated(x, q, sc, row_index=slot, smooth_scale=s)
-    y = torch.empty(slots, hidden, dtype=dtype, device="cuda")
+    kept = F32 if slots * hidden * 4 <= 32 << 20 else dtype
+    y = torch.empty(slots, hidden, dtype=kept, device="cuda")
     pg.moe.gemm_grouped(q, W, sc, ws, y, ends, c_row_index=slot)
     want = torch.empty_like(out)
     pg.moe.combine_slots(y, w, want, residual=r)
@@ -453,8 +458,8 @@ def test_gated_experts_is_its_three_steps(m, E, k, hidden, inner, dtype, residua
     total, mag = terms.sum(1), terms.abs().sum(1)
     if residual:
         total, mag = total + r.double(), mag + r.double().abs()
-    # each slot's product is rounded to the type before the sum
-    within(out, total, mag * (HALF_ULP[dtype] * 1.01 + 2.0 ** -19) + k * 2.0 ** -25, dtype)
+    # each slot's product is rounded to the kept type before the sum
+    within(out, total, mag * (HALF_ULP[kept] * 1.01 + 2.0 ** -19) + k * 2.0 ** -25, dtype)
 
 
 @pytest.mark.parametrize("m,E,k,hidden,inner", [(8, 8, 2, 4096, 2048), (2, 8, 2, 512, 4096), (900, 64, 4, 512, 768), (1500, 4, 2, 1024, 512)])
@@ -479,7 +484,7 @@ def test_gated_experts_back_to_back(m, E, k, hidden, inner):
     torch.cuda.synchronize()
     for src, out in zip(xs, outs):
         q, sc = torch.empty(slots, inner, dtype=torch.int8, device="cuda"), torch.empty(slots, device="cuda")
-        y, want = torch.empty(slots, hidden, dtype=BF16, device="cuda"), torch.empty_like(out)
+        y, want = torch.empty(slots, hidden, dtype=F32, device="cuda"), torch.empty_like(out)
         for step in (lambda: pg.quantization.quantize_gated(src, q, sc, row_index=slot),
                      lambda: pg.moe.gemm_grouped(q, W, sc, ws, y, ends, c_row_index=slot),
                      lambda: pg.moe.combine_slots(y, w, want)):

@@ -28,7 +28,7 @@ ROUTE = dict(logits=P, logits_type=0, num_tokens=4, num_experts=8, top_k=2, scor
 LINEAR = dict(m=4, n=8, k=32, A=P, B=P, A_scales=P, B_scales=P, C=P, c_type=1)
 GATED = dict(x=P, x_type=1, m=4, n=8, x_rows=4, xq=P, scales=P, max_val=127)
 GROUPED = dict(m=4, n=8, k=32, A=P, B=P, A_scales=P, B_scales=P, C=P, c_type=1, num_experts=2, routing_offsets=P)
-COMBINE = dict(slots=P, topk_weights=P, out=P, type=1, num_tokens=4, top_k=2, n=8)
+COMBINE = dict(slots=P, slots_type=1, topk_weights=P, out=P, type=1, num_tokens=4, top_k=2, n=8)
 EXPERTS = dict(x=P, type=1, num_tokens=4, top_k=2, num_experts=2, inner=16, hidden=8, max_val=127, w=P, w_scales=P,
                slot_indices=P, routing_offsets=P, topk_weights=P, out=P, workspace=P, workspace_bytes=1 << 20)
 
@@ -50,11 +50,11 @@ EXPERTS = dict(x=P, type=1, num_tokens=4, top_k=2, num_experts=2, inner=16, hidd
     *[("pb2_quantize_gated", _lib.GatedQuantParams, GATED, c, UNSUPPORTED) for c in (
         dict(n=12), dict(block_size=4), dict(block_size=16), dict(n=24, block_size=24), dict(n=512, block_size=512))],
     *[("pb2_gemm_grouped", _lib.GemmGroupedParams, GROUPED, c, BAD) for c in (
-        dict(m=-1), dict(n=0), dict(num_experts=0), dict(num_experts=257), dict(n=1 << 30, num_experts=4), dict(c_type=0),
+        dict(m=-1), dict(n=0), dict(num_experts=0), dict(num_experts=257), dict(n=1 << 30, num_experts=4), dict(c_type=3), dict(c_type=-1),
         dict(routing_offsets=None), dict(A=None), dict(B=P + 4), dict(c_row_index=P, c_rows=-1))],
     ("pb2_gemm_grouped", _lib.GemmGroupedParams, GROUPED, dict(k=40), UNSUPPORTED),
     *[("pb2_combine_slots", _lib.CombineParams, COMBINE, c, BAD) for c in (
-        dict(num_tokens=-1), dict(top_k=0), dict(n=0), dict(type=0), dict(slots=None), dict(topk_weights=None), dict(out=None))],
+        dict(num_tokens=-1), dict(top_k=0), dict(n=0), dict(type=0), dict(slots_type=2), dict(slots=None), dict(topk_weights=None), dict(out=None))],
     *[("pb2_gated_experts", _lib.GatedExpertsParams, EXPERTS, c, BAD) for c in (
         dict(num_tokens=-1), dict(top_k=0), dict(num_experts=0), dict(num_experts=257), dict(inner=0), dict(hidden=0), dict(type=0),
         dict(x=None), dict(w=None), dict(w=P + 8), dict(w_scales=None), dict(slot_indices=None), dict(routing_offsets=None),
@@ -71,7 +71,9 @@ def test_c_abi_refuses(entry, cls, good, change, status):
 def test_workspace_bytes():
     f = pg.moe.get_gated_experts_workspace_bytes
     assert f(0, 16, 8) == 0 and f(-1, 16, 8) == 0
-    assert f(2, 16, 8) == 3 * 256
+    assert f(2, 16, 8) == 3 * 256  # each part in whole 256 bytes
+    assert f(1024, 512, 8192) == 1024 * 512 + 1024 * 4 + 1024 * 8192 * 4  # 32 MB of f32 products
+    assert f(1025, 512, 8192) == 1025 * 512 + 17 * 256 + 1025 * 8192 * 2
     assert f(16384, 14336, 4096) == 16384 * 14336 + 16384 * 4 + 16384 * 4096 * 2
     assert f(1 << 20, 1 << 14, 1 << 13) == (1 << 34) + (1 << 22) + (1 << 34)
 

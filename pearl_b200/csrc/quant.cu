@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) quant_rows_reg_kern
 // rounding pass: x is read once and the activation computed once.  Rows of at
 // most 1024 products take a warp each (no block barrier), longer ones a block
 // of just the threads they need.  16384 rows of 14336: 211 us (5.6 TB/s of
-// 6.5; with expf and a division 345); 16384 of 768: 14.5 us (4.3 TB/s; a
+// 6.5; with expf and a division 345); 16384 of 768: 12.6 us (5.0 TB/s; a
 // block per row 25).
 struct GatedArgs {
   QuantArgs q;
@@ -295,7 +295,8 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : kGatedThreads, kWarpRow ? 4 :
     }
 #pragma unroll
     for (int it = 0; it < kGatedIters; ++it)
-      gated_vec<T, kAct>(a, it * threads + me, it * threads + me < nvec, g[it], u[it], v[it]);
+      if (!kWarpRow || it * threads < nvec)  // short rows: no work on vectors that no lane has
+        gated_vec<T, kAct>(a, it * threads + me, it * threads + me < nvec, g[it], u[it], v[it]);
   }
   auto again = [&](int it) {  // the products of one vector, without kKeep
     const int vec = it * threads + me;
@@ -304,6 +305,7 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : kGatedThreads, kWarpRow ? 4 :
   };
 #pragma unroll
   for (int it = 0; it < iters; ++it) {
+    if (kWarpRow && it * threads >= nvec) break;
     if constexpr (!kKeep) again(it);
 #pragma unroll
     for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[kKeep ? it : 0][i]));

@@ -5,7 +5,7 @@
 // the device.
 //
 // A TMA thread fills a ring of 128-byte K stages, a thread issues the tcgen05
-// int8 MMAs, and eight epilogue warps turn accumulators into C: the grid is
+// int8 MMAs, and the epilogue warps turn accumulators into C: the grid is
 // persistent and the accumulator double-buffered in tensor memory, or, for
 // few tiles, each tile's K is split over a cluster (kOnce below).  int32 sums
 // are exact; the epilogue works in f32 and rounds once.

@@ -16,7 +16,7 @@
 // 1.32 GHz and 990 W; its MMAs alone 248 and 285, its loads alone 240.  Few
 // rows: the weights' bytes (16 slots over 8 experts of 4096 x 14336: 63.5 us,
 // 6.5 TB/s).  Few rows and few weights: start, join and end, about 5 us
-// (1 x 4096 x 4096: 6.4 us of which the weights are 2.6).
+// (1 x 4096 x 4096: 5.8 us of which the weights are 2.6).
 #include <algorithm>
 #include <atomic>
 #include <cstring>
@@ -38,6 +38,11 @@ constexpr int kBoxBytes = 32 * 64;  // an epilogue warp's 32 rows x 32 16-bit co
 constexpr int kMaxGroups = 256;
 
 enum { kBiasNone = 0, kBiasF32 = 1, kBiasHalf = 2 };  // kBiasHalf: C's type
+
+// Shared memory for the sums a CTA receives from the other split - 1 ranges.
+__host__ __device__ constexpr int received_bytes(int rows, int tile_columns, int split) {
+  return rows * tile_columns * 4 / split * (split - 1);
+}
 
 struct ProductArgs {
   CUtensorMap tmA;  // A (rows, K) int8, boxes of box_rows rows
@@ -71,6 +76,7 @@ struct ProductSmem {
   uint64_t acc_full[2];
   uint64_t acc_empty[2];
   uint64_t drain;
+  uint64_t join;  // kOnce: the other K ranges' sums have arrived
   uint32_t tmem_base;
   int abort_flag;
   int tile0[kMaxGroups + 1];  // first tile of each group
@@ -201,6 +207,15 @@ __device__ __forceinline__ void cp_async16(void* to, const void* from) {
 }
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
+// `bytes` of this CTA's shared memory to the same place as `to` in the CTA of
+// cluster rank `peer`, counted on its barrier `bar`.
+__device__ __forceinline__ void copy_to_peer(const void* to, const void* from, uint32_t bytes, const uint64_t* bar, uint32_t peer) {
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   mapa(to, peer)),
+               "r"(smem_u32(from)), "r"(bytes), "r"(mapa(bar, peer))
+               : "memory");
+}
+
 template <int kAct>
 __device__ __forceinline__ void activate8(float* f) {
 #pragma unroll
@@ -320,8 +335,10 @@ __global__ void __launch_bounds__(product_threads(kOnce), kOnce ? 2 : 1) product
   const int stage_bytes = a.a_bytes + kBBytes;
   uint8_t* boxes = ring + a.stages * stage_bytes;
   float2* col_mem = reinterpret_cast<float2*>(boxes + kEpiWarps * kBoxBytes);
-  // kOnce needs neither boxes nor column scales in shared memory.
-  ProductSmem& S = *reinterpret_cast<ProductSmem*>(kOnce ? boxes : reinterpret_cast<uint8_t*>(col_mem + kEpiWarps * kCols));
+  // kOnce has neither boxes nor column scales, but the sums it receives.
+  uint8_t* received = boxes;
+  ProductSmem& S = *reinterpret_cast<ProductSmem*>(kOnce ? received + received_bytes(a.a_bytes / kTileK, kTN, a.split)
+                                                         : reinterpret_cast<uint8_t*>(col_mem + kEpiWarps * kCols));
   constexpr int kTmemCols = kOnce ? kTN : 2 * kTN;
   volatile int* abort_flag = &S.abort_flag;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -342,6 +359,7 @@ __global__ void __launch_bounds__(product_threads(kOnce), kOnce ? 2 : 1) product
       mbar_init(&S.acc_empty[i], kCtas * kEpiWarps);
     }
     mbar_init(&S.drain, 1);
+    mbar_init(&S.join, 1);
     S.abort_flag = 0;
     fence_barrier_init();
     tma_prefetch(&a.tmA);
@@ -358,7 +376,9 @@ __global__ void __launch_bounds__(product_threads(kOnce), kOnce ? 2 : 1) product
   }
   tc_fence_before();
   __syncthreads();
-  if constexpr (kPair) cluster_sync_all();  // both CTAs' barriers exist before a remote arrive or 2-SM load
+  // Every CTA of the cluster runs, its barriers set up, before a remote
+  // arrive, copy or 2-SM load.
+  if constexpr (kPair || kOnce) cluster_sync_all();
   tc_fence_after();
   const int kblocks = (a.K + kTileK - 1) / kTileK;
   const int range = kOnce ? int(crank) / kCtas : 0;
@@ -680,9 +700,13 @@ __global__ void __launch_bounds__(product_threads(kOnce), kOnce ? 2 : 1) product
   }
   if constexpr (kOnce) {
     // ------------------------------------------------------------ join of the K ranges
-    // Each CTA's accumulator goes to its own ring (idle by now) as rows of
-    // kTN int32, 16-byte piece j of row r at j ^ (r & 7); then every CTA
-    // adds up its columns over the ranges, a thread eight of them.
+    // A CTA finishes kTN / split of the tile's columns.  Its accumulator goes
+    // to its own ring (idle by now) as [finisher][row][columns] int32, 16-byte
+    // piece j of a row at j ^ (row & 7); one bulk copy a finisher takes its
+    // share over, and the sums are local when the copies have arrived.  (With
+    // a remote load per row, range and piece instead: 32 x 4096 x 4096 6.1 |
+    // 6.9 us, 128 x 4096 x 14336 16.4 | 17.9, in pairs 256 x 4096 x 14336
+    // 18.6 | 18.3, whose ring then has two stages more.)
     const bool has = first < tiles;
     const Tile w = has ? tile_at<kGrouped>(a, S, first) : Tile{0, 0, 0, 0};
     const int live = has ? min(max(min(w.rows, a.tile_rows) - int(rank) * kCtaRows, 0), kCtaRows) : 0;
@@ -690,6 +714,8 @@ __global__ void __launch_bounds__(product_threads(kOnce), kOnce ? 2 : 1) product
     const int width = kTN / split, pieces = width / 8;  // 64 or 32 columns
     // A thread keeps its piece of eight columns over all its rows.
     const int et = threadIdx.x - 64, step = 32 * kEpiWarps / pieces;
+    const int rows = a.a_bytes / kTileK;      // of a CTA's tile
+    const uint32_t share = live * width * 4;  // bytes of a finisher's columns from one range
     const int r0 = et / pieces, lc = range * width + (et - r0 * pieces) * 8;
     const int col = w.tn * kTN + lc;
     const bool cols_in = et >= 0 && has && col < a.N;
@@ -736,6 +762,7 @@ __global__ void __launch_bounds__(product_threads(kOnce), kOnce ? 2 : 1) product
           }
         }
       }
+      if (et == 0 && live > 0) mbar_arrive_expect_tx(&S.join, (split - 1) * share);
       named_barrier_sync(1, 32 * kEpiWarps);  // S.scale and S.dst are in
       if (!kGrouped && a.residual) res = load_residual(r0);
       const int q = warp & 3, h = (warp - 2) >> 2;
@@ -750,32 +777,43 @@ __global__ void __launch_bounds__(product_threads(kOnce), kOnce ? 2 : 1) product
           tmem_wait_ld_into(v);
           const int r = 32 * q + lane;
           if (r < live) {
-            uint4* row = reinterpret_cast<uint4*>(ring + r * kTN * 4);
+            const int c = h * kCols + 32 * ch, owner = c / width;  // width >= 32: a chunk has one finisher
+            const int j0 = (c - owner * width) / 4;
+            uint4* row = reinterpret_cast<uint4*>(ring + (owner * rows + r) * width * 4);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-              row[(h * (kCols / 4) + 8 * ch + j) ^ (r & 7)] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+              row[(j0 + j) ^ (r & 7)] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
           }
+        }
+        fence_proxy_async_smem();
+      }
+      named_barrier_sync(1, 32 * kEpiWarps);
+      if (live > 0 && !__any_sync(0xffffffffu, *abort_flag)) {
+        if (et < split && et != range)  // the finisher keeps the other ranges' sums in their order
+          copy_to_peer(received + (range - int(range > et)) * rows * width * 4, ring + et * rows * width * 4, share, &S.join,
+                       et * kCtas + rank);
+        mbar_wait_warp(&S.join, 0, abort_flag, a.sync, a.wait_budget, a.wait_hint_ns);
+      }
+      if (et == 0 && live > 0 && *abort_flag) {  // given up: no copy may still be on its way when the CTA ends (bounded)
+        const long long t0 = clock64();
+        while (!mbar_test(&S.join, 0) && clock64() - t0 < 100000000LL) {
         }
       }
     }
-    cluster_sync_all();
     if (cols_in && !*abort_flag) {
+      const int p4 = (lc - range * width) / 4;
       for (int r = r0; r < live; r += step) {
         const int dst = S.dst[r];
         int acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        auto add = [&](int4 x, int4 y) {
+        auto add = [&](const uint8_t* sums) {
+          const uint8_t* row = sums + r * width * 4;
+          const int4 x = *reinterpret_cast<const int4*>(row + ((p4 ^ (r & 7)) << 4));
+          const int4 y = *reinterpret_cast<const int4*>(row + (((p4 + 1) ^ (r & 7)) << 4));
           acc[0] += x.x; acc[1] += x.y; acc[2] += x.z; acc[3] += x.w;
           acc[4] += y.x; acc[5] += y.y; acc[6] += y.z; acc[7] += y.w;
         };
-        const uint8_t* p0 = ring + r * kTN * 4 + (((lc / 4) ^ (r & 7)) << 4);
-        const uint8_t* p1 = ring + r * kTN * 4 + (((lc / 4 + 1) ^ (r & 7)) << 4);
-        for (int s = 0; s < split; s += 2) {  // split is even: four loads in flight
-          const uint32_t c = s * kCtas + rank;
-          const int4 x0 = ld_cluster_v4(mapa(p0, c)), y0 = ld_cluster_v4(mapa(p1, c));
-          const int4 x1 = ld_cluster_v4(mapa(p0, c + kCtas)), y1 = ld_cluster_v4(mapa(p1, c + kCtas));
-          add(x0, y0);
-          add(x1, y1);
-        }
+        add(ring + range * rows * width * 4);
+        for (int s = 0; s + 1 < split; ++s) add(received + s * rows * width * 4);
         const uint4 mine = res;
         if (!kGrouped && a.residual) res = load_residual(r + step);
         if (dst < 0) continue;
@@ -861,7 +899,9 @@ int resident_pairs(int device, const void* kern, int smem) {
 // Shared memory of a CTA that leaves room for another on its SM: for short K
 // ranges, so that the set-up of one product overlaps the end of the one before
 // it (1 x 4096 x 4096 in ranges of 8 blocks 6.7 us, 7.0 with a full ring;
-// 64 x 4096 x 14336 in ranges of 28 blocks 18.6, 16.4 with a full ring).
+// 64 x 4096 x 14336 in ranges of 28 blocks 18.6, 16.4 with a full ring: taken
+// when sums were still loaded from their CTAs).  Tiles of more than 32 rows
+// leave such a ring too few stages beside the sums they receive.
 constexpr int kColsSm = 115712;
 
 template <bool kPair, int kTN, bool kGrouped, bool kOnce>
@@ -878,12 +918,14 @@ int launch_product(ProductArgs& a, const int8_t* A, const int8_t* B, int cta_row
       (st = make_tmap_2d(&a.tmB, B, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, uint64_t(std::max(a.groups, 1)) * a.N, kTileK,
                          kBRows, CU_TENSOR_MAP_SWIZZLE_128B)))
     return st;
-  const int fixed = 1024 + int(sizeof(ProductSmem)) + (kOnce ? 0 : epi_warps(false) * kBoxBytes + 4 * kTN * 8);
-  const bool half = kOnce && (a.K + kTileK - 1) / kTileK <= 8 * a.split;
+  const int fixed = 1024 + int(sizeof(ProductSmem)) +
+                    (kOnce ? received_bytes(cta_rows, kTN, a.split) : epi_warps(false) * kBoxBytes + 4 * kTN * 8);
+  const bool half = kOnce && cta_rows <= 32 && (a.K + kTileK - 1) / kTileK <= 8 * a.split;
   a.stages = std::min(kMaxStages, ((half ? kColsSm : 232448) - fixed) / (a.a_bytes + kBRows * kTileK));
   // Whole loads of A in a stage, and with kOnce a tile's sums in the ring.
   if (cta_rows % a.box_rows || cta_rows > kCtaRows || (kPair && cta_rows != kCtaRows) ||
-      (kOnce && (a.split < 2 || cta_rows * kTN * 4 > a.stages * (a.a_bytes + kBRows * kTileK))))
+      (kOnce && (a.split < 2 || kTN % a.split || kTN / a.split < 32 ||
+                 cta_rows * kTN * 4 > a.stages * (a.a_bytes + kBRows * kTileK))))
     return PB2_ERR_UNSUPPORTED_CONFIG;
   a.wait_budget = wait_budget_cycles();
   a.wait_hint_ns = suspend_hint_ns(a.wait_budget);
@@ -930,8 +972,8 @@ int run_linear(ProductArgs& a, const int8_t* A, const int8_t* B, int device, cud
   const double single = 4.5 + 0.25 * double(ceil_div(ceil_div(m, 128) * ceil_div(n, 128), sms) * kblocks);
   // One tile a cluster, K split over it as far as the SMs, a cluster of four
   // CTAs (of eight, most have to wait for a second round) and kMinRange K
-  // blocks a range allow.  (1 x 4096 x 4096: 6.5, unsplit 10.7;
-  // 256 x 4096 x 14336: 22 in pairs, unsplit 27.)
+  // blocks a range allow.  (1 x 4096 x 4096: 5.8, unsplit 10.7;
+  // 256 x 4096 x 14336: 21 in pairs, unsplit 27.)
   constexpr int kMinRange = 4;
   auto split_of = [&](int64_t tiles, int ctas) {
     int split = 1;

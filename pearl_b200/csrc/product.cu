@@ -16,7 +16,7 @@
 // 1.32 GHz and 990 W; its MMAs alone 248 and 285, its loads alone 240.  Few
 // rows: the weights' bytes (16 slots over 8 experts of 4096 x 14336: 63.5 us,
 // 6.5 TB/s).  Few rows and few weights: start, join and end, about 5 us
-// (1 x 4096 x 4096: 5.8 us of which the weights are 2.6).
+// (1 x 4096 x 4096: 6.3 us of which the weights are 2.6).
 #include <algorithm>
 #include <atomic>
 #include <cstring>
@@ -953,46 +953,56 @@ int launch_product(ProductArgs& a, const int8_t* A, const int8_t* B, int cta_row
 
 // The variant for a product is the one with the smallest estimate of its
 // time, in us: a start and end, and for each K block of a CTA's tiles what a
-// stage of that tile takes.  Fitted to products of 1 to 2048 rows, 2048 to
-// 14336 columns and 1040 to 14336 of K, whose measured times it meets within
-// about 15% and whose order it keeps; the measured pairs beside the rules
-// are us.
+// stage of that tile takes.  Fitted to products of 1 to 2048 rows, 300 to
+// 14336 columns and 304 to 16384 of K with weights from HBM; the variant it
+// takes was within 3% of the fastest for all 37 of them.
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 int run_linear(ProductArgs& a, const int8_t* A, const int8_t* B, int device, cudaStream_t s) {
-  const int64_t sms = std::max(1, sm_count(device)), pairs = sms / 2;
+  const int64_t sms = std::max(1, sm_count(device)), pairs = std::max<int64_t>(1, sms / 2);
   const int64_t kblocks = ceil_div(a.K, kTileK), m = a.M, n = a.N;
-  const int cta_rows = int(std::min<int64_t>(kCtaRows, ceil_div(m, 8) * 8));
-  a.box_rows = cta_rows;
-  // Persistent: 256 x 256 tiles of CTA pairs, 256 x 128 of pairs, 128 x 128.
-  // (1024 x 4096 x 4096: 18.7 | 19.5 | 20.7; 512 x 4096 x 14336: 41 | 28 | 32;
-  // 777 x 2048 x 2048: 11 | 8.8 | 8.2.)
-  const double wide = 8.0 + 0.33 * double(ceil_div(ceil_div(m, 256) * ceil_div(n, 256), pairs) * kblocks);
-  const double pair = 6.0 + 0.20 * double(ceil_div(ceil_div(m, 256) * ceil_div(n, 128), pairs) * kblocks);
-  const double single = 4.5 + 0.25 * double(ceil_div(ceil_div(m, 128) * ceil_div(n, 128), sms) * kblocks);
-  // One tile a cluster, K split over it as far as the SMs, a cluster of four
-  // CTAs (of eight, most have to wait for a second round) and kMinRange K
-  // blocks a range allow.  (1 x 4096 x 4096: 5.8, unsplit 10.7;
-  // 256 x 4096 x 14336: 21 in pairs, unsplit 27.)
-  constexpr int kMinRange = 4;
-  auto split_of = [&](int64_t tiles, int ctas) {
-    int split = 1;
-    while (2 * split * ctas <= 4 && tiles * ctas * 2 * split <= sms && kblocks / (2 * split) >= kMinRange) split *= 2;
-    return split;
+  enum { kWide, kPairs, kSingle } kind = kSingle;
+  double best = 1e30;
+  int cta_rows = kCtaRows;
+  auto offer = [&](double us, int k, int rows, int split) {
+    if (us >= best) return;
+    best = us;
+    kind = static_cast<decltype(kind)>(k);
+    cta_rows = rows;
+    a.split = split;
   };
-  const int split1 = split_of(ceil_div(m, 128) * ceil_div(n, 128), 1), split2 = split_of(ceil_div(m, 256) * ceil_div(n, 128), 2);
-  const double join = 5.0 + 0.035 * double(std::min<int64_t>(m, 128)), never = 1e30;
-  const double once1 = split1 > 1 ? join + 0.25 * double(ceil_div(kblocks, split1)) : never;
-  const double once2 = split2 > 1 && m > kCtaRows ? join + 0.20 * double(ceil_div(kblocks, split2)) : never;
-  const double best = std::min({m > kCtaRows ? std::min(wide, pair) : never, single, once1, once2});
-  if (best == once1 || best == once2) {
-    a.split = best == once1 ? split1 : split2;
-    if (best == once1) return launch_product<false, 128, false, true>(a, A, B, cta_rows, device, s);
-    return launch_product<true, 128, false, true>(a, A, B, cta_rows, device, s);
+  // Persistent pairs with tiles of 256 x 256 and 256 x 128 (1024 x 4096 x
+  // 4096: 18.7 | 19.5, single CTAs 20.7; 512 x 4096 x 14336: 41 | 28 | 32), or
+  // with 256 x 128 and K in two ranges (256 x 4096 x 14336: 19, unsplit 27,
+  // single CTAs with two ranges 21).
+  if (m > kCtaRows) {
+    offer(7.0 + 0.33 * double(ceil_div(ceil_div(m, 256) * ceil_div(n, 256), pairs) * kblocks), kWide, kCtaRows, 1);
+    const int64_t tiles = ceil_div(m, 256) * ceil_div(n, 128);
+    offer(5.0 + 0.20 * double(ceil_div(tiles, pairs) * kblocks), kPairs, kCtaRows, 1);
+    if (tiles * 2 <= pairs && kblocks >= 4) offer(7.5 + 0.20 * double(ceil_div(kblocks, 2)), kPairs, kCtaRows, 2);
   }
-  a.split = 1;
-  if (best == single) return launch_product<false, 128, false, false>(a, A, B, cta_rows, device, s);
-  if (best == pair) return launch_product<true, 128, false, false>(a, A, B, cta_rows, device, s);
+  // Single CTAs.  Tiles of fewer rows start and end sooner and occupy more
+  // SMs (200 x 2048 x 2048: 7.0 with 32 rows, 8.0 with 128; 200 x 1001 x 1040,
+  // whose odd rows are stored in pieces: 7.4 | 14.5).  K is split over a
+  // cluster of two or four CTAs (of eight, most have to wait for a second
+  // round) while every one has an SM (1 x 4096 x 4096: 6.3, unsplit 10.7;
+  // 100 x 1000 x 1008 with 32 rows: 5.0 | 5.5; 128 x 300 x 16384: 10.9 | 29).
+  for (int rows = 32; rows <= kCtaRows; rows *= 2) {
+    const int r = int(std::min<int64_t>(rows, ceil_div(m, 8) * 8));
+    const int64_t tiles = ceil_div(m, r) * ceil_div(n, 128);
+    const double block = 0.176 + 0.0005 * r;
+    offer(3.85 + 0.002 * r + block * double(ceil_div(tiles, sms) * kblocks), kSingle, r, 1);
+    for (int split = 2; split <= 4 && tiles * split <= sms && kblocks >= 2 * split; split *= 2)
+      offer(3.2 + 0.024 * r + 0.0056 * double(tiles * split) + block * double(ceil_div(kblocks, split)), kSingle, r, split);
+    if (r >= m) break;
+  }
+  a.box_rows = cta_rows;
+  if (a.split > 1) {
+    if (kind == kPairs) return launch_product<true, 128, false, true>(a, A, B, cta_rows, device, s);
+    return launch_product<false, 128, false, true>(a, A, B, cta_rows, device, s);
+  }
+  if (kind == kSingle) return launch_product<false, 128, false, false>(a, A, B, cta_rows, device, s);
+  if (kind == kPairs) return launch_product<true, 128, false, false>(a, A, B, cta_rows, device, s);
   return launch_product<true, 256, false, false>(a, A, B, cta_rows, device, s);
 }
 

@@ -89,6 +89,17 @@ def test_linear_sizes(m, n, k, dtype):
     linear_case(m, n, k, dtype, "silu", dtype, True)
 
 
+# Row tiles of 32, 64 and 128 rows, whole and ragged, K in one, two and four
+# ranges of even and uneven length, also in pairs.
+@pytest.mark.parametrize("m,n,k", [
+    (32, 4096, 1040), (40, 1024, 1040), (64, 1023, 14336), (65, 512, 1280), (97, 1000, 1008), (100, 768, 4112),
+    (128, 300, 16384), (129, 1024, 8208), (160, 4096, 8192), (200, 2048, 2048), (300, 304, 304), (333, 2048, 1040),
+    (500, 512, 512), (256, 4096, 4224)])
+@pytest.mark.parametrize("act,residual", [("none", False), ("gelu", True)])
+def test_linear_row_tiles(m, n, k, act, residual):
+    linear_case(m, n, k, BF16, act, torch.float32, residual)
+
+
 @pytest.mark.parametrize("act", list(pg.linear.ACTIVATIONS))
 @pytest.mark.parametrize("bias", [None, F32, BF16])
 @pytest.mark.parametrize("residual", [False, True])

@@ -608,7 +608,8 @@ PB2_API int pb2_combine_slots(const pb2_combine_params* p, void* stream);
  * expert order (slot_indices), gemm_grouped with w back to slot order,
  * combine_slots.  workspace: pb2_gated_experts_workspace_bytes(slots, inner,
  * hidden) bytes, 16-byte aligned.  Between the last two steps the slots'
- * products are f32 where they fit in 32 MB, else rounded to `type`. */
+ * products are f32 where they fit in 32 MB, else rounded to `type`.  Slots
+ * past the last expert's end (an id outside the experts) add nothing. */
 typedef struct pb2_gated_experts_params {
   int device;
   const void* x; /* (slots, 2 inner) of type */

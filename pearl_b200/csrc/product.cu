@@ -64,6 +64,7 @@ struct ProductArgs {
   int stages;
   int split;               // K ranges, one per CTA (pair) of the cluster
   int early;               // only A and sA come from the kernel before this one (see the start of the kernel)
+  int zero_rest;           // groups: rows past the last group's end are zeros in C, not left as they are
   int vec;                 // rows of C and residual can be moved 16 bytes at a time
   SignalSync* sync;
   long long wait_budget;
@@ -854,6 +855,23 @@ __global__ void __launch_bounds__(product_threads(kOnce), kOnce ? 2 : 1) product
       }
     }
   }
+  if constexpr (kGrouped) {
+    // Rows of no group (their expert is on another GPU): zeros, 16 bytes a
+    // thread where rows allow it.
+    for (int r = (a.zero_rest ? S.row0[a.groups] : a.M) + int(blockIdx.x); r < a.M; r += int(gridDim.x)) {
+      const int dst = a.c_rows ? a.c_rows[r] : r;
+      if (uint32_t(dst) >= uint32_t(a.c_dst_rows)) continue;
+      const int size = a.c_f32 ? 4 : 2;
+      uint8_t* row = static_cast<uint8_t*>(a.C) + int64_t(dst) * a.N * size;
+      if (a.vec) {
+        for (int64_t i = 16 * threadIdx.x; i < int64_t(a.N) * size; i += 16 * blockDim.x)
+          *reinterpret_cast<uint4*>(row + i) = make_uint4(0u, 0u, 0u, 0u);
+      } else {
+        for (int64_t i = 2 * threadIdx.x; i < int64_t(a.N) * size; i += 2 * blockDim.x)
+          *reinterpret_cast<uint16_t*>(row + i) = 0;
+      }
+    }
+  }
   // No CTA leaves while another of its cluster can still address its
   // barriers, tensor memory or sums.
   tc_fence_before();
@@ -1176,8 +1194,8 @@ extern "C" int pb2_gemm_epilogue(const pb2_gemm_epilogue_params* pp, void* strea
 }
 
 namespace pb2 {
-// `early`: see ProductArgs.
-int gemm_grouped(const pb2_gemm_grouped_params& p, bool early, cudaStream_t stream) {
+// `early`, `zero_rest`: see ProductArgs.
+int gemm_grouped(const pb2_gemm_grouped_params& p, bool early, bool zero_rest, cudaStream_t stream) {
   if (p.m < 0 || p.n <= 0 || p.k <= 0 || p.m > INT32_MAX || p.k > INT32_MAX) return PB2_ERR_INVALID_ARGUMENT;
   if (p.num_experts <= 0 || p.num_experts > kMaxGroups || p.n > INT32_MAX / p.num_experts) return PB2_ERR_INVALID_ARGUMENT;
   if (!type16(p.c_type) && p.c_type != PB2_TYPE_F32) return PB2_ERR_INVALID_ARGUMENT;
@@ -1205,6 +1223,7 @@ int gemm_grouped(const pb2_gemm_grouped_params& p, bool early, cudaStream_t stre
   a.vec = p.n % 8 == 0 && al16(p.C) && al16(p.B_scales);
   a.sync = static_cast<SignalSync*>(p.host_signal_sync);
   a.early = early;
+  a.zero_rest = zero_rest;
   return run_grouped(a, p.A, p.B, p.device, stream);
 }
 }  // namespace pb2
@@ -1212,7 +1231,7 @@ int gemm_grouped(const pb2_gemm_grouped_params& p, bool early, cudaStream_t stre
 extern "C" int pb2_gemm_grouped(const pb2_gemm_grouped_params* pp, void* stream) {
   pb2::NvtxRange nvtx_range("pb2_gemm_grouped");
   if (!pp) return PB2_ERR_INVALID_ARGUMENT;
-  return pb2::gemm_grouped(*pp, false, static_cast<cudaStream_t>(stream));
+  return pb2::gemm_grouped(*pp, false, false, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int pb2_combine_slots(const pb2_combine_params* pp, void* stream) {
@@ -1314,8 +1333,9 @@ extern "C" int pb2_gated_experts(const pb2_gated_experts_params* pp, void* strea
     return PB2_ERR_INVALID_ARGUMENT;
   if (p.inner % 16 != 0) return PB2_ERR_UNSUPPORTED_CONFIG;
   int st = pb2_quantize_gated(&q, stream);
-  // The quantizer writes A and its scales; weights and routing are older.
-  if (!st) st = gemm_grouped(g, true, static_cast<cudaStream_t>(stream));
+  // The quantizer writes A and its scales; weights and routing are older.  The
+  // combination reads every slot, also those of no expert.
+  if (!st) st = gemm_grouped(g, true, true, static_cast<cudaStream_t>(stream));
   if (!st) st = pb2_combine_slots(&c, stream);
   return st;
 }

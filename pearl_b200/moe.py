@@ -306,7 +306,9 @@ def gated_experts(x, w, w_scales, out, slot_indices, routing_offsets, topk_weigh
     ``smooth_scale`` (1, inner) or (inner,) float32.  ``workspace`` (uint8,
     get_gated_experts_workspace_bytes) is taken from torch's allocator when
     not given.  Before they are added up the slots' products are float32 where
-    they fit in 32 MB, else rounded to out's type."""
+    they fit in 32 MB, else rounded to out's type.  Slots past the last
+    expert's end (ids outside 0..E-1, an expert that another GPU holds) add
+    nothing to out."""
     if w.dim() != 3 or topk_weights.dim() != 2:
         _fail("w must be 3-D (num_experts, hidden, inner) and topk_weights 2D (m, top_k)")
     experts, hidden, inner = w.shape

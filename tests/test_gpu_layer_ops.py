@@ -473,6 +473,36 @@ def test_gated_experts_is_its_three_steps(m, E, k, hidden, inner, dtype, residua
     within(out, total, mag * (HALF_ULP[kept] * 1.01 + 2.0 ** -19) + k * 2.0 ** -25, dtype)
 
 
+@pytest.mark.parametrize("m,E,k,hidden,inner,dtype", [
+    (1, 4, 1, 64, 32, BF16), (1, 8, 2, 4096, 2048, F16), (3, 60, 4, 2041, 1360, F16), (300, 8, 2, 1000, 528, BF16),
+    (700, 200, 8, 136, 272, F16), (1500, 8, 6, 1024, 64, BF16)])
+@pytest.mark.parametrize("elsewhere", ["some", "all"])
+@pytest.mark.parametrize("residual", [False, True])
+def test_gated_experts_slots_of_no_expert_count_nothing(m, E, k, hidden, inner, dtype, elsewhere, residual):
+    """Ids outside 0..E-1 (an expert that another GPU holds) sort past the last
+    expert's end; whatever the workspace and those rows of x hold is not used."""
+    g = gen(m + hidden + 1)
+    w, ids = route(randn(g, m, E), k)
+    away = torch.rand(m, k, generator=g, device="cuda") < 0.6 if elsewhere == "some" else torch.ones(m, k, device="cuda") > 0
+    ids = torch.where(away, torch.where(torch.rand(m, k, generator=g, device="cuda") < 0.5, -1, 255), ids).int()
+    slots = m * k
+    data, slot, ends = (torch.empty(s, dtype=torch.int32, device="cuda") for s in (slots, slots, E))
+    scratch = torch.empty(pg.moe.get_build_routing_data_scratchpad_bytes(slots), dtype=torch.uint8, device="cuda")
+    pg.moe.build_routing_data(ids, data, slot, ends, scratch, E)
+    x = randn(g, slots, 2 * inner).to(dtype)
+    W, ws = int8(g, E, hidden, inner), (torch.rand(E, hidden, generator=g, device="cuda") + 0.5) * 1e-3
+    r = randn(g, m, hidden).to(dtype) if residual else None
+    space = torch.full((pg.moe.get_gated_experts_workspace_bytes(slots, inner, hidden),), 255, dtype=torch.uint8, device="cuda")
+    out, want = (torch.empty(m, hidden, dtype=dtype, device="cuda") for _ in range(2))
+    dirty = torch.where(away.view(-1, 1), float("nan"), x)
+    pg.moe.gated_experts(dirty, W, ws, out, slot, ends, w, residual=r, workspace=space)
+    # the same slots with an expert of their own (any) and no weight
+    home = torch.where(away, 0, ids)
+    pg.moe.build_routing_data(home, data, slot, ends, scratch, E)
+    pg.moe.gated_experts(x, W, ws, want, slot, ends, torch.where(away, 0.0, w), residual=r)
+    assert torch.equal(out, want)
+
+
 @pytest.mark.parametrize("m,E,k,hidden,inner", [(8, 8, 2, 4096, 2048), (2, 8, 2, 512, 4096), (900, 64, 4, 512, 768), (1500, 4, 2, 1024, 512)])
 def test_gated_experts_back_to_back(m, E, k, hidden, inner):
     """Calls queued one behind the other, each with inputs written just before

@@ -45,11 +45,11 @@ def _half_type(t, name: str) -> int:
     return _TYPES[t.dtype]
 
 
-def _sync_word(sync) -> int:
+def _sync_word(sync, index: int) -> int:
     if sync is None:
         return 0
-    if not sync.is_cuda or sync.numel() != _lib.HOST_SIGNAL_SYNC_SIZE:
-        _fail(f"host_signal_sync must be a {_lib.HOST_SIGNAL_SYNC_SIZE}-byte CUDA buffer")
+    if sync.get_device() != index or sync.numel() != _lib.HOST_SIGNAL_SYNC_SIZE or not sync.is_contiguous():
+        _fail(f"host_signal_sync must be a contiguous {_lib.HOST_SIGNAL_SYNC_SIZE}-byte buffer on cuda:{index}")
     return sync.data_ptr()
 
 
@@ -78,7 +78,7 @@ def gemm_epilogue(A, B, A_scales, B_scales, C, *, bias=None, activation: str = "
         0 if bias is None else _operand(bias, "bias", (n,), (C.dtype, torch.float32), at),
         0 if bias is None else _TYPES[bias.dtype], _activation(activation),
         0 if residual is None else _operand(residual, "residual", (m, n), (C.dtype,), at),
-        _sync_word(host_signal_sync)), "gemm_epilogue")
+        _sync_word(host_signal_sync, at)), "gemm_epilogue")
 
 
 __all__ = ["ACTIVATIONS", "gemm_epilogue"]

@@ -266,7 +266,7 @@ def gemm_grouped(A, B, A_scales, B_scales, C, routing_offsets, *, c_row_index=No
         _operand(C, "C", (rows, n), tuple(_TYPES), at), _TYPES[C.dtype], experts,
         _operand(routing_offsets, "routing_offsets", (experts,), _INT32, at),
         0 if c_row_index is None else _operand(c_row_index, "c_row_index", (m,), _INT32, at), rows,
-        _sync_word(host_signal_sync)), "gemm_grouped")
+        _sync_word(host_signal_sync, at)), "gemm_grouped")
 
 
 def combine_slots(slots, topk_weights, out, *, residual=None) -> None:
@@ -326,8 +326,9 @@ def gated_experts(x, w, w_scales, out, slot_indices, routing_offsets, topk_weigh
     need = get_gated_experts_workspace_bytes(slots, inner, hidden)
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
-    elif workspace.get_device() != at or workspace.dtype != torch.uint8 or workspace.numel() < need:
-        _fail(f"workspace must be a uint8 tensor on {x.device} of at least {need} bytes")
+    elif (workspace.get_device() != at or workspace.dtype != torch.uint8 or workspace.numel() < need
+          or not workspace.is_contiguous()):
+        _fail(f"workspace must be a contiguous uint8 tensor on {x.device} of at least {need} bytes")
     _call_on(at, "pb2_gated_experts", _PACK_EXPERTS(
         at, _operand(x, "x", (slots, 2 * inner), (x.dtype,), at), half, m, top_k, experts, inner, hidden,
         _activation(activation),
@@ -340,4 +341,4 @@ def gated_experts(x, w, w_scales, out, slot_indices, routing_offsets, topk_weigh
         _operand(topk_weights, "topk_weights", (m, top_k), _FLOAT, at),
         0 if residual is None else _operand(residual, "residual", (m, hidden), (x.dtype,), at),
         _operand(out, "out", (m, hidden), (x.dtype,), at), workspace.data_ptr(), workspace.numel(),
-        _sync_word(host_signal_sync)), "gated_experts")
+        _sync_word(host_signal_sync, at)), "gated_experts")

@@ -503,6 +503,22 @@ def test_gated_experts_slots_of_no_expert_count_nothing(m, E, k, hidden, inner, 
     assert torch.equal(out, want)
 
 
+def test_gated_experts_refuses_workspaces_without_their_bytes():
+    x, w, ws = torch.zeros(8, 64, dtype=BF16, device="cuda"), torch.zeros(2, 8, 32, dtype=torch.int8, device="cuda"), torch.ones(2, 8, device="cuda")
+    out, weights = torch.zeros(4, 8, dtype=BF16, device="cuda"), torch.ones(4, 2, device="cuda")
+    slot, ends = torch.arange(8, dtype=torch.int32, device="cuda"), torch.tensor([4, 8], dtype=torch.int32, device="cuda")
+    need = pg.moe.get_gated_experts_workspace_bytes(8, 32, 8)
+    one = torch.zeros(1, dtype=torch.uint8, device="cuda")
+    for space in (one.expand(need), torch.zeros(need - 1, dtype=torch.uint8, device="cuda"),
+                  torch.zeros(need, dtype=torch.int8, device="cuda"), torch.zeros(need, dtype=torch.uint8)):
+        with pytest.raises(RuntimeError, match="workspace must be"):
+            pg.moe.gated_experts(x, w, ws, out, slot, ends, weights, workspace=space)
+    word = torch.zeros(1, dtype=torch.int8, device="cuda")
+    for sync in (word.expand(pg._lib.HOST_SIGNAL_SYNC_SIZE), torch.zeros(pg._lib.HOST_SIGNAL_SYNC_SIZE, dtype=torch.int8), word):
+        with pytest.raises(RuntimeError, match="host_signal_sync must be"):
+            pg.moe.gated_experts(x, w, ws, out, slot, ends, weights, host_signal_sync=sync)
+
+
 @pytest.mark.parametrize("m,E,k,hidden,inner", [(8, 8, 2, 4096, 2048), (2, 8, 2, 512, 4096), (900, 64, 4, 512, 768), (1500, 4, 2, 1024, 512)])
 def test_gated_experts_back_to_back(m, E, k, hidden, inner):
     """Calls queued one behind the other, each with inputs written just before

@@ -262,6 +262,14 @@ __device__ __forceinline__ uint32_t round4(const float* v, float inv) {
   return __byte_perm(__byte_perm(b0, b1, 0x0040), __byte_perm(b2, b3, 0x0040), 0x5410);
 }
 
+// The larger, NaN if either is: a row that holds a NaN gets it as its scale,
+// so that it does not vanish from what the row is used for.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 constexpr int kGatedIters = 4;
 constexpr int kGatedThreads = 512;
 
@@ -308,15 +316,15 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : kGatedThreads, kWarpRow ? 4 :
     if (kWarpRow && it * threads >= nvec) break;
     if constexpr (!kKeep) again(it);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[kKeep ? it : 0][i]));
+    for (int i = 0; i < 8; ++i) amax = max_nan(amax, fabsf(v[kKeep ? it : 0][i]));
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  for (int o = 16; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   if constexpr (!kWarpRow) {
     if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x / 32] = amax;
     __syncthreads();
     amax = 0.f;
-    for (int w = 0; w < blockDim.x / 32; ++w) amax = fmaxf(amax, warp_max[w]);
+    for (int w = 0; w < blockDim.x / 32; ++w) amax = max_nan(amax, warp_max[w]);
   }
   const float inv = amax > 0.f ? a.q.max_val / amax : 0.f;
   if (me == 0) a.q.scales[row] = amax * a.q.inv_max_val;

@@ -56,7 +56,8 @@ def _sync_word(sync, index: int) -> int:
 def gemm_epilogue(A, B, A_scales, B_scales, C, *, bias=None, activation: str = "none", residual=None,
                   host_signal_sync=None) -> None:
     """C = act(A_scales * B_scales * (A . B^T) + bias) + residual, written
-    into ``C``: the integer sum exact, the epilogue in float32, one rounding.
+    into ``C``: the integer sum exact (in int32, which any values of k up to
+    131071 fit), the epilogue in float32, one rounding.
 
     A (m, k), B (n, k) int8 with k a multiple of 16; A_scales (m,), B_scales
     (n,) float32; C and ``residual`` (m, n) bfloat16 or float16; ``bias``

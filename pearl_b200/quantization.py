@@ -77,6 +77,8 @@ def quantize_gated(x, xq, xq_scales, *, activation: str = "silu", row_index=None
         xq_scales = amax_row(v) * fl(1 / max_val)
         xq = rint(v * (max_val / amax_row(v))), 0 for a row of zeros
 
+    (a NaN or an infinity in a row makes its scale one)
+
     xq (M, N) int8, xq_scales (M,) or (M, 1) float32.  With ``row_index``
     ((M,) int32) row i of the result is row row_index[i] of x -- a MoE
     layer's slots in expert order -- and an index outside x gives a row of

@@ -362,6 +362,25 @@ def test_quantize_gated(rows, n, dtype, act, smooth, block, max_val):
     assert torch.equal(q[live], q2[index[live].long()]) and torch.equal(sc[live, 0], sc2[index[live].long()])
 
 
+@pytest.mark.parametrize("n", [64, 1360, 4096, 20000])  # a warp, a block, a block in registers, in two passes
+@pytest.mark.parametrize("at", ["gate", "up"])
+def test_quantize_gated_keeps_nan_and_infinity(n, at):
+    g = gen(n)
+    x = randn(g, 9, 2 * n).to(BF16)
+    clean = x.clone()
+    column = n - 3 if at == "gate" else 2 * n - 3
+    x[2, column] = float("nan")
+    x[7, column] = float("inf")
+    clean[7, column % n] = clean[7, n + column % n] = 1.0  # a product of the infinity that is not NaN
+    x[7, column % n if at == "up" else n + column % n] = 1.0
+    q, sc, q2, sc2 = (torch.empty(s, dtype=t, device="cuda") for _ in range(2) for s, t in (((9, n), torch.int8), ((9,), F32)))
+    pg.quantization.quantize_gated(x, q, sc)
+    pg.quantization.quantize_gated(clean, q2, sc2)
+    assert sc.isnan().tolist() == [r == 2 for r in range(9)] and sc.isinf().tolist() == [r == 7 for r in range(9)]
+    others = [0, 1, 3, 4, 5, 6, 8]
+    assert torch.equal(q[others], q2[others]) and torch.equal(sc[others], sc2[others])
+
+
 # ------------------------------------------------------- experts' products --
 def routing(g, counts, seed_order=True):
     """(expert ids of the slots shuffled, slot_indices, offsets) with these rows per expert."""

@@ -15,9 +15,9 @@
 // tokens of 128 f32 logits (1.7 TB/s of 6.5).  A warp per token with indices
 // carried through the rounds and all scores computed took 27 us, bare keys
 // 20, no exponentials beside the chosen 16, eight lanes a token 11.4.  4099
-// tokens of 256 experts in 8 groups with a bias: 9.1 us, mostly the latency
-// of one token's chain (sixteen exact sigmoids a lane, four group rounds,
-// eight expert rounds); 4 tokens of 8 experts: 2.1 us.
+// tokens of 256 experts in 8 groups with a bias: 8.4 us, of which one token's
+// chain is 4.4 (eight exact sigmoids a lane, four group rounds, eight expert
+// rounds); 4 tokens of 8 experts: 2.0 us.
 #include <algorithm>
 
 #include "pb2_epilogue.cuh"
@@ -354,13 +354,24 @@ extern "C" int pb2_route_tokens(const pb2_route_params* pp, void* stream) {
   a.renorm = p.renormalize;
   a.scaling = p.scaling;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  // As few lanes a token as the choice allows (a lane per chosen expert): the
-  // rounds' instructions then serve several tokens at once.
-  if (a.top_k <= 8 && a.experts <= 128) {
+  // Many tokens: as few lanes a token as the choice allows (a lane per chosen
+  // expert), whose rounds' instructions then serve several tokens at once.
+  // Few tokens: a warp a token, whose chain is shorter (fewer experts a lane
+  // to score, sort and look up).  8 lanes | 32 lanes, us: 64 experts, top 6,
+  // 2048 tokens 2.64 | 2.53, 4099 2.78 | 3.07, 32768 6.9 | 12.8; 128 experts,
+  // top 8, 512 tokens 3.2 | 2.3, 4099 3.7 | 3.6, 8192 4.9 | 5.7, and with a
+  // bias, which takes every expert's score, 512 5.8 | 3.0, 8192 7.3 | 6.8,
+  // 32768 16 | 19; 256 experts in 16 lanes | 32, 64 tokens 3.5 | 2.4, 32768
+  // 22.8 | 22.1, and with groups and a bias 7.1 | 4.4 and 41 | 38.  (Where it
+  // is off most: a whole softmax over 128 at 9000 tokens, 5.8 | 6.4.)
+  const bool scores = a.bias || (!a.sigmoid && !a.renorm);
+  const int64_t few = int64_t(sm_count(p.device)) * (a.experts <= 64 ? 16 : 32) * (scores ? 2 : 1);
+  if (a.tokens > few && a.top_k <= 8 && a.experts <= 128) {
     if (a.experts <= 32) return launch_route<8, 4>(a, s);
     return a.experts <= 64 ? launch_route<8, 8>(a, s) : launch_route<8, 16>(a, s);
   }
-  if (a.top_k <= 16 && a.experts > 64) return a.experts <= 128 ? launch_route<16, 8>(a, s) : launch_route<16, 16>(a, s);
+  if (a.tokens > few && a.top_k <= 16 && a.experts > 64 && a.experts <= 128) return launch_route<16, 8>(a, s);
+  if (a.experts <= 32) return launch_route<32, 1>(a, s);
   if (a.experts <= 64) return launch_route<32, 2>(a, s);
   return a.experts <= 128 ? launch_route<32, 4>(a, s) : launch_route<32, 8>(a, s);
 }

@@ -309,6 +309,36 @@ def test_route_masked_experts():
     assert ids.tolist() == [[0, 1]]
 
 
+# So many tokens that several share a warp.
+MANY = [(5001, 1, 1, 1, 1), (6001, 8, 2, 1, 1), (5999, 8, 8, 4, 2 + 2), (9001, 31, 5, 1, 1), (9999, 60, 4, 1, 1), (5003, 64, 6, 8, 3),
+        (10007, 72, 4, 6, 5), (12001, 128, 8, 1, 1), (11003, 128, 16, 4, 2), (10001, 100, 12, 1, 1), (10003, 127, 9, 1, 1)]
+
+
+@pytest.mark.parametrize("m,E,k,G,kept", MANY)
+@pytest.mark.parametrize("dtype,scoring", [(F32, "softmax"), (BF16, "sigmoid")])
+def test_route_many_tokens(m, E, k, G, kept, dtype, scoring):
+    test_route_without_bias(m, E, k, G, kept, dtype, scoring)
+    test_route_with_bias(m, E, k, G, kept, scoring)
+
+
+@pytest.mark.parametrize("E,k,G,kept", [(4, 3, 1, 1), (4, 2, 2, 1), (60, 4, 1, 1), (128, 8, 8, 3), (100, 12, 1, 1)])
+@pytest.mark.parametrize("bias", [False, True])
+def test_route_does_not_depend_on_the_number_of_tokens(E, k, G, kept, bias):
+    """A token's experts are the same among many as among few, with masked
+    experts, ties, infinities and NaN; its weights up to the order of sums."""
+    g = gen(E + k)
+    x = (randn(g, 12000, E) * 2).round()
+    x[torch.rand(12000, E, generator=g, device="cuda") < 0.3] = -math.inf
+    x[5::17, 1] = math.nan
+    x[3::19] = -math.inf
+    kw = dict(num_groups=G, topk_groups=kept, bias=(randn(g, E) * 0.2).round(decimals=1) if bias else None, scoring="sigmoid")
+    w, ids = route(x, k, **kw)
+    for at in (0, 4000, 11500):
+        w2, ids2 = route(x[at:at + 500].contiguous(), k, **kw)
+        assert torch.equal(ids[at:at + 500], ids2)
+        torch.testing.assert_close(w[at:at + 500], w2, rtol=2.0 ** -20, atol=0)
+
+
 def test_route_no_tokens():
     w, ids = route(torch.empty(0, 8, device="cuda"), 2)
     assert w.shape == (0, 2)

@@ -208,6 +208,10 @@ __device__ __forceinline__ void cp_async16(void* to, const void* from) {
 }
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
+__device__ __forceinline__ int4 ld_int4(const uint8_t* p) { return *reinterpret_cast<const int4*>(p); }
+__device__ __forceinline__ int4 add4(int4 a, int4 b) { return make_int4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
 // `bytes` of this CTA's shared memory to the same place as `to` in the CTA of
 // cluster rank `peer`, counted on its barrier `bar`.
 __device__ __forceinline__ void copy_to_peer(const void* to, const void* from, uint32_t bytes, const uint64_t* bar, uint32_t peer) {
@@ -765,7 +769,15 @@ __global__ void __launch_bounds__(product_threads(kOnce), kOnce ? 2 : 1) product
       }
       if (et == 0 && live > 0) mbar_arrive_expect_tx(&S.join, (split - 1) * share);
       named_barrier_sync(1, 32 * kEpiWarps);  // S.scale and S.dst are in
-      if (!kGrouped && a.residual) res = load_residual(r0);
+      if (!kGrouped && a.residual) {
+        // The first row's residual, and the others' to L2, from where a load a
+        // row ahead is in time (from HBM a round of four waited 1600 clocks,
+        // 850 now; all of them in registers: 1 to 4% slower where rows are few).
+        res = load_residual(r0);
+        if (cols_in)
+          for (int r = r0 + step; r < live; r += step)
+            prefetch_l2(static_cast<const uint16_t*>(a.residual) + int64_t(S.dst[r]) * a.N + col);
+      }
       const int q = warp & 3, h = (warp - 2) >> 2;
       const bool ok = has && mbar_wait_warp(&S.acc_full[0], 0, abort_flag, a.sync, a.wait_budget, a.wait_hint_ns);
       tc_fence_after();
@@ -802,19 +814,29 @@ __global__ void __launch_bounds__(product_threads(kOnce), kOnce ? 2 : 1) product
       }
     }
     if (cols_in && !*abort_flag) {
-      const int p4 = (lc - range * width) / 4;
+      const int own = range * rows * width * 4;
+      // With 64 columns the upper half of a row's threads take their two pieces
+      // in the other order: eight threads' loads then meet all banks once
+      // (with the ranges' loads in flight together: 256 x 4096 x 14336 with a
+      // residual 19.5 us, 21.0 before both and the prefetch).
+      const int p4 = (lc - range * width) / 4, turn = (p4 >> 3) & 1;
       for (int r = r0; r < live; r += step) {
         const int dst = S.dst[r];
-        int acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        auto add = [&](const uint8_t* sums) {
-          const uint8_t* row = sums + r * width * 4;
-          const int4 x = *reinterpret_cast<const int4*>(row + ((p4 ^ (r & 7)) << 4));
-          const int4 y = *reinterpret_cast<const int4*>(row + (((p4 + 1) ^ (r & 7)) << 4));
-          acc[0] += x.x; acc[1] += x.y; acc[2] += x.z; acc[3] += x.w;
-          acc[4] += y.x; acc[5] += y.y; acc[6] += y.z; acc[7] += y.w;
-        };
-        add(ring + range * rows * width * 4);
-        for (int s = 0; s + 1 < split; ++s) add(received + s * rows * width * 4);
+        const int x_at = r * width * 4 + (((p4 + turn) ^ (r & 7)) << 4), y_at = r * width * 4 + (((p4 + 1 - turn) ^ (r & 7)) << 4);
+        int4 x = ld_int4(ring + own + x_at), y = ld_int4(ring + own + y_at);
+        // split is 2 or 4: the loads of two ranges in flight.
+        const int4 x1 = ld_int4(received + x_at), y1 = ld_int4(received + y_at);
+        if (split == 4) {
+          const uint8_t* more = received + rows * width * 4;
+          const int4 x2 = ld_int4(more + x_at), y2 = ld_int4(more + y_at);
+          const int4 x3 = ld_int4(more + rows * width * 4 + x_at), y3 = ld_int4(more + rows * width * 4 + y_at);
+          x = add4(x, add4(x2, x3));
+          y = add4(y, add4(y2, y3));
+        }
+        x = add4(x, x1);
+        y = add4(y, y1);
+        const int4 lo = turn ? y : x, hi = turn ? x : y;
+        const int acc[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
         const uint4 mine = res;
         if (!kGrouped && a.residual) res = load_residual(r + step);
         if (dst < 0) continue;
@@ -942,7 +964,7 @@ int launch_product(ProductArgs& a, const int8_t* A, const int8_t* B, int cta_row
   a.stages = std::min(kMaxStages, ((half ? kColsSm : 232448) - fixed) / (a.a_bytes + kBRows * kTileK));
   // Whole loads of A in a stage, and with kOnce a tile's sums in the ring.
   if (cta_rows % a.box_rows || cta_rows > kCtaRows || (kPair && cta_rows != kCtaRows) ||
-      (kOnce && (a.split < 2 || kTN % a.split || kTN / a.split < 32 ||
+      (kOnce && ((a.split != 2 && a.split != 4) ||
                  cta_rows * kTN * 4 > a.stages * (a.a_bytes + kBRows * kTileK))))
     return PB2_ERR_UNSUPPORTED_CONFIG;
   a.wait_budget = wait_budget_cycles();

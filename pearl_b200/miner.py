@@ -332,6 +332,9 @@ class PearlLinear:
         scales, gets it in elementwise steps behind it."""
         k, n = x.shape[-1], layer.weight.shape[0]
         m = x.numel() // k
+        if m == 0:
+            _activation(activation)
+            return torch.empty((0, n), dtype=x.dtype, device=x.device)
         mines = self.mining_enabled and self.job is not None and self.config.should_use_noisy_gemm(m, n, k)
         if mines and x.dtype is torch.bfloat16:  # the mined product writes bf16
             _activation(activation)
@@ -557,6 +560,8 @@ def moe_layer(x, router_logits, w1, w1_scale, w2, w2_scale, top_k: int, *, job: 
     weights = torch.empty((m, top_k), dtype=torch.float32, device=device)
     route_tokens(router_logits, weights, ids, **routing)
     mined = None
+    if m == 0:
+        return torch.empty((0, w2.shape[1]), dtype=x.dtype, device=device), None
     if job is not None and x.dtype is torch.bfloat16 and config.should_use_noisy_gemm(m, N, K):
         x_q, x_s, _ = quant_7bit(x, smooth_scale=smooth1)
         h, mined = moe_gemm1(x_q, x_s, ids, w1, w1_scale, job, config)

@@ -162,3 +162,16 @@ def test_apply_fused_mined_takes_the_epilogue_behind_it():
     plain = MN.PearlLinear(True).apply_fused(lay, x, bias=bias, activation="silu", residual=res)
     # the mined product is within the denoising tolerance (0.1 + 1%) of the plain one
     torch.testing.assert_close(got.float(), plain.float(), atol=0.12, rtol=0.02)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_no_tokens(dtype):
+    x, logits, w1, s1, w2, s2, res = layer(3, 4, 8, 256, 128, dtype)
+    out, mined = MN.moe_layer(x[:0], logits[:0], w1, s1, w2, s2, 2, residual=res[:0])
+    assert mined is None and out.shape == (0, w2.shape[1]) and out.dtype is dtype and out.is_cuda
+    lay = Layer()
+    lay.weight, lay.weight_scale = w2[0], s2[0]
+    got = MN.PearlLinear(False).apply_fused(lay, x[:0, :w2.shape[2]], activation="gelu")
+    assert got.shape == (0, w2.shape[1]) and got.dtype is dtype and got.is_cuda
+    with pytest.raises(RuntimeError, match="activation must be"):
+        MN.PearlLinear(False).apply_fused(lay, x[:0, :w2.shape[2]], activation="tanh")

@@ -995,7 +995,7 @@ int launch_product(ProductArgs& a, const int8_t* A, const int8_t* B, int cta_row
 // time, in us: a start and end, and for each K block of a CTA's tiles what a
 // stage of that tile takes.  Fitted to products of 1 to 2048 rows, 300 to
 // 14336 columns and 304 to 16384 of K with weights from HBM; the variant it
-// takes was within 3% of the fastest for all 37 of them.
+// takes was within 5% of the fastest for all 37 of them.
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 int run_linear(ProductArgs& a, const int8_t* A, const int8_t* B, int device, cudaStream_t s) {

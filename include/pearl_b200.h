@@ -606,9 +606,11 @@ PB2_API int pb2_combine_slots(const pb2_combine_params* p, void* stream);
 /* gated_experts: the second half of the experts' MLP in one call:
  * quantize_gated of x (slots = num_tokens * top_k rows in slot order) into
  * expert order (slot_indices), gemm_grouped with w back to slot order,
- * combine_slots.  workspace: pb2_gated_experts_workspace_bytes(slots, inner,
- * hidden) bytes, 16-byte aligned.  Between the last two steps the slots'
- * products are f32 where they fit in 32 MB, else rounded to `type`.  Slots
+ * combine_slots.  workspace: at least pb2_gated_experts_workspace_bytes(
+ * slots, inner, hidden) bytes, 16-byte aligned.  Between the last two steps
+ * the slots' products are f32; in f16 they are rounded to it where they are
+ * over 32 MB.  Products over 32 MB take the columns in two halves, with the
+ * workspace of 2 * hidden columns in one pass, to the same results.  Slots
  * past the last expert's end (an id outside the experts) add nothing. */
 typedef struct pb2_gated_experts_params {
   int device;

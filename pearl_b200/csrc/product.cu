@@ -46,7 +46,7 @@ __host__ __device__ constexpr int received_bytes(int rows, int tile_columns, int
 
 struct ProductArgs {
   CUtensorMap tmA;  // A (rows, K) int8, boxes of box_rows rows
-  CUtensorMap tmB;  // B (groups * N, K) int8
+  CUtensorMap tmB;  // B (N rows every b_rows, K) int8
   const float* sA;
   const float* sB;
   void* C;
@@ -56,6 +56,7 @@ struct ProductArgs {
   int M, N, K;
   int tiles_m, tiles_n;    // of the whole product (tiles_m: without groups)
   int groups;              // 0: one product of M rows
+  int b_rows;              // rows of B and column scales from one group's to the next's
   const int32_t* ends;     // groups: end row of each group
   const int32_t* c_rows;   // optional: row r of the product goes to row c_rows[r] of C
   int c_dst_rows;
@@ -421,7 +422,7 @@ __global__ void __launch_bounds__(product_threads(kOnce), kOnce ? 2 : 1) product
       const Tile w = tile_at<kGrouped>(a, S, t);
       if (leader && ok) {
         const int arow = w.row0 + int(rank) * kCtaRows;
-        const int brow = w.group * a.N + w.tn * kTN + int(rank) * kBRows;
+        const int brow = w.group * a.b_rows + w.tn * kTN + int(rank) * kBRows;
         // Only loads of A with rows of this tile: the rest of the stage keeps
         // what it held, and rows past the tile's are never stored.
         auto boxes_of = [&](int r) {
@@ -574,7 +575,7 @@ __global__ void __launch_bounds__(product_threads(kOnce), kOnce ? 2 : 1) product
       for (int j = 0; j < kCols / 32; ++j) {
         const int c = c0 + 32 * j + lane;
         if (c < a.N) {
-          m.col[j].x = a.sB[int64_t(w.group) * a.N + c];
+          m.col[j].x = a.sB[int64_t(w.group) * a.b_rows + c];
           if (!kGrouped && a.bias_kind)
             m.col[j].y = a.bias_kind == kBiasF32 ? static_cast<const float*>(a.bias)[c] : half_at(a.bias, c, f16);
         }
@@ -743,7 +744,7 @@ __global__ void __launch_bounds__(product_threads(kOnce), kOnce ? 2 : 1) product
 #pragma unroll
       for (int j = 0; j < 8; ++j) sb[j] = bias[j] = 0.f;
       if (cols_in) {
-        const float* p = a.sB + int64_t(w.group) * a.N + col;
+        const float* p = a.sB + int64_t(w.group) * a.b_rows + col;
         if (a.vec) {
           *reinterpret_cast<float4*>(sb) = *reinterpret_cast<const float4*>(p);
           *reinterpret_cast<float4*>(sb + 4) = *reinterpret_cast<const float4*>(p + 4);
@@ -879,7 +880,8 @@ __global__ void __launch_bounds__(product_threads(kOnce), kOnce ? 2 : 1) product
   }
   if constexpr (kGrouped) {
     // Rows of no group (their expert is on another GPU): zeros, 16 bytes a
-    // thread where rows allow it.
+    // thread where rows allow it.  The kernel before may still read them.
+    if (a.early) griddep_wait();
     for (int r = (a.zero_rest ? S.row0[a.groups] : a.M) + int(blockIdx.x); r < a.M; r += int(gridDim.x)) {
       const int dst = a.c_rows ? a.c_rows[r] : r;
       if (uint32_t(dst) >= uint32_t(a.c_dst_rows)) continue;
@@ -955,8 +957,8 @@ int launch_product(ProductArgs& a, const int8_t* A, const int8_t* B, int cta_row
   int st;
   if ((st = make_tmap_2d(&a.tmA, A, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, a.M, kTileK, a.box_rows,
                          CU_TENSOR_MAP_SWIZZLE_128B)) ||
-      (st = make_tmap_2d(&a.tmB, B, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, uint64_t(std::max(a.groups, 1)) * a.N, kTileK,
-                         kBRows, CU_TENSOR_MAP_SWIZZLE_128B)))
+      (st = make_tmap_2d(&a.tmB, B, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.K, uint64_t(std::max(a.groups, 1) - 1) * a.b_rows + a.N,
+                         kTileK, kBRows, CU_TENSOR_MAP_SWIZZLE_128B)))
     return st;
   const int fixed = 1024 + int(sizeof(ProductSmem)) +
                     (kOnce ? received_bytes(cta_rows, kTN, a.split) : epi_warps(false) * kBoxBytes + 4 * kTN * 8);
@@ -1087,6 +1089,7 @@ struct CombineArgs {
   const void* residual;
   void* out;
   int top_k, n, f16, vec;
+  int64_t out_n;  // columns from one row of residual and out to the next
 };
 constexpr int kCombineBatch = 4;
 // Eight columns of a slot.
@@ -1142,7 +1145,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
       add16(e.lo, w);
     }
   };
-  const uint4 res = a.residual ? load8(a.residual, a.vec, t * a.n + col, left) : zero;
+  const uint4 res = a.residual ? load8(a.residual, a.vec, t * a.out_n + col, left) : zero;
   for (int j0 = 0; j0 < a.top_k; j0 += kCombineBatch) {
     Eight r[kCombineBatch];
     float w[kCombineBatch];
@@ -1157,7 +1160,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
       if (w[j] != 0.f) add(r[j], w[j]);  // whatever a slot without weight holds does not count
   }
   if (a.residual) add16(res, 1.0f);
-  uint16_t* o = static_cast<uint16_t*>(a.out) + t * a.n + col;
+  uint16_t* o = static_cast<uint16_t*>(a.out) + t * a.out_n + col;
   if (a.vec) {
     *reinterpret_cast<uint4*>(o) = make_uint4(pack_half2(acc[0], acc[1], f16), pack_half2(acc[2], acc[3], f16),
                                               pack_half2(acc[4], acc[5], f16), pack_half2(acc[6], acc[7], f16));
@@ -1168,13 +1171,22 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
   }
 }
 
-// The type gated_experts keeps the slots' products in between its product and
-// its combination: f32 while they stay in L2 beside what else passes through
-// it, else the output's 16 bits, whose rounding then is as large as the
-// output's own (the error against 64 bits 1.4 times that of one rounding; f32
-// would double the 134 MB each way of 16384 slots of 4096).
-constexpr int64_t kSlotF32Bytes = 32 << 20;
-bool slots_f32(int64_t slots, int64_t hidden) { return slots * hidden * 4 <= kSlotF32Bytes; }
+// Between its product and its combination gated_experts holds the slots'
+// products in f32, so that a result is rounded once: of all columns where the
+// workspace has room for them, else of half of them at a time (as many bytes
+// as 16-bit products of all columns).  2048 tokens of 128 experts, 134 MB of
+// f32: 103 us, in halves 112, with bf16 products 79 and 1.4 times the error
+// against 64 bits; 8192 tokens of 8 wide experts 1038 | 1072 | 1002.
+constexpr int64_t kSlotBytes = 32 << 20;
+bool slots_fit(int64_t slots, int64_t hidden) { return slots * hidden * 4 <= kSlotBytes; }
+int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
+// Workspace of f32 products of `columns` columns, and the least it may be.
+int64_t workspace_bytes(int64_t slots, int64_t inner, int64_t columns) {
+  return round256(slots * inner) + round256(slots * 4) + round256(slots * columns * 4);
+}
+int64_t least_columns(int64_t slots, int64_t hidden) {
+  return slots_fit(slots, hidden) ? hidden : std::min(hidden, ((hidden + 1) / 2 + 7) / 8 * 8);
+}
 
 bool type16(int t) { return t == PB2_TYPE_BF16 || t == PB2_TYPE_F16; }
 
@@ -1208,7 +1220,7 @@ extern "C" int pb2_gemm_epilogue(const pb2_gemm_epilogue_params* pp, void* strea
   a.c_f16 = p.c_type == PB2_TYPE_F16;
   a.act = p.activation;
   a.M = int(p.m);
-  a.N = int(p.n);
+  a.N = a.b_rows = int(p.n);
   a.K = int(p.k);
   a.vec = p.n % 8 == 0 && al16(p.C) && al16(p.residual) && al16(p.B_scales) && al16(p.bias);
   a.sync = static_cast<SignalSync*>(p.host_signal_sync);
@@ -1216,10 +1228,10 @@ extern "C" int pb2_gemm_epilogue(const pb2_gemm_epilogue_params* pp, void* strea
 }
 
 namespace pb2 {
-// `early`, `zero_rest`: see ProductArgs.
-int gemm_grouped(const pb2_gemm_grouped_params& p, bool early, bool zero_rest, cudaStream_t stream) {
+// `b_rows`, `early`, `zero_rest`: see ProductArgs.
+int gemm_grouped(const pb2_gemm_grouped_params& p, int64_t b_rows, bool early, bool zero_rest, cudaStream_t stream) {
   if (p.m < 0 || p.n <= 0 || p.k <= 0 || p.m > INT32_MAX || p.k > INT32_MAX) return PB2_ERR_INVALID_ARGUMENT;
-  if (p.num_experts <= 0 || p.num_experts > kMaxGroups || p.n > INT32_MAX / p.num_experts) return PB2_ERR_INVALID_ARGUMENT;
+  if (p.num_experts <= 0 || p.num_experts > kMaxGroups || b_rows > INT32_MAX / p.num_experts) return PB2_ERR_INVALID_ARGUMENT;
   if (!type16(p.c_type) && p.c_type != PB2_TYPE_F32) return PB2_ERR_INVALID_ARGUMENT;
   if (p.k % 16 != 0) return PB2_ERR_UNSUPPORTED_CONFIG;
   if (p.c_row_index && p.c_rows < 0) return PB2_ERR_INVALID_ARGUMENT;
@@ -1237,12 +1249,13 @@ int gemm_grouped(const pb2_gemm_grouped_params& p, bool early, bool zero_rest, c
   a.c_f32 = p.c_type == PB2_TYPE_F32;
   a.M = int(p.m);
   a.N = int(p.n);
+  a.b_rows = int(b_rows);
   a.K = int(p.k);
   a.groups = int(p.num_experts);
   a.ends = p.routing_offsets;
   a.c_rows = p.c_row_index;
   a.c_dst_rows = int(std::min<int64_t>(p.c_row_index ? p.c_rows : p.m, INT32_MAX));
-  a.vec = p.n % 8 == 0 && al16(p.C) && al16(p.B_scales);
+  a.vec = p.n % 8 == 0 && b_rows % 8 == 0 && al16(p.C) && al16(p.B_scales);
   a.sync = static_cast<SignalSync*>(p.host_signal_sync);
   a.early = early;
   a.zero_rest = zero_rest;
@@ -1253,14 +1266,12 @@ int gemm_grouped(const pb2_gemm_grouped_params& p, bool early, bool zero_rest, c
 extern "C" int pb2_gemm_grouped(const pb2_gemm_grouped_params* pp, void* stream) {
   pb2::NvtxRange nvtx_range("pb2_gemm_grouped");
   if (!pp) return PB2_ERR_INVALID_ARGUMENT;
-  return pb2::gemm_grouped(*pp, false, false, static_cast<cudaStream_t>(stream));
+  return pb2::gemm_grouped(*pp, pp->n, false, false, static_cast<cudaStream_t>(stream));
 }
 
-extern "C" int pb2_combine_slots(const pb2_combine_params* pp, void* stream) {
-  pb2::NvtxRange nvtx_range("pb2_combine_slots");
-  using namespace pb2;
-  if (!pp) return PB2_ERR_INVALID_ARGUMENT;
-  const pb2_combine_params& p = *pp;
+namespace pb2 {
+// `out_n`: see CombineArgs.
+int combine(const pb2_combine_params& p, int64_t out_n, cudaStream_t s) {
   if (p.num_tokens < 0 || p.top_k <= 0 || p.n <= 0 || p.num_tokens > INT32_MAX || p.top_k > INT32_MAX || p.n > INT32_MAX)
     return PB2_ERR_INVALID_ARGUMENT;
   if (!type16(p.type) || (p.slots_type != p.type && p.slots_type != PB2_TYPE_F32)) return PB2_ERR_INVALID_ARGUMENT;
@@ -1279,17 +1290,23 @@ extern "C" int pb2_combine_slots(const pb2_combine_params* pp, void* stream) {
   a.top_k = int(p.top_k);
   a.n = int(p.n);
   a.f16 = p.type == PB2_TYPE_F16;
-  a.vec = p.n % 8 == 0 && al16(p.slots) && al16(p.out) && al16(p.residual);
+  a.out_n = out_n;
+  a.vec = p.n % 8 == 0 && out_n % 8 == 0 && al16(p.slots) && al16(p.out) && al16(p.residual);
   const dim3 grid(unsigned(p.num_tokens), static_cast<unsigned>(across));
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (p.slots_type == PB2_TYPE_F32) return launch_programmatic(combine_kernel<true>, grid, int(threads), 0, s, 1, a);
   return launch_programmatic(combine_kernel<false>, grid, int(threads), 0, s, 1, a);
+}
+}  // namespace pb2
+
+extern "C" int pb2_combine_slots(const pb2_combine_params* pp, void* stream) {
+  pb2::NvtxRange nvtx_range("pb2_combine_slots");
+  if (!pp) return PB2_ERR_INVALID_ARGUMENT;
+  return pb2::combine(*pp, pp->n, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int64_t pb2_gated_experts_workspace_bytes(int64_t slots, int64_t inner, int64_t hidden) {
   if (slots <= 0 || inner <= 0 || hidden <= 0) return 0;
-  auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
-  return up(slots * inner) + up(slots * 4) + up(slots * hidden * (pb2::slots_f32(slots, hidden) ? 4 : 2));
+  return pb2::workspace_bytes(slots, inner, pb2::least_columns(slots, hidden));
 }
 
 extern "C" int pb2_gated_experts(const pb2_gated_experts_params* pp, void* stream) {
@@ -1301,7 +1318,6 @@ extern "C" int pb2_gated_experts(const pb2_gated_experts_params* pp, void* strea
       p.num_tokens > INT32_MAX / p.top_k)
     return PB2_ERR_INVALID_ARGUMENT;
   const int64_t slots = p.num_tokens * p.top_k;
-  auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
   if (slots > 0 && (!p.workspace || !al16(p.workspace) ||
                     p.workspace_bytes < pb2_gated_experts_workspace_bytes(slots, p.inner, p.hidden) || !p.slot_indices))
     return PB2_ERR_INVALID_ARGUMENT;
@@ -1317,21 +1333,19 @@ extern "C" int pb2_gated_experts(const pb2_gated_experts_params* pp, void* strea
   q.row_index = p.slot_indices;
   q.smooth = p.smooth;
   q.xq = reinterpret_cast<int8_t*>(ws);
-  q.scales = reinterpret_cast<float*>(ws + up(slots * p.inner));
+  q.scales = reinterpret_cast<float*>(ws + round256(slots * p.inner));
   q.max_val = p.max_val;
   q.block_size = p.block_size;
   pb2_gemm_grouped_params g;
   std::memset(&g, 0, sizeof(g));
   g.device = p.device;
   g.m = slots;
-  g.n = p.hidden;
   g.k = p.inner;
   g.A = q.xq;
-  g.B = p.w;
   g.A_scales = q.scales;
-  g.B_scales = p.w_scales;
-  g.C = ws + up(slots * p.inner) + up(slots * 4);
-  g.c_type = slots_f32(slots, p.hidden) ? PB2_TYPE_F32 : p.type;
+  g.C = ws + round256(slots * p.inner) + round256(slots * 4);
+  const bool f32 = p.type != PB2_TYPE_F16 || slots_fit(slots, p.hidden);
+  g.c_type = f32 ? PB2_TYPE_F32 : p.type;
   g.num_experts = p.num_experts;
   g.routing_offsets = p.routing_offsets;
   g.c_row_index = p.slot_indices;
@@ -1343,21 +1357,28 @@ extern "C" int pb2_gated_experts(const pb2_gated_experts_params* pp, void* strea
   c.slots = g.C;
   c.slots_type = g.c_type;
   c.topk_weights = p.topk_weights;
-  c.residual = p.residual;
-  c.out = p.out;
   c.type = p.type;
   c.num_tokens = p.num_tokens;
   c.top_k = p.top_k;
-  c.n = p.hidden;
   // The later steps' arguments before any step is queued.
   if (!type16(p.type) || p.num_experts <= 0 || p.num_experts > kMaxGroups || p.hidden > INT32_MAX / p.num_experts ||
       p.inner > INT32_MAX || (slots > 0 && (!p.w || !al16(p.w) || !p.w_scales || !p.routing_offsets || !p.topk_weights || !p.out)))
     return PB2_ERR_INVALID_ARGUMENT;
   if (p.inner % 16 != 0) return PB2_ERR_UNSUPPORTED_CONFIG;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool whole = !f32 || p.workspace_bytes >= workspace_bytes(slots, p.inner, p.hidden);
+  const int64_t step = whole ? p.hidden : least_columns(slots, p.hidden);
   int st = pb2_quantize_gated(&q, stream);
-  // The quantizer writes A and its scales; weights and routing are older.  The
-  // combination reads every slot, also those of no expert.
-  if (!st) st = gemm_grouped(g, true, true, static_cast<cudaStream_t>(stream));
-  if (!st) st = pb2_combine_slots(&c, stream);
+  for (int64_t at = 0; at < p.hidden && !st; at += step) {
+    g.n = c.n = std::min(step, p.hidden - at);
+    g.B = p.w + at * p.inner;
+    g.B_scales = p.w_scales + at;
+    c.residual = p.residual ? static_cast<const uint16_t*>(p.residual) + at : nullptr;
+    c.out = static_cast<uint16_t*>(p.out) + at;
+    // The quantizer writes A and its scales; weights and routing are older.
+    // The combination reads every slot, also those of no expert.
+    st = gemm_grouped(g, p.hidden, true, true, s);
+    if (!st) st = combine(c, p.hidden, s);
+  }
   return st;
 }

@@ -288,9 +288,12 @@ def combine_slots(slots, topk_weights, out, *, residual=None) -> None:
         _operand(out, "out", (m, n), (out.dtype,), at), half, m, top_k, n), "combine_slots")
 
 
-def get_gated_experts_workspace_bytes(slots: int, inner: int, hidden: int) -> int:
-    """Workspace bytes of gated_experts for ``slots`` routed slots."""
-    return int(_lib.load().pb2_gated_experts_workspace_bytes(int(slots), int(inner), int(hidden)))
+def get_gated_experts_workspace_bytes(slots: int, inner: int, hidden: int, one_pass: bool = False) -> int:
+    """Workspace bytes that gated_experts needs for ``slots`` routed slots, or
+    with ``one_pass`` those with which it always takes all columns at once
+    (the least is enough for half of them where their float32 products are
+    over 32 MB; the result is the same)."""
+    return int(_lib.load().pb2_gated_experts_workspace_bytes(int(slots), int(inner), int(hidden) * (2 if one_pass else 1)))
 
 
 def gated_experts(x, w, w_scales, out, slot_indices, routing_offsets, topk_weights, *, residual=None,
@@ -304,9 +307,10 @@ def gated_experts(x, w, w_scales, out, slot_indices, routing_offsets, topk_weigh
     ``routing_offsets`` (E,) are build_routing_data's, ``topk_weights`` (m,
     top_k) route_tokens'.  x, out and ``residual`` are all bf16 or all fp16;
     ``smooth_scale`` (1, inner) or (inner,) float32.  ``workspace`` (uint8,
-    get_gated_experts_workspace_bytes) is taken from torch's allocator when
-    not given.  Before they are added up the slots' products are float32 where
-    they fit in 32 MB, else rounded to out's type.  Slots past the last
+    get_gated_experts_workspace_bytes, for one pass or the least) is taken
+    from torch's allocator, for one pass, when not given.  Before they are
+    added up the slots' products are float32; in fp16 they are rounded to it
+    where they are over 32 MB.  Slots past the last
     expert's end (ids outside 0..E-1, an expert that another GPU holds) add
     nothing to out."""
     if w.dim() != 3 or topk_weights.dim() != 2:
@@ -325,7 +329,8 @@ def gated_experts(x, w, w_scales, out, slot_indices, routing_offsets, topk_weigh
     half = _half_type(x, "x")
     need = get_gated_experts_workspace_bytes(slots, inner, hidden)
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+        workspace = torch.empty(get_gated_experts_workspace_bytes(slots, inner, hidden, one_pass=True), dtype=torch.uint8,
+                                device=x.device)
     elif (workspace.get_device() != at or workspace.dtype != torch.uint8 or workspace.numel() < need
           or not workspace.is_contiguous()):
         _fail(f"workspace must be a contiguous uint8 tensor on {x.device} of at least {need} bytes")

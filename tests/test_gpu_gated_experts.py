@@ -1,0 +1,84 @@
+"""gated_experts where the sizes change how it works: slot products beyond
+32 MB."""
+
+import itertools
+
+import pytest
+import torch
+
+import pearl_b200 as pg
+from tests.test_gpu_layer_ops import BF16, gen, int8, randn, route, within
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    yield
+    torch.cuda.synchronize()
+
+
+def order(ids, E):
+    """(slot_indices, routing_offsets) of these ids."""
+    slots = ids.numel()
+    data, slot, ends = (torch.empty(s, dtype=torch.int32, device="cuda") for s in (slots, slots, E))
+    scratch = torch.empty(pg.moe.get_build_routing_data_scratchpad_bytes(slots), dtype=torch.uint8, device="cuda")
+    pg.moe.build_routing_data(ids, data, slot, ends, scratch, E)
+    return slot, ends
+
+
+def products64(x, W, ws, slot, ends):
+    """Every slot's product in float64 from its quantized row, zeros where no
+    expert has the slot."""
+    slots, inner = x.shape[0], W.shape[2]
+    q, sc = torch.empty(slots, inner, dtype=torch.int8, device="cuda"), torch.empty(slots, device="cuda")
+    pg.quantization.quantize_gated(x, q, sc, row_index=slot)
+    y = torch.zeros(slots, W.shape[1], dtype=torch.float64, device="cuda")
+    for e, (lo, hi) in enumerate(itertools.pairwise([0] + ends.tolist())):
+        y[slot[lo:hi].long()] = (q[lo:hi].double() @ W[e].double().T) * sc[lo:hi, None].double() * ws[e].double()
+    return y
+
+
+def run(x, W, ws, slot, ends, w, residual=None):
+    """The call with a workspace of exactly its bytes, full of NaN; with its
+    own workspace the result is the same."""
+    slots, inner, hidden = x.shape[0], W.shape[2], W.shape[1]
+    space = torch.full((pg.moe.get_gated_experts_workspace_bytes(slots, inner, hidden),), 255, dtype=torch.uint8, device="cuda")
+    out = torch.empty(w.shape[0], hidden, dtype=x.dtype, device="cuda")
+    pg.moe.gated_experts(x, W, ws, out, slot, ends, w, residual=residual, workspace=space)
+    again = torch.empty_like(out)
+    pg.moe.gated_experts(x, W, ws, again, slot, ends, w, residual=residual)
+    assert torch.equal(out.view(torch.int16), again.view(torch.int16))
+    return out
+
+
+# Even and odd numbers of columns, whole and ragged tiles, many slots of few columns.
+LARGE = [(1025, 8, 2, 4096, 64), (2100, 8, 2, 2056, 64), (1100, 64, 8, 1001, 48), (70000, 4, 2, 72, 32), (1100000, 4, 1, 8, 16),
+         (4200000, 2, 2, 1, 16)]
+
+
+@pytest.mark.parametrize("m,E,k,hidden,inner", LARGE)
+@pytest.mark.parametrize("residual", [False, True])
+def test_slot_products_beyond_32_mb_are_rounded_once(m, E, k, hidden, inner, residual):
+    """bf16: the result is the formula's but for one rounding, and a token's
+    does not depend on how many others are in the call."""
+    assert m * k * hidden * 4 > 32 << 20
+    g = gen(m + hidden)
+    w, ids = route(randn(g, m, E), k)
+    slot, ends = order(ids, E)
+    x = randn(g, m * k, 2 * inner).to(BF16)
+    W, ws = int8(g, E, hidden, inner), (torch.rand(E, hidden, generator=g, device="cuda") + 0.5) * 1e-3
+    r = randn(g, m, hidden).to(BF16) if residual else None
+    out = run(x, W, ws, slot, ends, w, r)
+    terms = products64(x, W, ws, slot, ends).view(m, k, hidden) * w.double()[:, :, None]
+    total, mag = terms.sum(1), terms.abs().sum(1)
+    if residual:
+        total, mag = total + r.double(), mag + r.double().abs()
+    # two roundings of a product, one a term and one for the residual, in f32
+    within(out, total, (k + 4) * 2.0 ** -24 * mag, BF16)
+    few = 50
+    slot, ends = order(ids[:few].contiguous(), E)
+    small = run(x[:few * k].contiguous(), W, ws, slot, ends, w[:few].contiguous(), r[:few].contiguous() if residual else None)
+    assert torch.equal(out[:few], small)

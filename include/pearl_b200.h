@@ -608,8 +608,8 @@ PB2_API int pb2_combine_slots(const pb2_combine_params* p, void* stream);
  * expert order (slot_indices), gemm_grouped with w back to slot order,
  * combine_slots.  workspace: at least pb2_gated_experts_workspace_bytes(
  * slots, inner, hidden) bytes, 16-byte aligned.  Between the last two steps
- * the slots' products are f32; in f16 they are rounded to it where they are
- * over 32 MB.  Products over 32 MB take the columns in two halves, with the
+ * the slots' products are f32; in f16, where they are over 32 MB, those that
+ * it holds are rounded to it.  Products over 32 MB take the columns in two halves, with the
  * workspace of 2 * hidden columns in one pass, to the same results.  Slots
  * past the last expert's end (an id outside the experts) add nothing. */
 typedef struct pb2_gated_experts_params {

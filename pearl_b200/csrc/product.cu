@@ -1090,6 +1090,7 @@ struct CombineArgs {
   void* out;
   int top_k, n, f16, vec;
   int64_t out_n;  // columns from one row of residual and out to the next
+  int round_f16;  // f32 slots: rounded to f16 where it holds them
 };
 constexpr int kCombineBatch = 4;
 // Eight columns of a slot.
@@ -1140,7 +1141,14 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
     if constexpr (kSlotF32) {
       const uint32_t x[8] = {e.lo.x, e.lo.y, e.lo.z, e.lo.w, e.hi.x, e.hi.y, e.hi.z, e.hi.w};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j] = fmaf(w, __uint_as_float(x[j]), acc[j]);
+      for (int j = 0; j < 8; ++j) {
+        float v = __uint_as_float(x[j]);
+        if (a.round_f16) {
+          const float h = __half2float(__float2half_rn(v));
+          v = isinf(h) ? v : h;
+        }
+        acc[j] = fmaf(w, v, acc[j]);
+      }
     } else {
       add16(e.lo, w);
     }
@@ -1177,6 +1185,12 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
 // as 16-bit products of all columns).  2048 tokens of 128 experts, 134 MB of
 // f32: 103 us, in halves 112, with bf16 products 79 and 1.4 times the error
 // against 64 bits; 8192 tokens of 8 wide experts 1038 | 1072 | 1002.
+//
+// f16 outputs of more than 32 MB of products keep the values that they have
+// always had, those of gemm_grouped into f16 and combine_slots: each product
+// is rounded to f16's eleven bits before its weight.  Held in f32, one beyond
+// 65504 stays what it is: in f16 it was infinite, and so was its sum, however
+// small its weight.
 constexpr int64_t kSlotBytes = 32 << 20;
 bool slots_fit(int64_t slots, int64_t hidden) { return slots * hidden * 4 <= kSlotBytes; }
 int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
@@ -1270,8 +1284,8 @@ extern "C" int pb2_gemm_grouped(const pb2_gemm_grouped_params* pp, void* stream)
 }
 
 namespace pb2 {
-// `out_n`: see CombineArgs.
-int combine(const pb2_combine_params& p, int64_t out_n, cudaStream_t s) {
+// `out_n`, `round_f16`: see CombineArgs.
+int combine(const pb2_combine_params& p, int64_t out_n, bool round_f16, cudaStream_t s) {
   if (p.num_tokens < 0 || p.top_k <= 0 || p.n <= 0 || p.num_tokens > INT32_MAX || p.top_k > INT32_MAX || p.n > INT32_MAX)
     return PB2_ERR_INVALID_ARGUMENT;
   if (!type16(p.type) || (p.slots_type != p.type && p.slots_type != PB2_TYPE_F32)) return PB2_ERR_INVALID_ARGUMENT;
@@ -1291,6 +1305,7 @@ int combine(const pb2_combine_params& p, int64_t out_n, cudaStream_t s) {
   a.n = int(p.n);
   a.f16 = p.type == PB2_TYPE_F16;
   a.out_n = out_n;
+  a.round_f16 = round_f16;
   a.vec = p.n % 8 == 0 && out_n % 8 == 0 && al16(p.slots) && al16(p.out) && al16(p.residual);
   const dim3 grid(unsigned(p.num_tokens), static_cast<unsigned>(across));
   if (p.slots_type == PB2_TYPE_F32) return launch_programmatic(combine_kernel<true>, grid, int(threads), 0, s, 1, a);
@@ -1301,7 +1316,7 @@ int combine(const pb2_combine_params& p, int64_t out_n, cudaStream_t s) {
 extern "C" int pb2_combine_slots(const pb2_combine_params* pp, void* stream) {
   pb2::NvtxRange nvtx_range("pb2_combine_slots");
   if (!pp) return PB2_ERR_INVALID_ARGUMENT;
-  return pb2::combine(*pp, pp->n, static_cast<cudaStream_t>(stream));
+  return pb2::combine(*pp, pp->n, false, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int64_t pb2_gated_experts_workspace_bytes(int64_t slots, int64_t inner, int64_t hidden) {
@@ -1344,8 +1359,7 @@ extern "C" int pb2_gated_experts(const pb2_gated_experts_params* pp, void* strea
   g.A = q.xq;
   g.A_scales = q.scales;
   g.C = ws + round256(slots * p.inner) + round256(slots * 4);
-  const bool f32 = p.type != PB2_TYPE_F16 || slots_fit(slots, p.hidden);
-  g.c_type = f32 ? PB2_TYPE_F32 : p.type;
+  g.c_type = PB2_TYPE_F32;
   g.num_experts = p.num_experts;
   g.routing_offsets = p.routing_offsets;
   g.c_row_index = p.slot_indices;
@@ -1366,7 +1380,7 @@ extern "C" int pb2_gated_experts(const pb2_gated_experts_params* pp, void* strea
     return PB2_ERR_INVALID_ARGUMENT;
   if (p.inner % 16 != 0) return PB2_ERR_UNSUPPORTED_CONFIG;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool whole = !f32 || p.workspace_bytes >= workspace_bytes(slots, p.inner, p.hidden);
+  const bool whole = p.workspace_bytes >= workspace_bytes(slots, p.inner, p.hidden);
   const int64_t step = whole ? p.hidden : least_columns(slots, p.hidden);
   int st = pb2_quantize_gated(&q, stream);
   for (int64_t at = 0; at < p.hidden && !st; at += step) {
@@ -1378,7 +1392,7 @@ extern "C" int pb2_gated_experts(const pb2_gated_experts_params* pp, void* strea
     // The quantizer writes A and its scales; weights and routing are older.
     // The combination reads every slot, also those of no expert.
     st = gemm_grouped(g, p.hidden, true, true, s);
-    if (!st) st = combine(c, p.hidden, s);
+    if (!st) st = combine(c, p.hidden, p.type == PB2_TYPE_F16 && !slots_fit(slots, p.hidden), s);
   }
   return st;
 }

@@ -309,8 +309,8 @@ def gated_experts(x, w, w_scales, out, slot_indices, routing_offsets, topk_weigh
     ``smooth_scale`` (1, inner) or (inner,) float32.  ``workspace`` (uint8,
     get_gated_experts_workspace_bytes, for one pass or the least) is taken
     from torch's allocator, for one pass, when not given.  Before they are
-    added up the slots' products are float32; in fp16 they are rounded to it
-    where they are over 32 MB.  Slots past the last
+    added up the slots' products are float32; in fp16, where they are over 32
+    MB, those that it holds are rounded to it.  Slots past the last
     expert's end (ids outside 0..E-1, an expert that another GPU holds) add
     nothing to out."""
     if w.dim() != 3 or topk_weights.dim() != 2:

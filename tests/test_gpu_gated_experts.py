@@ -1,5 +1,5 @@
 """gated_experts where the sizes change how it works: slot products beyond
-32 MB."""
+32 MB, and values beyond a 16-bit type's range."""
 
 import itertools
 
@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import pearl_b200 as pg
-from tests.test_gpu_layer_ops import BF16, gen, int8, randn, route, within
+from tests.test_gpu_layer_ops import BF16, F16, gen, int8, randn, route, within
 
 pytestmark = pytest.mark.gpu
 
@@ -82,3 +82,20 @@ def test_slot_products_beyond_32_mb_are_rounded_once(m, E, k, hidden, inner, res
     slot, ends = order(ids[:few].contiguous(), E)
     small = run(x[:few * k].contiguous(), W, ws, slot, ends, w[:few].contiguous(), r[:few].contiguous() if residual else None)
     assert torch.equal(out[:few], small)
+
+
+@pytest.mark.parametrize("m,E,k,hidden,inner", [(40, 8, 2, 2056, 64), (2100, 8, 2, 2056, 64), (1100, 64, 8, 1001, 48)])
+def test_f16_slot_products_beyond_its_range(m, E, k, hidden, inner):
+    """Products of 10^5 and more whose weighted sum f16 does hold."""
+    g = gen(m + inner)
+    w, ids = route(randn(g, m, E), k, scaling=0.05)
+    slot, ends = order(ids, E)
+    x = randn(g, m * k, 2 * inner).to(F16)
+    W, ws = int8(g, E, hidden, inner), (torch.rand(E, hidden, generator=g, device="cuda") + 0.5) * 150
+    out = run(x, W, ws, slot, ends, w)
+    y = products64(x, W, ws, slot, ends)
+    terms = y.view(m, k, hidden) * w.double()[:, :, None]
+    total, mag = terms.sum(1), terms.abs().sum(1)
+    assert float(y.abs().max()) > 2 * 65504 and float(total.abs().max()) < 60000
+    # at most one rounding of each product to f16's eleven bits before the sum
+    within(out, total, mag * (2.0 ** -11 * 1.01 + (k + 4) * 2.0 ** -24) + k * 2.0 ** -25, F16)

@@ -41,9 +41,16 @@ __device__ __forceinline__ float normal_cdf(float x) {
   return x < 0.0f ? tail : 1.0f - tail;
 }
 
+// The larger, NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 template <int kAct>
 __device__ __forceinline__ float activate(float x) {
-  if constexpr (kAct == PB2_ACT_RELU) return fmaxf(x, 0.0f);
+  if constexpr (kAct == PB2_ACT_RELU) return max_nan(x, 0.0f);  // a NaN stays one, as in the other activations
   if constexpr (kAct == PB2_ACT_SILU) return x * sigmoid_fast(x);
   if constexpr (kAct == PB2_ACT_GELU) return x * normal_cdf(x);
   // 0.5 (1 + tanh u) = sigmoid(2 u)

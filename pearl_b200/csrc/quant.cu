@@ -262,17 +262,12 @@ __device__ __forceinline__ uint32_t round4(const float* v, float inv) {
   return __byte_perm(__byte_perm(b0, b1, 0x0040), __byte_perm(b2, b3, 0x0040), 0x5410);
 }
 
-// The larger, NaN if either is: a row that holds a NaN gets it as its scale,
-// so that it does not vanish from what the row is used for.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 constexpr int kGatedIters = 4;
 constexpr int kGatedThreads = 512;
 
+// The row's maximum takes NaN along (max_nan): a row that holds one gets it as
+// its scale, so that it does not vanish from what the row is used for.
+//
 // kWarpRow: a warp per row, else a block per row.  kKeep: the row's products
 // fit in the registers (kGatedIters vectors a thread), else both passes
 // compute them.

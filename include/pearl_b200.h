@@ -544,7 +544,9 @@ PB2_API int pb2_gemm_epilogue(const pb2_gemm_epilogue_params* p, void* stream);
  *   v = act(g) * u, Hadamard transform of width block_size (as pb2_quantize,
  *   0 = none), times smooth (n), in f32;
  *   scales[i] = max|v| * fl(1 / max_val), xq = rint(v * (max_val / max|v|))
- *   clamped to +-max_val (0 for a row of zeros).
+ *   clamped to +-max_val (0 for a row of zeros); a NaN or an infinity in
+ *   the row makes its scale one, and its bytes are then 0, but +-max_val for
+ *   the infinite values of a row without NaN.
  * x_rows is the number of rows of x; an index outside it gives a row of
  * zeros.  n % 8 == 0, x and smooth 16-byte and xq 8-byte aligned. */
 typedef struct pb2_gated_quant_params {

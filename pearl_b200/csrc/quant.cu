@@ -262,6 +262,20 @@ __device__ __forceinline__ uint32_t round4(const float* v, float inv) {
   return __byte_perm(__byte_perm(b0, b1, 0x0040), __byte_perm(b2, b3, 0x0040), 0x5410);
 }
 
+// Rows whose maximum has no finite factor max_val / maximum, or a useless one.
+// Below 2^-64 (the factor overflows below 2^-121) products and maximum are
+// taken 2^64 times as large, exactly; an infinite maximum leaves +-1 for the
+// infinite products, which is what the formula tends to, and 0 for the others.
+constexpr float kTiny = 0x1p-64f, kLift = 0x1p64f;
+__device__ __forceinline__ bool extreme(float amax) { return amax != 0.f && !(amax >= kTiny && amax < INFINITY); }
+__device__ __forceinline__ float extreme_factor(float max_val, float amax) {
+  return amax < kTiny ? max_val / (amax * kLift) : amax > 0.f ? max_val : 0.f;  // 0 for NaN
+}
+__device__ __forceinline__ void settle_extreme(float* v, float amax) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = amax < kTiny ? v[i] * kLift : isinf(v[i]) ? copysignf(1.f, v[i]) : 0.f;
+}
+
 constexpr int kGatedIters = 4;
 constexpr int kGatedThreads = 512;
 
@@ -321,13 +335,22 @@ __global__ void __launch_bounds__(kWarpRow ? 256 : kGatedThreads, kWarpRow ? 4 :
     amax = 0.f;
     for (int w = 0; w < blockDim.x / 32; ++w) amax = max_nan(amax, warp_max[w]);
   }
-  const float inv = amax > 0.f ? a.q.max_val / amax : 0.f;
+  float inv = amax > 0.f ? a.q.max_val / amax : 0.f;
+  const bool odd = extreme(amax);
+  if (odd) {
+    inv = extreme_factor(a.q.max_val, amax);
+    if constexpr (kKeep) {
+#pragma unroll
+      for (int it = 0; it < kGatedIters; ++it) settle_extreme(v[it], amax);
+    }
+  }
   if (me == 0) a.q.scales[row] = amax * a.q.inv_max_val;
 #pragma unroll
   for (int it = 0; it < iters; ++it) {
     const int vec = it * threads + me;
     if constexpr (!kKeep) again(it);
-    const float* w = v[kKeep ? it : 0];
+    float* w = v[kKeep ? it : 0];
+    if (!kKeep && odd) settle_extreme(w, amax);
     if (vec < nvec)
       *reinterpret_cast<uint2*>(a.q.xq + row * a.q.n + 8 * vec) = make_uint2(round4(w, inv), round4(w + 4, inv));
   }

@@ -77,7 +77,9 @@ def quantize_gated(x, xq, xq_scales, *, activation: str = "silu", row_index=None
         xq_scales = amax_row(v) * fl(1 / max_val)
         xq = rint(v * (max_val / amax_row(v))), 0 for a row of zeros
 
-    (a NaN or an infinity in a row makes its scale one)
+    A NaN or an infinity in a row makes its scale one; the bytes of a row with
+    an infinity are +-max_val where it is infinite and 0 elsewhere, those of a
+    row with a NaN all 0.
 
     xq (M, N) int8, xq_scales (M,) or (M, 1) float32.  With ``row_index``
     ((M,) int32) row i of the result is row row_index[i] of x -- a MoE

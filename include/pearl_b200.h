@@ -161,7 +161,8 @@ PB2_API int pb2_commitment_hash_from_merkle_roots(const pb2_commitment_params* p
  * 40-166): for the (num_tokens, top_k) int32 expert ids, slot_indices = flat
  * slot indices stably sorted by expert id (8-bit ids, num_experts <= 256),
  * routing_data = slot_indices / top_k, routing_offsets[e] = number of slots
- * with expert id <= e.  scratchpad: at least
+ * with expert id in 0..e.  Slots of other ids than 0..num_experts-1 come after
+ * all of these.  scratchpad: at least
  * pb2_build_routing_data_scratchpad_bytes(num_tokens * top_k) bytes, 4-byte
  * aligned. */
 typedef struct pb2_routing_params {
@@ -613,7 +614,7 @@ PB2_API int pb2_combine_slots(const pb2_combine_params* p, void* stream);
  * the slots' products are f32; in f16, where they are over 32 MB, those that
  * it holds are rounded to it.  Products over 32 MB take the columns in two halves, with the
  * workspace of 2 * hidden columns in one pass, to the same results.  Slots
- * past the last expert's end (an id outside the experts) add nothing. */
+ * past the last expert's end (ids outside 0..num_experts-1) add nothing. */
 typedef struct pb2_gated_experts_params {
   int device;
   const void* x; /* (slots, 2 inner) of type */

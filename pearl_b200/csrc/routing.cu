@@ -5,10 +5,12 @@
 // For the (m, top_k) expert ids, slot_indices lists the flat slot indices
 // stably sorted by expert id (8-bit keys), routing_data = slot_indices /
 // top_k (the token of each slot), and routing_offsets[e] = the number of
-// slots whose expert id is <= e (exclusive segment ends).
+// slots whose expert id is <= e (exclusive segment ends).  Ids that are no
+// 8-bit number go past all experts: to the last key, or with 256 experts to
+// one more.  (Their low byte alone would put them among an expert's slots.)
 //
 // A stable counting sort in three launches over blocks of 8192 slots:
-// per-block 256-bin histograms (shared-memory atomics), one CTA that turns
+// per-block 257-bin histograms (shared-memory atomics), one CTA that turns
 // them into each block's first output position per bin (bin-major scan, which
 // is what makes the sort stable across blocks), and a scatter in which every
 // block walks its slots in index order, 1024 at a time: __match_any_sync
@@ -20,7 +22,8 @@
 namespace pb2 {
 namespace {
 
-constexpr int kBins = 256;
+constexpr int kMaxExperts = 256;
+constexpr int kBins = kMaxExperts + 1;
 constexpr int kSortThreads = 1024;
 constexpr int kSlotsPerThread = 8;
 constexpr int kBlockSlots = kSortThreads * kSlotsPerThread;
@@ -34,6 +37,10 @@ struct RoutingArgs {
   int numel, top_k, num_experts, blocks;
 };
 
+__device__ __forceinline__ int key_of(const RoutingArgs& a, int id) {
+  return uint32_t(id) < uint32_t(kMaxExperts) ? id : a.num_experts < kMaxExperts ? kMaxExperts - 1 : kMaxExperts;
+}
+
 __global__ void __launch_bounds__(kSortThreads) routing_count_kernel(const RoutingArgs a) {
   __shared__ int32_t hist[kBins];
   const int t = threadIdx.x;
@@ -42,7 +49,7 @@ __global__ void __launch_bounds__(kSortThreads) routing_count_kernel(const Routi
   const int first = blockIdx.x * kBlockSlots;
   for (int i = t; i < kBlockSlots; i += kSortThreads) {
     const int idx = first + i;
-    if (idx < a.numel) atomicAdd(&hist[a.ids[idx] & (kBins - 1)], 1);
+    if (idx < a.numel) atomicAdd(&hist[key_of(a, a.ids[idx])], 1);
   }
   __syncthreads();
   if (t < kBins) a.table[blockIdx.x * kBins + t] = hist[t];
@@ -84,7 +91,7 @@ __global__ void __launch_bounds__(kSortThreads) routing_scatter_kernel(const Rou
     __syncthreads();
     const int idx = first + r * kSortThreads + t;  // (warp, lane) order is index order
     const bool valid = idx < a.numel;
-    const int key = valid ? (a.ids[idx] & (kBins - 1)) : -1;
+    const int key = valid ? key_of(a, a.ids[idx]) : -1;
     const unsigned same = __match_any_sync(0xffffffffu, key);
     const int rank = __popc(same & ((1u << lane) - 1u));
     if (valid && lane == __ffs(same) - 1) warp_count[warp][key] = __popc(same);
@@ -123,7 +130,7 @@ extern "C" int pb2_build_routing_data(const pb2_routing_params* pp, void* stream
   if (!pp) return PB2_ERR_INVALID_ARGUMENT;
   const pb2_routing_params& p = *pp;
   if (p.num_tokens < 0 || p.top_k <= 0 || p.num_experts <= 0) return PB2_ERR_INVALID_ARGUMENT;
-  if (p.num_experts > kBins) return PB2_ERR_INVALID_ARGUMENT;  // 8-bit expert ids
+  if (p.num_experts > kMaxExperts) return PB2_ERR_INVALID_ARGUMENT;  // 8-bit expert ids
   const int64_t numel = p.num_tokens * p.top_k;
   if (numel > INT32_MAX) return PB2_ERR_INVALID_ARGUMENT;
   if (!p.routing_offsets || (numel > 0 && (!p.topk_ids || !p.routing_data || !p.slot_indices)))

@@ -36,7 +36,8 @@ def build_routing_data(
     (build_routing_data.cu:127-166): ``slot_indices`` = flat slot indices
     sorted by expert id, ``routing_data`` = their tokens
     (``slot_indices // top_k``), ``routing_offsets[e]`` = exclusive end of
-    expert e's segment."""
+    expert e's segment.  Slots of ids outside 0..num_experts-1 come after the
+    last segment."""
     named = ((topk_ids, "topk_ids"), (routing_data, "routing_data"), (slot_indices, "slot_indices"),
              (routing_offsets, "routing_offsets"), (scratchpad, "scratchpad"))
     for t, name in named:

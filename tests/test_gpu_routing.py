@@ -1,10 +1,11 @@
-"""Routing orders of ids outside the experts."""
+"""The router's scores far below the top logit, and routing orders of ids
+outside the experts."""
 
 import pytest
 import torch
 
 import pearl_b200 as pg
-from tests.test_gpu_layer_ops import BF16, gen, int8, randn, route
+from tests.test_gpu_layer_ops import BF16, F32, gen, int8, randn, route, route64, weights64
 
 pytestmark = pytest.mark.gpu
 
@@ -15,6 +16,22 @@ def _cuda():
         pytest.skip("no CUDA device")
     yield
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("m,E,k", [(300, 8, 8), (300, 60, 32), (300, 256, 32), (9001, 31, 8), (12001, 128, 8)])
+@pytest.mark.parametrize("renormalize", [False, True])
+@pytest.mark.parametrize("bias", [False, True])
+def test_softmax_weights_far_below_the_top(m, E, k, renormalize, bias):
+    """Logits down to 80 below the top, on a grid where differences are exact:
+    a weight is within 2 ulps of f32 for the exponential, 16 half ulps for
+    the sum of up to 256 terms, two divisions and the renormalized sum."""
+    g = gen(m + E)
+    x = (torch.rand(m, E, generator=g, device="cuda") * -80 * 8).round() / 8
+    b = torch.linspace(0, 0.5, E, device="cuda") if bias else None
+    w, ids = route(x, k, bias=b, renormalize=renormalize)
+    _, scores = route64(x, k)
+    want = weights64(scores, ids, renormalize)
+    torch.testing.assert_close(w.double(), want, rtol=2.0 ** -19, atol=2.0 ** -126)
 
 
 @pytest.mark.parametrize("E", [1, 8, 64, 255, 256])

@@ -462,7 +462,7 @@ extern "C" int pb2_quantize_gated(const pb2_gated_quant_params* pp, void* stream
   const pb2_gated_quant_params& p = *pp;
   if (p.m < 0 || p.n <= 0 || p.m > INT32_MAX || p.n > INT32_MAX || p.x_rows < 0 || p.x_rows > INT32_MAX)
     return PB2_ERR_INVALID_ARGUMENT;
-  if (p.m > 0 && (!p.x || !p.xq || !p.scales)) return PB2_ERR_INVALID_ARGUMENT;
+  if (p.m > 0 && ((p.x_rows > 0 && !p.x) || !p.xq || !p.scales)) return PB2_ERR_INVALID_ARGUMENT;
   if (!p.row_index && p.x_rows != p.m) return PB2_ERR_INVALID_ARGUMENT;
   if (p.max_val <= 0 || p.max_val > 127) return PB2_ERR_INVALID_ARGUMENT;
   if (p.x_type != PB2_TYPE_BF16 && p.x_type != PB2_TYPE_F16) return PB2_ERR_INVALID_ARGUMENT;

@@ -63,3 +63,10 @@ def test_rows_with_nan_are_zeros(n):
     q, sc = torch.full((2, n), 99, dtype=torch.int8, device="cuda"), torch.empty(2, device="cuda")
     pg.quantization.quantize_gated(x, q, sc)
     assert sc.isnan().tolist() == [False, True] and not bool(q[1].any()) and bool(q[0].any())
+
+
+def test_every_index_outside_an_empty_x():
+    index = torch.tensor([0, -1, 7], dtype=torch.int32, device="cuda")
+    q, sc = torch.full((3, 64), 99, dtype=torch.int8, device="cuda"), torch.full((3,), 9.0, device="cuda")
+    pg.quantization.quantize_gated(torch.empty(0, 128, dtype=BF16, device="cuda"), q, sc, row_index=index)
+    assert not bool(q.any()) and sc.tolist() == [0.0] * 3

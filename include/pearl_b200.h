@@ -517,8 +517,9 @@ typedef struct pb2_route_params {
 PB2_API int pb2_route_tokens(const pb2_route_params* p, void* stream);
 
 /* gemm_epilogue: C = act(A_scales * B_scales * (A . B^T) + bias) + residual,
- * the sum of products exact in int32, the rest in f32, rounded to C's type
- * once.  A (m,k), B (n,k) int8, 16-byte aligned, k % 16 == 0; any m and n
+ * the sum of products in int32, the rest in f32, rounded to C's type once.
+ * The sum is exact while it fits in int32, which any values do for k up to
+ * 131071; beyond, it wraps where the values let it.  A (m,k), B (n,k) int8, 16-byte aligned, k % 16 == 0; any m and n
  * (rows of C move 16 bytes at a time when n % 8 == 0 and C and residual are
  * 16-byte aligned).  residual may be C.  host_signal_sync (optional, as for
  * pb2_gemm) receives PB2_ERR_DEVICE_TIMEOUT in its error word. */
@@ -572,8 +573,8 @@ PB2_API int pb2_quantize_gated(const pb2_gated_quant_params* p, void* stream);
  *   C[row] = A_scales[row] * B_scales[e] * (A[row] . B[e]^T),
  * written to row c_row_index[row] of C's c_rows rows when the index is given
  * (rows outside are skipped).  Rows past the last expert's end are not
- * written.  num_experts <= 256; C of
- * f32, bf16 or f16; alignment and host_signal_sync as for pb2_gemm_epilogue. */
+ * written.  num_experts <= 256; C of f32, bf16 or f16; range of k, alignment
+ * and host_signal_sync as for pb2_gemm_epilogue. */
 typedef struct pb2_gemm_grouped_params {
   int device;
   int64_t m, n, k;

@@ -57,7 +57,8 @@ def gemm_epilogue(A, B, A_scales, B_scales, C, *, bias=None, activation: str = "
                   host_signal_sync=None) -> None:
     """C = act(A_scales * B_scales * (A . B^T) + bias) + residual, written
     into ``C``: the integer sum exact (in int32, which any values of k up to
-    131071 fit), the epilogue in float32, one rounding.
+    131071 fit; beyond, it wraps where the values let it), the epilogue in
+    float32, one rounding.
 
     A (m, k), B (n, k) int8 with k a multiple of 16; A_scales (m,), B_scales
     (n,) float32; C and ``residual`` (m, n) bfloat16 or float16; ``bias``

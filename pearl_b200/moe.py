@@ -250,7 +250,8 @@ def gemm_grouped(A, B, A_scales, B_scales, C, routing_offsets, *, c_row_index=No
 
     With ``c_row_index`` ((m,) int32, e.g. slot_indices) row i goes to row
     c_row_index[i] of C instead; rows outside C are skipped.  Rows past the
-    last expert's end are not written.  k a multiple of 16, E <= 256."""
+    last expert's end are not written.  k a multiple of 16, E <= 256; sums as in
+    gemm_epilogue."""
     if A.dim() != 2 or B.dim() != 3 or C.dim() != 2:
         _fail("A and C must be 2-D and B 3-D (num_experts, n, k)")
     m, k = A.shape

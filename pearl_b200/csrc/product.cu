@@ -912,10 +912,10 @@ __global__ void __launch_bounds__(product_threads(kOnce), kOnce ? 2 : 1) product
 // ------------------------------------------------------------------ host
 bool al16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-// CTA pairs that can be resident at once (SM pairs of one GPC).
-int resident_pairs(int device, const void* kern, int smem) {
-  static int cached[64] = {0};
-  int& n = cached[device & 63];
+// CTA pairs of this kernel that can be resident at once (SM pairs of one GPC).
+// Asked once a device and kernel; threads that ask together get the same.
+int resident_pairs(std::atomic<int>& cached, int device, const void* kern, int smem) {
+  int n = cached.load(std::memory_order_relaxed);
   if (n == 0) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2, 1, 1);
@@ -934,6 +934,7 @@ int resident_pairs(int device, const void* kern, int smem) {
       clusters = std::max(1, sm_count(device) / 2);
     }
     n = clusters;
+    cached.store(n, std::memory_order_relaxed);
   }
   return n;
 }
@@ -944,7 +945,7 @@ int resident_pairs(int device, const void* kern, int smem) {
 // 64 x 4096 x 14336 in ranges of 28 blocks 18.6, 16.4 with a full ring: taken
 // when sums were still loaded from their CTAs).  Tiles of more than 32 rows
 // leave such a ring too few stages beside the sums they receive.
-constexpr int kColsSm = 115712;
+constexpr int kHalfSm = 115712;
 
 template <bool kPair, int kTN, bool kGrouped, bool kOnce>
 int launch_product(ProductArgs& a, const int8_t* A, const int8_t* B, int cta_rows, int device, cudaStream_t s) {
@@ -963,7 +964,7 @@ int launch_product(ProductArgs& a, const int8_t* A, const int8_t* B, int cta_row
   const int fixed = 1024 + int(sizeof(ProductSmem)) +
                     (kOnce ? received_bytes(cta_rows, kTN, a.split) : epi_warps(false) * kBoxBytes + 4 * kTN * 8);
   const bool half = kOnce && cta_rows <= 32 && (a.K + kTileK - 1) / kTileK <= 8 * a.split;
-  a.stages = std::min(kMaxStages, ((half ? kColsSm : 232448) - fixed) / (a.a_bytes + kBRows * kTileK));
+  a.stages = std::min(kMaxStages, ((half ? kHalfSm : 232448) - fixed) / (a.a_bytes + kBRows * kTileK));
   // Whole loads of A in a stage, and with kOnce a tile's sums in the ring.
   if (cta_rows % a.box_rows || cta_rows > kCtaRows || (kPair && cta_rows != kCtaRows) ||
       (kOnce && ((a.split != 2 && a.split != 4) ||
@@ -985,7 +986,8 @@ int launch_product(ProductArgs& a, const int8_t* A, const int8_t* B, int cta_row
   int64_t clusters = tiles_m * a.tiles_n;
   if (clusters > INT32_MAX / 8) return PB2_ERR_INVALID_ARGUMENT;
   if (!kOnce) {
-    const int most = kPair ? resident_pairs(device, reinterpret_cast<const void*>(kern), smem)
+    static std::atomic<int> pairs[64];
+    const int most = kPair ? resident_pairs(pairs[device & 63], device, reinterpret_cast<const void*>(kern), smem)
                            : std::max(1, sm_count(device));
     clusters = std::min<int64_t>(clusters, most);
   }

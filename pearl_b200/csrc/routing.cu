@@ -16,14 +16,16 @@
 // block walks its slots in index order, 1024 at a time: __match_any_sync
 // ranks equal keys inside a warp and a per-bin prefix over the 32 warps ranks
 // them across the warps of the round.  The scratch holds the block x bin
-// table (4 bytes each).
+// table (4 bytes each) without the bin past 256 experts, whose place in a
+// block's output follows from the others.
 #include "pb2_common.cuh"
 
 namespace pb2 {
 namespace {
 
 constexpr int kMaxExperts = 256;
-constexpr int kBins = kMaxExperts + 1;
+constexpr int kBins = kMaxExperts;  // of the table
+constexpr int kCounts = kBins + 1;  // of a block's counts: with the ids past 256 experts
 constexpr int kSortThreads = 1024;
 constexpr int kSlotsPerThread = 8;
 constexpr int kBlockSlots = kSortThreads * kSlotsPerThread;
@@ -42,9 +44,9 @@ __device__ __forceinline__ int key_of(const RoutingArgs& a, int id) {
 }
 
 __global__ void __launch_bounds__(kSortThreads) routing_count_kernel(const RoutingArgs a) {
-  __shared__ int32_t hist[kBins];
+  __shared__ int32_t hist[kCounts];
   const int t = threadIdx.x;
-  if (t < kBins) hist[t] = 0;
+  if (t < kCounts) hist[t] = 0;
   __syncthreads();
   const int first = blockIdx.x * kBlockSlots;
   for (int i = t; i < kBlockSlots; i += kSortThreads) {
@@ -80,14 +82,22 @@ __global__ void __launch_bounds__(kBins) routing_scan_kernel(const RoutingArgs a
 }
 
 __global__ void __launch_bounds__(kSortThreads) routing_scatter_kernel(const RoutingArgs a) {
-  __shared__ int32_t next[kBins];             // this block's next output slot per bin
-  __shared__ int32_t warp_count[32][kBins];   // per-warp counts, then per-warp starts
+  __shared__ int32_t next[kCounts];            // this block's next output slot per bin
+  __shared__ int32_t warp_count[32][kCounts];  // per-warp counts, then per-warp starts
   const int t = threadIdx.x;
   const int warp = t / 32, lane = t % 32;
-  if (t < kBins) next[t] = a.table[blockIdx.x * kBins + t];
   const int first = blockIdx.x * kBlockSlots;
+  const bool full = a.num_experts == kMaxExperts;
+  if (t < kCounts) next[t] = t < kBins ? a.table[blockIdx.x * kBins + t] : full ? a.offsets[kMaxExperts - 1] + first : 0;
+  if (full) {
+    // Ids of no expert: after all experts' slots, and after those of them in
+    // earlier blocks, which are the earlier slots less the counted ones (how
+    // far each bin has come since the first block).
+    __syncthreads();
+    if (t < kBins) atomicSub(&next[kBins], next[t] - a.table[t]);
+  }
   for (int r = 0; r < kSlotsPerThread; ++r) {
-    for (int i = t; i < 32 * kBins; i += kSortThreads) (&warp_count[0][0])[i] = 0;
+    for (int i = t; i < 32 * kCounts; i += kSortThreads) (&warp_count[0][0])[i] = 0;
     __syncthreads();
     const int idx = first + r * kSortThreads + t;  // (warp, lane) order is index order
     const bool valid = idx < a.numel;
@@ -97,7 +107,7 @@ __global__ void __launch_bounds__(kSortThreads) routing_scatter_kernel(const Rou
     if (valid && lane == __ffs(same) - 1) warp_count[warp][key] = __popc(same);
     __syncthreads();
     int round_total = 0;
-    if (t < kBins) {
+    if (t < kCounts) {
       for (int w = 0; w < 32; ++w) {
         const int c = warp_count[w][t];
         warp_count[w][t] = round_total;
@@ -111,7 +121,7 @@ __global__ void __launch_bounds__(kSortThreads) routing_scatter_kernel(const Rou
       a.routing_data[pos] = idx / a.top_k;
     }
     __syncthreads();
-    if (t < kBins) next[t] += round_total;
+    if (t < kCounts) next[t] += round_total;
   }
 }
 

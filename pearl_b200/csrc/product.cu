@@ -12,11 +12,12 @@
 //
 // What bounds it.  Many rows: the tensor cores under the power cap, and
 // beside them the 32 KB a CTA of a 256 x 256 pair tile loads per K block.
-// 8192 x 14336 x 4096: 314 us in a burst (3.06 POPS), 356 in a long run at
+// 8192 x 14336 x 4096: 304 us in a burst (3.16 POPS), 356 in a long run at
 // 1.32 GHz and 990 W; its MMAs alone 248 and 285, its loads alone 240.  Few
 // rows: the weights' bytes (16 slots over 8 experts of 4096 x 14336: 63.5 us,
 // 6.5 TB/s).  Few rows and few weights: start, join and end, about 5 us
-// (1 x 4096 x 4096: 6.3 us of which the weights are 2.6).
+// (1 x 4096 x 4096: 6.2 us with weights from HBM, whose bytes are 2.6 of them;
+// 5.3 from L2).
 #include <algorithm>
 #include <atomic>
 #include <cstring>
@@ -941,10 +942,10 @@ int resident_pairs(std::atomic<int>& cached, int device, const void* kern, int s
 
 // Shared memory of a CTA that leaves room for another on its SM: for short K
 // ranges, so that the set-up of one product overlaps the end of the one before
-// it (1 x 4096 x 4096 in ranges of 8 blocks 6.7 us, 7.0 with a full ring;
-// 64 x 4096 x 14336 in ranges of 28 blocks 18.6, 16.4 with a full ring: taken
-// when sums were still loaded from their CTAs).  Tiles of more than 32 rows
-// leave such a ring too few stages beside the sums they receive.
+// it (weights from HBM, half an SM | a full ring: 1 x 4096 x 4096 in ranges of
+// 8 blocks 6.2 | 7.4 us, 16 x 2048 x 8192 in ranges of 16 8.4 | 8.2, 32 x 4096
+// x 14336 in ranges of 28 15.5 | 13.7).  Tiles of more than 32 rows leave such
+// a ring too few stages beside the sums they receive.
 constexpr int kHalfSm = 115712;
 
 template <bool kPair, int kTN, bool kGrouped, bool kOnce>
@@ -1017,7 +1018,7 @@ int run_linear(ProductArgs& a, const int8_t* A, const int8_t* B, int device, cud
   };
   // Persistent pairs with tiles of 256 x 256 and 256 x 128 (1024 x 4096 x
   // 4096: 18.7 | 19.5, single CTAs 20.7; 512 x 4096 x 14336: 41 | 28 | 32), or
-  // with 256 x 128 and K in two ranges (256 x 4096 x 14336: 19, unsplit 27,
+  // with 256 x 128 and K in two ranges (256 x 4096 x 14336: 19, unsplit 25,
   // single CTAs with two ranges 21).
   if (m > kCtaRows) {
     offer(7.0 + 0.33 * double(ceil_div(ceil_div(m, 256) * ceil_div(n, 256), pairs) * kblocks), kWide, kCtaRows, 1);
@@ -1026,11 +1027,11 @@ int run_linear(ProductArgs& a, const int8_t* A, const int8_t* B, int device, cud
     if (tiles * 2 <= pairs && kblocks >= 4) offer(7.5 + 0.20 * double(ceil_div(kblocks, 2)), kPairs, kCtaRows, 2);
   }
   // Single CTAs.  Tiles of fewer rows start and end sooner and occupy more
-  // SMs (200 x 2048 x 2048: 7.0 with 32 rows, 8.0 with 128; 200 x 1001 x 1040,
-  // whose odd rows are stored in pieces: 7.4 | 14.5).  K is split over a
+  // SMs (200 x 2048 x 2048: 6.5 with 32 rows, 7.6 with 128; 200 x 1001 x 1040,
+  // whose odd rows are stored in pieces: 6.2 | 14.5).  K is split over a
   // cluster of two or four CTAs (of eight, most have to wait for a second
-  // round) while every one has an SM (1 x 4096 x 4096: 6.3, unsplit 10.7;
-  // 100 x 1000 x 1008 with 32 rows: 5.0 | 5.5; 128 x 300 x 16384: 10.9 | 29).
+  // round) while every one has an SM (1 x 4096 x 4096: 6.2, unsplit 9.0;
+  // 100 x 1000 x 1008 with 32 rows: 4.8 | 5.3; 128 x 300 x 16384: 9.8 | 25).
   for (int rows = 32; rows <= kCtaRows; rows *= 2) {
     const int r = int(std::min<int64_t>(rows, ceil_div(m, 8) * 8));
     const int64_t tiles = ceil_div(m, r) * ceil_div(n, 128);
@@ -1081,9 +1082,10 @@ int run_grouped(ProductArgs& a, const int8_t* A, const int8_t* B, int device, cu
 }
 
 // out[t] = residual[t] + sum_j w[t, j] * slots[t * top_k + j], f32 sums in
-// slot order.  HBM-bound (2 (top_k + 2) bytes a column): a block per token
-// and 256 vectors of eight columns, kCombineBatch slots' loads in flight at a
-// time with the residual's.  8192 tokens of two slots of 4096: 44 us (6.1 TB/s;
+// slot order.  HBM-bound (4 top_k + 4 bytes a column of f32 slots, 2 top_k + 4
+// of 16-bit ones): a block per token and 256 vectors of eight columns,
+// kCombineBatch slots' loads in flight at a time with the residual's.  8192
+// tokens of two slots of 4096: 67 us (6.0 TB/s), of bf16 slots 44 (6.1 TB/s;
 // slot by slot 72, two vectors a thread 72).
 struct CombineArgs {
   const void* slots;

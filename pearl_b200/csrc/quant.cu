@@ -225,8 +225,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) quant_rows_reg_kern
 // registers (kIters vectors of eight a thread) between the max pass and the
 // rounding pass: x is read once and the activation computed once.  Rows of at
 // most 1024 products take a warp each (no block barrier), longer ones a block
-// of just the threads they need.  16384 rows of 14336: 211 us (5.6 TB/s of
-// 6.5; with expf and a division 345); 16384 of 768: 12.6 us (5.0 TB/s; a
+// of just the threads they need.  16384 rows of 14336: 213 us (5.5 TB/s of
+// 6.5; with expf and a division 345); 16384 of 768: 12.8 us (4.9 TB/s; a
 // block per row 25).
 struct GatedArgs {
   QuantArgs q;

@@ -11,13 +11,15 @@
 // bias are taken of the chosen alone, and renormalized softmax weights are a
 // softmax over the chosen, which needs no other exponential.
 //
-// What bounds it is instruction issue, not the logits: 11.4 us for 32768
-// tokens of 128 f32 logits (1.7 TB/s of 6.5).  A warp per token with indices
-// carried through the rounds and all scores computed took 27 us, bare keys
-// 20, no exponentials beside the chosen 16, eight lanes a token 11.4.  4099
-// tokens of 256 experts in 8 groups with a bias: 8.4 us, of which one token's
-// chain is 4.4 (eight exact sigmoids a lane, four group rounds, eight expert
-// rounds); 4 tokens of 8 experts: 2.0 us.
+// 32768 tokens of 128 f32 logits take 12.1 us (1.6 TB/s of 6.5).  An SM at work
+// issues in 61% of its slots, with 7.7 warps a scheduler of which 2.2 could go
+// on; what the others wait for is, in this order, their logits, the integer
+// pipe (minima, maxima and selects, 53% busy), shuffles.  Over the whole launch
+// 44% of the slots: the rest is its start and its last blocks.  A warp per
+// token with indices carried through the rounds and all scores computed took
+// 27 us, bare keys 20, no exponentials beside the chosen 16, eight lanes a
+// token 11.4, the full exponential 12.1.  4099 tokens of 256 experts in 8
+// groups with a bias: 8.2 us; 4 tokens of 8 experts: 1.9 us.
 #include <algorithm>
 
 #include "pb2_epilogue.cuh"
